@@ -31,6 +31,7 @@ extern "C" {
 /* element types */
 #define VS_F16 0
 #define VS_F32 1
+#define VS_BF16 2   /* attention over chosen blocks and the cache only */
 
 /* kernel families: the reference's wmma* entry points map to TENSOR, its cuda* entry points to CUDA_CORE.  CUDA_CORE takes what
  * the cuda* entry points take (V = 1, widths that are multiples of 8 or 4, fp32); its products of fp16 operands with fp16
@@ -267,6 +268,93 @@ int vs_sddmm_host(int path, int in_dtype, int out_dtype, int m_vec, int k, int n
  * device), optionally clearing it.  0 = no kernel ever gave up.
  * ---------------------------------------------------------------------------------------------------- */
 int vs_device_status(int clear, uint32_t *status);
+
+/* ------------------------------------------------------------------------------------------------------
+ * Attention over blocks of 64 keys that the data choose: the choice, the attention, its gradients.  No counterpart in the
+ * reference.  Beside vs_attention_cvse, whose mask is fixed ahead of the call.
+ *
+ * q, grad_out: [batch][queries][heads][d]; k, v: [batch][keys][kv_heads][d]; dtype VS_F16 or VS_BF16; the last dimension contiguous, the other
+ * strides given as three HOST int64 in elements (batch, token, head), multiples of 8 and, where the dimension is larger than one, not 0.
+ * Results are contiguous in the same order.  Device pointers of tensors 16-byte aligned.
+ * heads is a multiple of kv_heads: heads / kv_heads (at most 128) query heads share a head of keys, and its list of blocks.
+ * d: a multiple of 8 up to 128.  keys: up to 1 048 576.
+ * Query i stands at position p = i + keys - queries.  causal != 0 (then queries <= keys): it attends to keys t <= p.
+ * lengths (or NULL): int32 [batch], how many tokens of a padded batch are there (queries == keys); queries behind the end attend to
+ * nothing, keys behind it are not attended to, and what stands there is not looked at.
+ *
+ * vs_select_blocks: for each query and head of keys the blocks to attend to, lists[batch][kv_heads][queries][count], ascending, -1 behind them.
+ *   score(i, j) = (sum of q over the heads of the group) . (mean of the keys of block j), in 64 bits
+ * causal: the query's own block and the count - 1 best of the blocks before it; else the count best.  Equal scores: the lower block; a score
+ * that is no number is the lowest.  workspace: vs_select_blocks_workspace_bytes.
+ *
+ * vs_selected_attention: out = softmax(scale * q k^T) v over the keys of the listed blocks.  A list is a set: order and repetitions do not count,
+ * entries that are no block are passed over.  A query that attends to no key has zeros.  Keys and values that a query does not
+ * attend to do not reach its result, whatever stands there.  lse: float [batch][heads][queries], the base-2 logarithm of the sum of
+ * exp(scale * score), +inf where a query attends to nothing; out_low (or NULL, as out): what the rounding of out left over.  The backward pass
+ * reads lse and, for rowsum(out o grad_out), out and out_low: from the rounded out alone the gradients of q and k would be twice as far off.  scale: finite and above 0.
+ * Scores, their maximum and sum, and all sums over keys are fp32; the weights (at most 256 in magnitude ahead of the division)
+ * are rounded to the type for the product with v, as are they and the scores' gradients in the backward pass.
+ *
+ * vs_selected_attention_backward: gradients of q, k and v (all three written whole) for grad_out; the gradients of a head of keys are summed over its group,
+ * in the same order in every call.  Both take a workspace of vs_selected_attention_workspace_bytes(..., backward).
+ * ---------------------------------------------------------------------------------------------------- */
+int64_t vs_select_blocks_workspace_bytes(int batch, int keys, int kv_heads, int d);
+int vs_select_blocks(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal,
+                     const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const int32_t *lengths,
+                     int32_t *lists, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t vs_selected_attention_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int d, int backward);
+int vs_selected_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal,
+                          const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                          const int64_t *v_strides, const int32_t *lengths, const int32_t *lists, void *out, void *out_low, float *lse,
+                          float scale, void *workspace, int64_t workspace_bytes, void *stream);
+int vs_selected_attention_backward(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal,
+                                   const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                                   const int64_t *v_strides, const int32_t *lengths, const int32_t *lists, const void *out,
+                                   const void *out_low, const float *lse, const void *grad_out, const int64_t *grad_out_strides, void *grad_q, void *grad_k,
+                                   void *grad_v, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * The same for single tokens, over a cache whose complete blocks are held in 8 bits.  No counterpart in the reference.
+ *
+ *   k_codes, v_codes    int8  [pages][kv_heads][64][d]    a block of a sequence is a page
+ *   k_scales, v_scales  float [pages][kv_heads]           value = code * scale
+ *   k_sums              int16 [pages][kv_heads][d]        sum of the codes of a block of keys
+ *   k_ring, v_ring      dtype [tails][kv_heads][128][d]   the newest tokens in 16 bits: token t of a sequence at t % 128, for the tokens
+ *                                                         of its newest complete block and of the block behind it
+ *   table               int32 [sequences][max_blocks]     page of each complete block
+ *   tail_indices        int32 [sequences]                 the sequence's ring
+ *   lengths             int32 [sequences]                 tokens in the cache
+ * d: a multiple of 16 up to 128.  All device pointers, tensors 16-byte aligned.  Sequences of one call have pages and rings of their own; a page or ring
+ * that is not there (an index out of range, a block behind max_blocks) is neither written nor read.
+ *
+ * vs_cache_append: up to `tokens` new tokens for each sequence, counts[r] (NULL: tokens) of them, behind its lengths[r]; k, v
+ * [sequences][tokens][kv_heads][d] with strides as above.  A block whose last token arrives is rounded into its page:
+ * scale = max |x| over its finite values times 1.f / 127, code = round-half-even(x / scale) within +-127, 0 for what is no number.  lengths itself is the
+ * caller's to advance.  Until a block is complete its tokens are in the ring alone, so a sequence may also go back to where it was, as far as
+ * the start of its newest incomplete block.
+ *
+ * vs_cache_select: for each sequence and head of keys the complete blocks that a token's query attends to, lists[sequences][kv_heads][count],
+ * ascending, -1 behind them: the newest complete block and the count - 1 best others by
+ *   score(j) = (sum of q over the heads of the group) . (sum of the block's codes) * scale, in 64 bits.
+ * Ties and what is no number as in vs_select_blocks; q [sequences][heads][d], strides (sequence, head).  max_blocks: up to 16384.
+ *
+ * vs_cache_attention: out [sequences][heads][d] = softmax(scale * q k^T) v over all complete blocks, or the listed ones (lists as vs_cache_select writes them;
+ * a set, as above), and the tokens behind the last complete block.  Zeros for a sequence without tokens.  workspace:
+ * vs_cache_attention_workspace_bytes(..., units) with units = count where there are lists, else max_blocks; may be 0.
+ * ---------------------------------------------------------------------------------------------------- */
+int vs_cache_append(int dtype, int pages, int tails, int kv_heads, int d, int8_t *k_codes, int8_t *v_codes, float *k_scales,
+                    float *v_scales, int16_t *k_sums, void *k_ring, void *v_ring, int sequences, int tokens, const void *k,
+                    const int64_t *k_strides, const void *v, const int64_t *v_strides, const int32_t *table, int max_blocks,
+                    const int32_t *tail_indices, const int32_t *lengths, const int32_t *counts, void *stream);
+int vs_cache_select(int dtype, int pages, int heads, int kv_heads, int d, const float *k_scales, const int16_t *k_sums, int sequences,
+                    const void *q, const int64_t *q_strides, const int32_t *table, int max_blocks, const int32_t *lengths, int count,
+                    int32_t *lists, void *stream);
+int64_t vs_cache_attention_workspace_bytes(int sequences, int heads, int kv_heads, int d, int units);
+int vs_cache_attention(int dtype, int pages, int tails, int heads, int kv_heads, int d, const int8_t *k_codes, const int8_t *v_codes,
+                       const float *k_scales, const float *v_scales, const void *k_ring, const void *v_ring, int sequences,
+                       const void *q, const int64_t *q_strides, const int32_t *table, int max_blocks, const int32_t *tail_indices,
+                       const int32_t *lengths, const int32_t *lists, int count, void *out, float scale, void *workspace,
+                       int64_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------------------------
  * Plan scratch in the caller's hands (no counterpart in the reference, whose kernels keep no workspace:

@@ -1,0 +1,313 @@
+"""Attention over chosen blocks: the choice, the attention and its gradients against plain forms in 64 bits.
+
+Tolerances.  u = finfo.eps / 2 is the largest relative error of one rounding to the type.  A result is a sum over keys of weights (rounded to
+the type: u each) times values (exact), divided in fp32 and rounded (u): within u * (sum of |weight * value| + |result|) and fp32 noise of the
+scores, 2^-20 of the same sums.  A gradient's terms carry the rounding of the weight or of the score's gradient (u), and that of `out` in
+rowsum(out o grad_out) (u of sum |out * grad_out|, as large as |weight| * |grad_out| * |v| terms): 3 u of the sums of magnitudes bounds both, and its own rounding
+adds u of the value."""
+import numpy as np
+import pytest
+import torch
+
+import block_util as plain
+from vectorsparse_b200 import VsError, ops, torch_ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def tensors(B, Lq, Lk, Hq, Hkv, D, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g).to(dtype).to(DEV) for s in ((B, Lq, Hq, D), (B, Lk, Hkv, D), (B, Lk, Hkv, D), (B, Lq, Hq, D))]
+
+
+def lists(B, Hkv, Lq, Lk, count, seed):
+    """Any lists: unordered, with repetitions, -1 and numbers that are no block."""
+    return torch.from_numpy(np.random.default_rng(seed).integers(-2, -(-Lk // 64) + 2, (B, Hkv, Lq, count)).astype(np.int32)).to(DEV)
+
+
+def magnitudes(q, k, v, blocks, scale, causal, lengths, grad):
+    """Sums of the magnitudes of the terms of out, grad_q, grad_k, grad_v."""
+    (B, Lq, Hq, D), (_, Lk, Hkv, _) = q.shape, k.shape
+    group = Hq // Hkv
+    o, gq, gk, gv = np.zeros_like(q), np.zeros_like(q), np.zeros_like(k), np.zeros_like(v)
+    for b in range(B):
+        for h in range(Hkv):
+            for i in range(Lq):
+                t = plain.named(blocks, b, h, i, Lq, Lk, causal, lengths)
+                if not len(t):
+                    continue
+                rows = slice(h * group, (h + 1) * group)
+                s = q[b, i, rows] @ k[b, t, h].T * scale
+                p = np.exp(s - s.max(1, keepdims=True))
+                p /= p.sum(1, keepdims=True)
+                d = np.abs(grad[b, i, rows])
+                av = np.abs(v[b, t, h])
+                o[b, i, rows] = p @ av
+                dp = d @ av.T
+                ds = p * (dp + (p * dp).sum(1, keepdims=True)) * scale
+                gq[b, i, rows] = ds @ np.abs(k[b, t, h])
+                gk[b, t, h] += ds.T @ np.abs(q[b, i, rows])
+                gv[b, t, h] += p.T @ d
+    return o, gq, gk, gv
+
+
+def check(dtype, q, k, v, blocks, scale, causal, lengths, grad):
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+    out = torch_ops.selected_attention(*leaves, blocks, scale, causal, n)
+    got = (out, *torch.autograd.grad(out, leaves, grad))
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
+    args = [plain.f64(x) for x in (q, k, v)] + [blocks.cpu().numpy(), scale, causal, lengths, plain.f64(grad)]
+    u = torch.finfo(dtype).eps / 2
+    for name, a, b, m in zip(("out", "grad_q", "grad_k", "grad_v"), got, plain.attention(*args), magnitudes(*args)):
+        assert a.dtype == dtype and tuple(a.shape) == b.shape
+        error = np.abs(plain.f64(a) - b)
+        bound = (3 * u + 2.0 ** -18) * m + u * np.abs(b) + 2.0 ** -24   # the last: fp16 below its normal range
+        assert (error <= bound).all(), (name, float((error - bound).max()), float(error.max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,count", [
+    (1, 1, 1, 1, 1, 64, 1), (2, 1, 200, 4, 2, 128, 2), (1, 64, 64, 2, 1, 64, 1), (1, 65, 65, 8, 1, 128, 2), (2, 130, 257, 3, 3, 40, 3), (1, 191, 191, 7, 1, 96, 3),
+    (1, 33, 300, 16, 1, 80, 4), (1, 100, 100, 10, 2, 8, 2), (1, 150, 400, 2, 2, 128, 5), (1, 40, 90, 32, 1, 64, 2), (1, 5, 70, 128, 1, 64, 2), (3, 97, 97, 6, 2, 32, 2)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_and_gradients(dtype, B, Lq, Lk, Hq, Hkv, D, count, causal):
+    q, k, v, grad = tensors(B, Lq, Lk, Hq, Hkv, D, dtype, 7 * Lq + D)
+    check(dtype, q, k, v, lists(B, Hkv, Lq, Lk, count, Lq), D ** -0.5, causal, None, grad)
+
+
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_padded_batches(group):
+    """Whatever stands behind a sequence's end, in every operand, reaches nothing; results there are zeros."""
+    lengths = [150, 1, 64, 0, 129]
+    q, k, v, grad = tensors(5, 150, 150, 2 * group, 2, 64, torch.float16, group)
+    blocks = lists(5, 2, 150, 150, 3, group)
+    for causal in (True, False):
+        check(torch.float16, q, k, v, blocks, 0.125, causal, lengths, grad)
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    want = torch_ops.selected_attention(q, k, v, blocks, 0.125, True, n)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 0.125, True, n), leaves, grad)
+    dirty = [x.clone() for x in (q, k, v, grad)]
+    for x in dirty:
+        for b, m in enumerate(lengths):
+            x[b, m::2], x[b, m + 1::2] = float("nan"), float("inf")
+    leaves = [x.requires_grad_() for x in dirty[:3]]
+    out = torch_ops.selected_attention(*leaves, blocks, 0.125, True, n)
+    again = torch.autograd.grad(out, leaves, dirty[3])
+    assert ops.device_status() == 0
+    for name, a, b in (("out", out, want), *zip(("grad_q", "grad_k", "grad_v"), again, grads)):
+        assert torch.isfinite(a).all(), name
+        for r, m in enumerate(lengths):
+            assert (a[r, m:] == 0).all(), name
+        assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -9, atol=2.0 ** -9), name   # another order of sums where a tile was computed again
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf"), 65504.0])
+def test_masked_keys_reach_nothing(value):
+    """A key or value that a query does not attend to - not listed, or behind it - may be anything."""
+    q, k, v, grad = tensors(1, 192, 192, 4, 1, 64, torch.float16, 3)
+    blocks = torch.zeros((1, 1, 192, 2), dtype=torch.int32, device=DEV)
+    blocks[:, :, 64:, 1] = torch.arange(64, 192, device=DEV) // 64
+    blocks[:, :, 100:, 0] = -1          # of block 1 the queries 64 .. 99 see block 0
+    n, m = 70, 130                      # what a key at 70 reaches: queries 70 .. 127; at 130: 130 ..
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    want = torch_ops.selected_attention(*leaves, blocks, 0.125)
+    grads = torch.autograd.grad(want, leaves, grad)
+    k2, v2 = k.clone(), v.clone()
+    k2[:, n], v2[:, m] = value, value
+    reached = torch.zeros(192, dtype=torch.bool, device=DEV)
+    reached[n:128] = True
+    reached[m:] = True
+    out = torch_ops.selected_attention(q, k2, v2, blocks, 0.125)
+    assert torch.allclose(out[:, ~reached].float(), want[:, ~reached].float(), rtol=2.0 ** -9, atol=2.0 ** -9)
+    leaves = [q.clone().requires_grad_(), k2.requires_grad_(), v2.requires_grad_()]
+    gq, _, _ = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 0.125), leaves, grad)
+    assert torch.allclose(gq[:, ~reached].float(), grads[0][:, ~reached].float(), rtol=2.0 ** -9, atol=2.0 ** -9)
+    # a query and a row of grad_out reach the gradients of the keys that they attend to: here of block 1 alone
+    q2, g2 = q.clone(), grad.clone()
+    q2[:, 110], g2[:, 111] = value, value
+    leaves = [q2.requires_grad_(), k.clone().requires_grad_(), v.clone().requires_grad_()]
+    again = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 0.125), leaves, g2)
+    for i in (1, 2):
+        for block in (slice(0, 64), slice(128, 192)):
+            assert torch.allclose(again[i][:, block].float(), grads[i][:, block].float(), rtol=2.0 ** -8, atol=2.0 ** -8)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale,size", [(0.125, 8.0), (1e-3, 1.0), (3.0, 4.0), (1e-30, 1.0)])
+def test_scores_of_any_size(dtype, scale, size):
+    """Scores that the running maximum has to follow by hundreds, or that are all alike."""
+    q, k, v, _ = tensors(1, 160, 320, 4, 2, 64, dtype, 5)
+    k = k * torch.linspace(0.1, size, 320, device=DEV)[None, :, None, None].to(dtype)
+    blocks = lists(1, 2, 160, 320, 4, 5)
+    got = plain.f64(torch_ops.selected_attention(q, k, v, blocks, scale))
+    args = [plain.f64(x) for x in (q, k, v)] + [blocks.cpu().numpy(), scale, True, None]
+    want = plain.attention(*args)
+    u = torch.finfo(dtype).eps / 2
+    # a score s is off by fp32 noise: its weight by |s| 2^-22, and no score is above |q| |k| scale
+    top = float(np.abs(args[0]).sum(-1).max() * np.abs(args[1]).max() * scale)
+    bound = (3 * u + 2.0 ** -18 + top * 2.0 ** -21) * np.abs(args[2]).max()
+    assert np.abs(got - want).max() <= bound
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,count", [(1, 1, 1, 1, 1, 64, 1), (2, 300, 300, 4, 2, 64, 3), (1, 70, 700, 6, 1, 128, 4), (1, 40, 900, 2, 2, 24, 20),
+                                                    (1, 9, 200, 16, 1, 128, 1), (1, 64, 3000, 2, 1, 8, 5)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_selection(dtype, B, Lq, Lk, Hq, Hkv, D, count, causal):
+    q, k, _, _ = tensors(B, Lq, Lk, Hq, Hkv, D, dtype, Lk)
+    got = torch_ops.select_blocks(q, k, count, causal)
+    assert np.array_equal(got.cpu().numpy(), plain.select(plain.f64(q), plain.f64(k), count, causal, None))
+
+
+def test_selection_of_padded_batches_ties_and_what_is_no_number():
+    lengths = [400, 1, 0, 130]
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    q, k, _, _ = tensors(4, 400, 400, 4, 2, 32, torch.bfloat16, 1)
+    for b, m in enumerate(lengths):
+        q[b, m:], k[b, m:] = float("nan"), float("nan")
+    k[0, 64:128] = k[0, 0:64]                # equal scores: the lower block
+    k[0, 200, 0, 3], k[0, 300, 1, 5] = float("nan"), float("inf")
+    q[0, 399, 0] = 0
+    with np.errstate(all="ignore"):
+        for causal in (True, False):
+            for count in (1, 2, 3, 9):
+                got = torch_ops.select_blocks(q, k, count, causal, n).cpu().numpy()
+                assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), count, causal, lengths)), (causal, count)
+
+
+def test_many_blocks():
+    """Lists over more blocks than one CTA keeps scores for 32, and for 8, queries of."""
+    for keys in (64 * 700 + 5, 64 * 4000):
+        q, k, v, _ = tensors(1, 3, keys, 2, 1, 64, torch.float16, 2)
+        got = torch_ops.select_blocks(q, k, 6)
+        assert np.array_equal(got.cpu().numpy(), plain.select(plain.f64(q), plain.f64(k), 6, True, None))
+        out = torch_ops.selected_attention(q, k, v, got, 0.125)
+        want = plain.attention(plain.f64(q), plain.f64(k), plain.f64(v), got.cpu().numpy(), 0.125, True, None)
+        assert np.abs(plain.f64(out) - want).max() <= 2.0 ** -9
+
+
+def test_layouts():
+    """[B, H, L, D] seen as [B, L, H, D], slices of a wider projection, expanded and misaligned operands: the results of contiguous ones."""
+    q, k, v, grad = tensors(2, 100, 100, 4, 2, 64, torch.bfloat16, 9)
+    blocks = torch_ops.select_blocks(q, k, 2)
+    want = torch_ops.selected_attention(q, k, v, blocks, 0.125)
+    heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    packed = torch.cat([q, k, v], 2)
+    sliced = packed[:, :, :4], packed[:, :, 4:6], packed[:, :, 6:]
+    odd = [torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape).copy_(x) for x in (q, k, v)]
+    for x in (heads_first, sliced, odd):
+        assert torch.equal(torch_ops.select_blocks(x[0], x[1], 2), blocks)
+        assert torch.equal(torch_ops.selected_attention(*x, blocks, 0.125), want)
+    one = k[:1].clone().requires_grad_()
+    shared = one.expand(2, -1, -1, -1)
+    out = torch_ops.selected_attention(q, shared, v, blocks, 0.125)
+    assert torch.equal(out, torch_ops.selected_attention(q, shared.contiguous(), v, blocks, 0.125))
+    g, = torch.autograd.grad(out, one, grad)
+    both = shared.detach().contiguous().requires_grad_()
+    whole, = torch.autograd.grad(torch_ops.selected_attention(q, both, v, blocks, 0.125), both, grad)
+    assert torch.equal(g, whole.sum(0, keepdim=True))
+
+
+def test_gradients_against_differences():
+    """Directional derivatives of the operator itself, bf16 leaves: the loss moves as the gradients say."""
+    q, k, v, w = tensors(1, 96, 96, 4, 2, 64, torch.float16, 21)
+    blocks = torch_ops.select_blocks(q, k, 2)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 0.125), leaves, w)
+    args = [plain.f64(x) for x in (q, k, v)]
+    at = [blocks.cpu().numpy(), 0.125, True, None]
+    rng = np.random.default_rng(0)
+    for i in range(3):
+        d = rng.standard_normal(args[i].shape)
+        moved = []
+        for e in (1e-4, -1e-4):
+            x = list(args)
+            x[i] = x[i] + e * d
+            moved.append((plain.attention(*x, *at) * plain.f64(w)).sum())
+        slope, said = (moved[0] - moved[1]) / 2e-4, (plain.f64(grads[i]) * d).sum()
+        # each element is off by 4 u of its magnitude's terms at most, at random signs under d: the root of the sum of squares, times 4
+        size = np.sqrt((plain.f64(grads[i]) ** 2).sum())
+        assert abs(slope - said) <= 4 * 4 * 2.0 ** -11 * size * 4, i
+
+
+def test_results_do_not_depend_on_the_run():
+    q, k, v, grad = tensors(2, 500, 500, 8, 2, 128, torch.bfloat16, 4)
+    def step():
+        blocks = torch_ops.select_blocks(q, k, 3)
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = torch_ops.selected_attention(*leaves, blocks, 0.1)
+        return (blocks, out, *torch.autograd.grad(out, leaves, grad))
+    first = step()
+    for _ in range(3):
+        for a, b in zip(first, step()):
+            assert torch.equal(a, b)
+
+
+def test_captured_and_on_another_stream():
+    q, k, v, grad = tensors(1, 300, 300, 4, 2, 64, torch.float16, 8)
+    def step(q, k, v):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out = torch_ops.selected_attention(*leaves, torch_ops.select_blocks(q, k, 3), 0.125)
+        return (out, *torch.autograd.grad(out, leaves, grad))
+    want = step(q, k, v)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = step(q, k, v)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, again))
+    x = [torch.zeros_like(t) for t in (q, k, v)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(*x)
+    for a, b in zip(x, (q, k, v)):
+        a.copy_(b)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, held))
+
+
+def test_empty_calls():
+    for B, Lq, Lk in ((0, 5, 5), (2, 0, 5), (2, 0, 0), (2, 3, 0)):
+        q, k, v, _ = tensors(B, Lq, Lk, 2, 1, 64, torch.float16, 0)
+        blocks = torch_ops.select_blocks(q, k, 2, causal=False)
+        assert blocks.shape == (B, 1, Lq, 2) and (blocks == -1).all() or Lk > 0
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        out = torch_ops.selected_attention(*leaves, blocks, 1.0, causal=False)
+        for g in (out, *torch.autograd.grad(out, leaves, torch.ones_like(out))):
+            assert (g == 0).all()
+
+
+def test_refusals():
+    q, k, v, _ = tensors(1, 8, 8, 4, 2, 64, torch.float16, 0)
+    blocks = torch_ops.select_blocks(q, k, 2)
+    good = (q, k, v, blocks, 0.125)
+    def refused(error, *args, **kw):
+        with pytest.raises(error):
+            torch_ops.selected_attention(*args, **kw)
+    refused(VsError, q, k, v, blocks, 0.0)
+    refused(VsError, q, k, v, blocks, -1.0)
+    refused(VsError, q, k, v, blocks, float("nan"))
+    refused(VsError, q.float(), k.float(), v.float(), blocks, 0.125)
+    refused(TypeError, q, k.bfloat16(), v, blocks, 0.125)
+    refused(TypeError, q, k, v, blocks.long(), 0.125)
+    refused(ValueError, q, k, v[:, :4], blocks, 0.125)
+    refused(ValueError, q, k, v, blocks[:, :1], 0.125)
+    refused(ValueError, q[:, :, :3], k, v, blocks, 0.125)
+    refused(VsError, q, k[:, :4], v[:, :4], blocks, 0.125)                       # causal with more queries than keys
+    refused(VsError, q[:, 4:], k, v, blocks[:, :, 4:].contiguous(), 0.125, lengths=torch.ones(1, dtype=torch.int32, device=DEV))
+    refused(ValueError, *good, lengths=torch.ones(2, dtype=torch.int32, device=DEV))
+    refused(TypeError, *good, lengths=torch.ones(1, device=DEV))
+    refused(TypeError, q, k.cpu(), v, blocks, 0.125)
+    wide = torch.zeros((1, 8, 2, 136), dtype=torch.float16, device=DEV)
+    with pytest.raises(VsError):
+        torch_ops.select_blocks(wide, wide, 1)
+    with pytest.raises(RuntimeError):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        g, = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 0.125).sum(), leaves[0], create_graph=True)
+        g.sum().backward()

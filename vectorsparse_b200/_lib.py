@@ -11,7 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # VSPARSE_B200_LIB selects another build of the same library (an instrumented one, for instance)
 LIB_PATH = os.environ.get("VSPARSE_B200_LIB") or os.path.join(_HERE, "libvsparse_b200.so")
 
-VS_F16, VS_F32 = 0, 1
+VS_F16, VS_F32, VS_BF16 = 0, 1, 2
 VS_PATH_TENSOR, VS_PATH_CUDA_CORE = 0, 1
 
 ERRORS = {
@@ -45,6 +45,15 @@ SIGNATURES = {
     "vs_softmax_cvse_backward": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _f, _i, _i64, _vp]),
     "vs_attention_cvse_backward": (_i, [_i, _i, _i, _i, _i, _i] + [_vp] * 15 + [_f, _i, _vp]),
     "vs_attention_cvse_static": (_i, [_i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp]),
+    "vs_select_blocks_workspace_bytes": (_i64, [_i] * 4),
+    "vs_select_blocks": (_i, [_i] * 9 + [_vp] * 7 + [_i64, _vp]),
+    "vs_selected_attention_workspace_bytes": (_i64, [_i] * 7),
+    "vs_selected_attention": (_i, [_i] * 9 + [_vp] * 11 + [_f, _vp, _i64, _vp]),
+    "vs_selected_attention_backward": (_i, [_i] * 9 + [_vp] * 16 + [_f, _vp, _i64, _vp]),
+    "vs_cache_append": (_i, [_i] * 5 + [_vp] * 7 + [_i] * 2 + [_vp] * 5 + [_i] + [_vp] * 4),
+    "vs_cache_select": (_i, [_i] * 5 + [_vp] * 2 + [_i] + [_vp] * 3 + [_i, _vp, _i, _vp, _vp]),
+    "vs_cache_attention_workspace_bytes": (_i64, [_i] * 5),
+    "vs_cache_attention": (_i, [_i] * 6 + [_vp] * 6 + [_i] + [_vp] * 3 + [_i] + [_vp] * 3 + [_i, _vp, _f, _vp, _i64, _vp]),
     "vs_spmm_host": (_i, [_i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vs_sddmm_host": (_i, [_i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i]),
     "vs_device_status": (_i, [_i, C.POINTER(C.c_uint32)]),

@@ -26,7 +26,7 @@ def _nvcc() -> str:
 
 def _sources():
     c = os.path.join(HERE, "csrc")
-    return [os.path.join(c, "vsparse_abi.cu"), os.path.join(c, "host_build.cpp")]
+    return [os.path.join(c, "vsparse_abi.cu"), os.path.join(c, "block_attention.cu"), os.path.join(c, "host_build.cpp")]
 
 
 def _stale(target: str, deps) -> bool:
@@ -46,7 +46,7 @@ def _all_deps():
 def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale(LIB, _all_deps()):
         return LIB
-    cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
+    cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-t", "0", "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
            "-I", os.path.join(ROOT, "include"), "-I", os.path.join(HERE, "csrc"), "-o", LIB, *_sources()]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

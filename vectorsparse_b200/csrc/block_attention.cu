@@ -1,0 +1,400 @@
+// extern "C" entry points of attention over chosen blocks and of the 8-bit cache: argument validation and launches.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+#include <cstdlib>
+#include <cstring>
+#include <utility>
+
+#include "vsparse_b200.h"
+#include "common.cuh"
+#include "host.h"
+#include "blocks.cuh"
+#include "cache.cuh"
+
+#define VS_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+using namespace vs;
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int kMaxSmem = 227 * 1024;
+
+template <typename... Exp, typename... Act>
+cudaError_t launch_behind(void (*kernel)(Exp...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, Act &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Act>(args)...);
+}
+// The most shared memory that a kernel may ask for, told to the runtime once per device and kernel (the kernel's address is the key).
+template <auto kKernel> int allow_smem(int bytes) {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64) return VS_ERR_ARG;
+    if (known[dev].load(std::memory_order_acquire) >= bytes) return VS_OK;
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return (int)e;
+    int now = known[dev].load(std::memory_order_relaxed);
+    while (now < bytes && !known[dev].compare_exchange_weak(now, bytes, std::memory_order_release)) {}
+    return VS_OK;
+}
+
+// ---- attention over chosen blocks -----------------------------------------------------------------------------------
+
+// Sizes and types of a call; nothing of it needs a device.
+int check_shape(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const int32_t *lengths, blocks::Shape &s) {
+    if (dtype != VS_F16 && dtype != VS_BF16) return VS_ERR_DTYPE;
+    if (batch < 0 || queries < 0 || keys < 0) return VS_ERR_SHAPE;
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads / kv_heads > 128) return VS_ERR_SHAPE;
+    if (d < 8 || d > blocks::kMaxD || d % 8 != 0) return VS_ERR_SHAPE;
+    if (count < 1 || keys > blocks::kMaxBlocks * blocks::kBlock) return VS_ERR_SHAPE;
+    if (causal != 0 && causal != 1) return VS_ERR_ARG;
+    if (causal && queries > keys) return VS_ERR_SHAPE;
+    if (lengths && queries != keys) return VS_ERR_SHAPE;
+    if (lengths && !aligned4(lengths)) return VS_ERR_ALIGN;
+    s.batch = batch; s.queries = queries; s.keys = keys; s.heads = heads; s.kv_heads = kv_heads; s.d = d; s.count = count; s.causal = causal;
+    s.group = heads / kv_heads;
+    s.blocks = (keys + blocks::kBlock - 1) / blocks::kBlock;
+    s.words = (queries + 31) / 32;
+    s.lengths = lengths;
+    const int64_t pairs = (int64_t)batch * kv_heads;
+    // CTAs of any launch: a word, a query (tiles of one) or a block of keys each
+    if (pairs * std::max<int64_t>(queries, s.blocks) > kMaxGrid || (int64_t)batch * heads > kMaxGrid || (int64_t)batch * heads * queries > kMaxGrid * 16) return VS_ERR_SHAPE;
+    return VS_OK;
+}
+int operand(blocks::Operand &o, const void *at, const int64_t *strides, int batch, int tokens, int heads) {
+    if (!at || !strides) return VS_ERR_NULL;
+    if (!aligned16(at)) return VS_ERR_ALIGN;
+    const int extent[3] = {batch, tokens, heads};
+    for (int i = 0; i < 3; ++i) {
+        if (strides[i] < 0 || (strides[i] == 0 && extent[i] > 1)) return VS_ERR_SHAPE;
+        if (strides[i] % 8 != 0) return VS_ERR_ALIGN;
+    }
+    o.at = at; o.batch = strides[0]; o.token = strides[1]; o.head = strides[2];
+    return VS_OK;
+}
+void contiguous(blocks::Operand &o, const void *at, int64_t tokens, int64_t heads, int64_t d) {
+    o.at = at; o.batch = tokens * heads * d; o.token = heads * d; o.head = d;
+}
+inline int64_t up256(int64_t bytes) { return (bytes + 255) & ~255ll; }
+inline int64_t bits_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * s.words * s.blocks * 4); }
+
+// Queries of a tile: the largest power of two whose rows (queries x heads of the group) fit 128.
+inline int tile_queries(int group) {
+    int t = 128;
+    while (t * group > 128) t /= 2;
+    return t;
+}
+
+template <typename T, int QT> int launch_scores(const blocks::Shape &s, const blocks::Operand &q, const double *means, int32_t *lists, cudaStream_t st) {
+    const int smem = (int)blocks::score_bytes<QT>(s.blocks, s.d);
+    const int rc = allow_smem<blocks::score_kernel<T, QT>>(smem);
+    if (rc != VS_OK) return rc;
+    const int64_t grid = (int64_t)s.batch * s.kv_heads * ((s.queries + QT - 1) / QT);
+    blocks::score_kernel<T, QT><<<(unsigned)grid, blocks::kScoreThreads, smem, st>>>(s, q, means, lists);
+    return (int)cudaGetLastError();
+}
+template <typename T> int select(const blocks::Shape &s, const blocks::Operand &q, const blocks::Operand &k, int32_t *lists, double *means, cudaStream_t st) {
+    if (s.blocks > 0) {
+        blocks::means_kernel<T><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.blocks), blocks::kMeanThreads, 0, st>>>(s, k, means);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return (int)e;
+    }
+    // as many queries to a CTA as their scores leave room for
+    if (blocks::score_bytes<32>(s.blocks, s.d) <= kMaxSmem) return launch_scores<T, 32>(s, q, means, lists, st);
+    if (blocks::score_bytes<8>(s.blocks, s.d) <= kMaxSmem) return launch_scores<T, 8>(s, q, means, lists, st);
+    return launch_scores<T, 1>(s, q, means, lists, st);
+}
+static_assert(blocks::score_bytes<1>(blocks::kMaxBlocks, blocks::kMaxD) <= kMaxSmem, "scores of one query");
+
+int make_bits(const blocks::Shape &s, const int32_t *lists, uint32_t *bits, cudaStream_t st) {
+    if (s.blocks == 0) return VS_OK;
+    blocks::bits_kernel<<<(unsigned)((int64_t)s.batch * s.kv_heads * s.words), blocks::kBitsThreads, 0, st>>>(s, lists, bits);
+    return (int)cudaGetLastError();
+}
+
+template <typename T> int attention(blocks::Args a, cudaStream_t st) {
+    const blocks::Shape &s = a.s;
+    a.tile = 1;
+    blocks::rows_kernel<T, false><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.queries), blocks::kRowThreads, 0, st>>>(a);
+    return (int)cudaGetLastError();
+}
+template <typename T> int attention_backward(blocks::Args a, void *grad_q, cudaStream_t st) {
+    const blocks::Shape &s = a.s;
+    const int64_t rows = (int64_t)s.batch * s.queries * s.heads;
+    blocks::delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+    a.tile = 1;
+    a.result = grad_q;
+    blocks::rows_kernel<T, true><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.queries), blocks::kRowThreads, 0, st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+    blocks::keys_kernel<T><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.blocks), blocks::kRowThreads, 0, st>>>(a);
+    return (int)cudaGetLastError();
+}
+
+inline bool scale_ok(float scale) { return scale > 0.f && std::isfinite(scale); }
+
+}  // namespace
+
+VS_EXPORT int64_t vs_select_blocks_workspace_bytes(int batch, int keys, int kv_heads, int d) {
+    if (batch < 1 || keys < 1 || kv_heads < 1 || d < 1) return 0;
+    return up256((int64_t)batch * kv_heads * ((keys + blocks::kBlock - 1) / blocks::kBlock) * d * 8);
+}
+
+VS_EXPORT int vs_select_blocks(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const void *q,
+                               const int64_t *q_strides, const void *k, const int64_t *k_strides, const int32_t *lengths, int32_t *lists, void *workspace,
+                               int64_t workspace_bytes, void *stream) {
+    blocks::Shape s;
+    int rc = check_shape(dtype, batch, queries, keys, heads, kv_heads, d, count, causal, lengths, s);
+    if (rc != VS_OK) return rc;
+    if (batch == 0 || queries == 0) return VS_OK;
+    blocks::Operand oq, ok = {};
+    if ((rc = operand(oq, q, q_strides, batch, queries, heads)) != VS_OK) return rc;
+    if (keys > 0 && (rc = operand(ok, k, k_strides, batch, keys, kv_heads)) != VS_OK) return rc;
+    if (!lists || (keys > 0 && !workspace)) return VS_ERR_NULL;
+    if (!aligned16(workspace) || !aligned4(lists)) return VS_ERR_ALIGN;
+    if (workspace_bytes < vs_select_blocks_workspace_bytes(batch, keys, kv_heads, d)) return VS_ERR_SHAPE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    double *means = static_cast<double *>(workspace);
+    return dtype == VS_F16 ? select<__half>(s, oq, ok, lists, means, st) : select<__nv_bfloat16>(s, oq, ok, lists, means, st);
+}
+
+VS_EXPORT int64_t vs_selected_attention_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int d, int backward) {
+    blocks::Shape s;
+    if (check_shape(VS_F16, batch, queries, keys, heads, kv_heads, d, 1, 0, nullptr, s) != VS_OK) return 0;
+    return bits_bytes(s) + (backward ? up256((int64_t)batch * heads * queries * 4) : 0);
+}
+
+VS_EXPORT int vs_selected_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const void *q,
+                                    const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v, const int64_t *v_strides,
+                                    const int32_t *lengths, const int32_t *lists, void *out, void *out_low, float *lse, float scale, void *workspace,
+                                    int64_t workspace_bytes, void *stream) {
+    blocks::Args a = {};
+    int rc = check_shape(dtype, batch, queries, keys, heads, kv_heads, d, count, causal, lengths, a.s);
+    if (rc != VS_OK) return rc;
+    if (!scale_ok(scale)) return VS_ERR_ARG;
+    if (batch == 0 || queries == 0) return VS_OK;
+    if ((rc = operand(a.q, q, q_strides, batch, queries, heads)) != VS_OK) return rc;
+    if (keys > 0 && ((rc = operand(a.k, k, k_strides, batch, keys, kv_heads)) != VS_OK || (rc = operand(a.v, v, v_strides, batch, keys, kv_heads)) != VS_OK)) return rc;
+    if (!lists || !out || !lse || (keys > 0 && !workspace)) return VS_ERR_NULL;
+    if (!aligned16(out) || !aligned16(out_low) || !aligned16(workspace) || !aligned4(lists) || !aligned4(lse)) return VS_ERR_ALIGN;
+    if (workspace_bytes < vs_selected_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, d, 0)) return VS_ERR_SHAPE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    uint32_t *bits = static_cast<uint32_t *>(workspace);
+    if ((rc = make_bits(a.s, lists, bits, st)) != VS_OK) return rc;
+    a.bits = bits; a.lse = lse; a.result = out; a.result_low = out_low; a.scale = scale;
+    return dtype == VS_F16 ? attention<__half>(a, st) : attention<__nv_bfloat16>(a, st);
+}
+
+VS_EXPORT int vs_selected_attention_backward(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal,
+                                             const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                                             const int64_t *v_strides, const int32_t *lengths, const int32_t *lists, const void *out, const void *out_low, const float *lse,
+                                             const void *grad_out, const int64_t *grad_out_strides, void *grad_q, void *grad_k, void *grad_v, float scale,
+                                             void *workspace, int64_t workspace_bytes, void *stream) {
+    blocks::Args a = {};
+    int rc = check_shape(dtype, batch, queries, keys, heads, kv_heads, d, count, causal, lengths, a.s);
+    if (rc != VS_OK) return rc;
+    if (!scale_ok(scale)) return VS_ERR_ARG;
+    if (batch == 0) return VS_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (queries == 0 || keys == 0) {   // no query attends to a key
+        const size_t q_bytes = (size_t)batch * queries * heads * d * 2, k_bytes = (size_t)batch * keys * kv_heads * d * 2;
+        if ((q_bytes && !grad_q) || (k_bytes && (!grad_k || !grad_v))) return VS_ERR_NULL;
+        cudaError_t e = cudaSuccess;
+        if (q_bytes) e = cudaMemsetAsync(grad_q, 0, q_bytes, st);
+        if (e == cudaSuccess && k_bytes) e = cudaMemsetAsync(grad_k, 0, k_bytes, st);
+        if (e == cudaSuccess && k_bytes) e = cudaMemsetAsync(grad_v, 0, k_bytes, st);
+        return (int)e;
+    }
+    if ((rc = operand(a.q, q, q_strides, batch, queries, heads)) != VS_OK || (rc = operand(a.k, k, k_strides, batch, keys, kv_heads)) != VS_OK || (rc = operand(a.v, v, v_strides, batch, keys, kv_heads)) != VS_OK ||
+        (rc = operand(a.grad_out, grad_out, grad_out_strides, batch, queries, heads)) != VS_OK)
+        return rc;
+    if (!lists || !out || !lse || !grad_q || !grad_k || !grad_v || !workspace) return VS_ERR_NULL;
+    if (!aligned16(out) || !aligned16(out_low) || !aligned16(grad_q) || !aligned16(grad_k) || !aligned16(grad_v) || !aligned16(workspace) || !aligned4(lists) || !aligned4(lse)) return VS_ERR_ALIGN;
+    if (workspace_bytes < vs_selected_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, d, 1)) return VS_ERR_SHAPE;
+    contiguous(a.out, out, queries, heads, d);
+    a.out_low = out_low;
+    uint32_t *bits = static_cast<uint32_t *>(workspace);
+    if ((rc = make_bits(a.s, lists, bits, st)) != VS_OK) return rc;
+    a.bits = bits; a.lse = const_cast<float *>(lse); a.scale = scale;
+    a.delta = reinterpret_cast<float *>(static_cast<char *>(workspace) + bits_bytes(a.s));
+    a.grad_k = grad_k; a.grad_v = grad_v;
+    return dtype == VS_F16 ? attention_backward<__half>(a, grad_q, st) : attention_backward<__nv_bfloat16>(a, grad_q, st);
+}
+
+// ---- the cache ----------------------------------------------------------------------------------------------------------
+
+namespace {
+
+int check_cache(int dtype, int pages, int tails, int kv_heads, int d, int sequences, int max_blocks) {
+    if (dtype != VS_F16 && dtype != VS_BF16) return VS_ERR_DTYPE;
+    if (pages < 0 || tails < 0 || sequences < 0 || kv_heads < 1 || max_blocks < 0) return VS_ERR_SHAPE;
+    if (d < 16 || d > blocks::kMaxD || d % 16 != 0) return VS_ERR_SHAPE;
+    if ((int64_t)sequences * kv_heads > kMaxGrid) return VS_ERR_SHAPE;
+    return VS_OK;
+}
+
+template <typename T, int NK> int launch_decode(const cache::AttentionArgs &a, int items, cudaStream_t st) {
+    const int smem = cache::kWarps * cache::kSlots * blocks::kBlock * NK * 16;
+    const int rc = allow_smem<cache::decode_kernel<T, NK>>(smem);
+    if (rc != VS_OK) return rc;
+    cache::decode_kernel<T, NK><<<(unsigned)(items * a.pieces), cache::kDecodeThreads, smem, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && a.pieces > 1) e = launch_behind(cache::join_kernel<T>, (unsigned)items, 128u, 0, st, a);
+    return (int)e;
+}
+template <typename T> int decode(const cache::AttentionArgs &a, int items, cudaStream_t st) {
+    switch (a.c.d / 16) {
+        case 1: return launch_decode<T, 1>(a, items, st);
+        case 2: return launch_decode<T, 2>(a, items, st);
+        case 3: return launch_decode<T, 3>(a, items, st);
+        case 4: return launch_decode<T, 4>(a, items, st);
+        case 5: return launch_decode<T, 5>(a, items, st);
+        case 6: return launch_decode<T, 6>(a, items, st);
+        case 7: return launch_decode<T, 7>(a, items, st);
+        default: return launch_decode<T, 8>(a, items, st);
+    }
+}
+
+// Pieces that the blocks of a sequence and head are shared out in: about eight CTAs an SM in all, so that sequences of unlike lengths even out, but at
+// least two blocks to a warp.
+int decode_pieces(int64_t items, int units) {
+    constexpr int kCtas = 148 * 8;
+    const int64_t want = (kCtas + items - 1) / items, most = std::max(1, units / (2 * cache::kWarps));
+    return (int)std::min<int64_t>({want, most, 64});
+}
+
+}  // namespace
+
+VS_EXPORT int vs_cache_append(int dtype, int pages, int tails, int kv_heads, int d, int8_t *k_codes, int8_t *v_codes, float *k_scales, float *v_scales,
+                              int16_t *k_sums, void *k_ring, void *v_ring, int sequences, int tokens, const void *k, const int64_t *k_strides,
+                              const void *v, const int64_t *v_strides, const int32_t *table, int max_blocks, const int32_t *tail_indices,
+                              const int32_t *lengths, const int32_t *counts, void *stream) {
+    int rc = check_cache(dtype, pages, tails, kv_heads, d, sequences, max_blocks);
+    if (rc != VS_OK) return rc;
+    if (tokens < 0) return VS_ERR_SHAPE;
+    if (sequences == 0 || tokens == 0) return VS_OK;
+    blocks::Operand n[2];
+    if ((rc = operand(n[0], k, k_strides, sequences, tokens, kv_heads)) != VS_OK || (rc = operand(n[1], v, v_strides, sequences, tokens, kv_heads)) != VS_OK) return rc;
+    if ((pages > 0 && (!k_codes || !v_codes || !k_scales || !v_scales || !k_sums)) || (tails > 0 && (!k_ring || !v_ring)) || (max_blocks > 0 && !table) ||
+        !tail_indices || !lengths)
+        return VS_ERR_NULL;
+    for (const void *p : {(const void *)k_codes, (const void *)v_codes, (const void *)k_ring, (const void *)v_ring, (const void *)k_sums})
+        if (!aligned16(p)) return VS_ERR_ALIGN;
+    for (const void *p : {(const void *)table, (const void *)tail_indices, (const void *)lengths, (const void *)counts, (const void *)k_scales, (const void *)v_scales})
+        if (!aligned4(p)) return VS_ERR_ALIGN;
+    cache::AppendArgs a;
+    a.c = {pages, tails, kv_heads, d, {k_codes, v_codes}, {k_scales, v_scales}, k_sums, {k_ring, v_ring}};
+    a.s = {sequences, table, max_blocks, tail_indices, lengths};
+    a.tokens = tokens;
+    a.touched = (int)(((int64_t)tokens + blocks::kBlock - 2) / blocks::kBlock + 1);
+    a.counts = counts;
+    for (int i = 0; i < 2; ++i) {
+        a.at[i] = n[i].at; a.batch[i] = n[i].batch; a.token[i] = n[i].token; a.head[i] = n[i].head;
+    }
+    const int64_t grid = (int64_t)sequences * kv_heads * a.touched;
+    if (grid > kMaxGrid) return VS_ERR_SHAPE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == VS_F16) cache::append_kernel<__half><<<dim3((unsigned)grid, 2), cache::kAppendThreads, 0, st>>>(a);
+    else cache::append_kernel<__nv_bfloat16><<<dim3((unsigned)grid, 2), cache::kAppendThreads, 0, st>>>(a);
+    return (int)cudaGetLastError();
+}
+
+VS_EXPORT int vs_cache_select(int dtype, int pages, int heads, int kv_heads, int d, const float *k_scales, const int16_t *k_sums, int sequences,
+                              const void *q, const int64_t *q_strides, const int32_t *table, int max_blocks, const int32_t *lengths, int count,
+                              int32_t *lists, void *stream) {
+    int rc = check_cache(dtype, pages, 0, kv_heads, d, sequences, max_blocks);
+    if (rc != VS_OK) return rc;
+    if (heads < kv_heads || heads % kv_heads != 0 || count < 1 || max_blocks > blocks::kMaxBlocks) return VS_ERR_SHAPE;
+    if (sequences == 0) return VS_OK;
+    if (!q || !q_strides || !lengths || !lists || (max_blocks > 0 && !table) || (pages > 0 && (!k_scales || !k_sums))) return VS_ERR_NULL;
+    if (!aligned16(q) || !aligned16(k_sums)) return VS_ERR_ALIGN;
+    for (const void *p : {(const void *)table, (const void *)lengths, (const void *)lists, (const void *)k_scales})
+        if (!aligned4(p)) return VS_ERR_ALIGN;
+    for (int i = 0; i < 2; ++i) {
+        if (q_strides[i] < 0) return VS_ERR_SHAPE;
+        if (q_strides[i] % 8 != 0) return VS_ERR_ALIGN;
+    }
+    cache::SelectArgs a = {};
+    a.c.pages = pages; a.c.kv_heads = kv_heads; a.c.d = d; a.c.scales[0] = const_cast<float *>(k_scales); a.c.sums = const_cast<int16_t *>(k_sums);
+    a.s = {sequences, table, max_blocks, nullptr, lengths};
+    a.q = q; a.batch = q_strides[0]; a.head = q_strides[1];
+    a.group = heads / kv_heads; a.wanted = count; a.lists = lists;
+    const int smem = (int)((int64_t)max_blocks * 8 + (max_blocks + 31) / 32 * 4), threads = max_blocks > 256 ? 1024 : 256;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == VS_F16) {
+        if ((rc = allow_smem<cache::select_kernel<__half>>(smem)) != VS_OK) return rc;
+        cache::select_kernel<__half><<<(unsigned)(sequences * kv_heads), threads, smem, st>>>(a);
+    } else {
+        if ((rc = allow_smem<cache::select_kernel<__nv_bfloat16>>(smem)) != VS_OK) return rc;
+        cache::select_kernel<__nv_bfloat16><<<(unsigned)(sequences * kv_heads), threads, smem, st>>>(a);
+    }
+    return (int)cudaGetLastError();
+}
+
+VS_EXPORT int64_t vs_cache_attention_workspace_bytes(int sequences, int heads, int kv_heads, int d, int units) {
+    if (sequences < 1 || kv_heads < 1 || heads < kv_heads || d < 1 || units < 0) return 0;
+    const int64_t items = (int64_t)sequences * kv_heads * ((heads / kv_heads + 15) / 16);
+    const int pieces = decode_pieces(items, units);
+    return pieces > 1 ? up256(items * pieces * 16 * (d + 2) * 4) : 0;
+}
+
+VS_EXPORT int vs_cache_attention(int dtype, int pages, int tails, int heads, int kv_heads, int d, const int8_t *k_codes, const int8_t *v_codes,
+                                 const float *k_scales, const float *v_scales, const void *k_ring, const void *v_ring, int sequences, const void *q,
+                                 const int64_t *q_strides, const int32_t *table, int max_blocks, const int32_t *tail_indices, const int32_t *lengths,
+                                 const int32_t *lists, int count, void *out, float scale, void *workspace, int64_t workspace_bytes, void *stream) {
+    int rc = check_cache(dtype, pages, tails, kv_heads, d, sequences, max_blocks);
+    if (rc != VS_OK) return rc;
+    if (heads < kv_heads || heads % kv_heads != 0 || (lists && count < 1)) return VS_ERR_SHAPE;
+    if (!scale_ok(scale)) return VS_ERR_ARG;
+    if (sequences == 0) return VS_OK;
+    if (!q || !q_strides || !lengths || !out || !tail_indices || (max_blocks > 0 && !table) || (pages > 0 && (!k_codes || !v_codes || !k_scales || !v_scales)) ||
+        (tails > 0 && (!k_ring || !v_ring)))
+        return VS_ERR_NULL;
+    for (const void *p : {q, (const void *)k_codes, (const void *)v_codes, k_ring, v_ring, (const void *)out, (const void *)workspace})
+        if (!aligned16(p)) return VS_ERR_ALIGN;
+    for (const void *p : {(const void *)table, (const void *)tail_indices, (const void *)lengths, (const void *)lists, (const void *)k_scales, (const void *)v_scales})
+        if (!aligned4(p)) return VS_ERR_ALIGN;
+    for (int i = 0; i < 2; ++i) {
+        if (q_strides[i] < 0) return VS_ERR_SHAPE;
+        if (q_strides[i] % 8 != 0) return VS_ERR_ALIGN;
+    }
+    const int units = lists ? count : max_blocks;
+    cache::AttentionArgs a = {};
+    a.parts = (heads / kv_heads + 15) / 16;
+    const int64_t items = (int64_t)sequences * kv_heads * a.parts;
+    a.pieces = decode_pieces(items, units);
+    if (items * a.pieces > kMaxGrid) return VS_ERR_SHAPE;
+    if (workspace_bytes < vs_cache_attention_workspace_bytes(sequences, heads, kv_heads, d, units)) return VS_ERR_SHAPE;
+    if (a.pieces > 1 && !workspace) return VS_ERR_NULL;
+    int sms = 0;
+    if ((rc = current_device(&sms, &a.status)) != VS_OK) return rc;
+    a.c = {pages, tails, kv_heads, d, {const_cast<int8_t *>(k_codes), const_cast<int8_t *>(v_codes)}, {const_cast<float *>(k_scales), const_cast<float *>(v_scales)},
+           nullptr, {const_cast<void *>(k_ring), const_cast<void *>(v_ring)}};
+    a.s = {sequences, table, max_blocks, tail_indices, lengths};
+    a.q = q; a.batch = q_strides[0]; a.head = q_strides[1];
+    a.group = heads / kv_heads; a.lists = lists; a.wanted = count; a.scale = scale; a.out = out;
+    a.partial = static_cast<float *>(workspace);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == VS_F16 ? decode<__half>(a, (int)items, st) : decode<__nv_bfloat16>(a, (int)items, st);
+}

@@ -1,0 +1,449 @@
+// Attention over blocks of 64 keys that are chosen for each query: the choice, the lists as bits, and the operators row by row.
+//
+// Query i of batch entry b stands at position p = i + keys - queries.  For every head of keys and query there is a list of blocks; the query's
+// `group` heads (heads / kv_heads) attend to the keys t of the listed blocks with t < length and, causal, t <= p.
+//
+// The kernels that multiply take a tile of queries through the union of its lists, so the lists are first turned into bits:
+// bits[b, kv head][word w][block j], bit x set when query 32 w + x has block j on its list and it can hold a key for that query.
+// A list is a set here: order and repetitions do not count, and entries that are no block are none.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+#include <stdint.h>
+
+namespace vs {
+namespace blocks {
+
+constexpr int kBlock = 64;
+constexpr int kMaxD = 128;
+constexpr int kMaxBlocks = 16384;   // per sequence: scores of one query fit in shared memory
+
+struct Shape {
+    int batch, queries, keys, heads, kv_heads, d, count;
+    int causal;
+    int group;    // heads / kv_heads
+    int blocks;   // of keys
+    int words;    // of 32 queries
+    const int32_t *lengths;   // tokens of each batch entry (queries == keys), or null: all
+
+    __device__ __forceinline__ int length(int b) const { return lengths ? min(max(lengths[b], 0), keys) : keys; }
+    __device__ __forceinline__ int rows(int b) const { return lengths ? min(max(lengths[b], 0), queries) : queries; }
+    __device__ __forceinline__ int position(int i) const { return i + keys - queries; }
+    // keys that query i may attend to end here
+    __device__ __forceinline__ int end(int i, int len) const { return causal ? min(len, position(i) + 1) : len; }
+};
+struct Operand {   // [batch, tokens, heads, d], the last dimension contiguous; strides in elements
+    const void *at;
+    int64_t batch, token, head;
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T> __device__ __forceinline__ void load8(const T *p, float (&f)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    const T *h = reinterpret_cast<const T *>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(h[i]);
+}
+
+// ---- lists as bits ------------------------------------------------------------------------------------------------
+// One CTA takes a word of 32 queries: it collects their bits in shared memory and writes the word's row for all blocks, so that nothing has to
+// be cleared beforehand.  Bound by the reading of the lists.
+constexpr int kBitsThreads = 128, kBitsChunk = 4096;
+__global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const int32_t *lists, uint32_t *bits) {
+    __shared__ uint32_t row[kBitsChunk];
+    const int64_t at = blockIdx.x;
+    const int w = (int)(at % s.words);
+    const int b = (int)(at / s.words / s.kv_heads);
+    const int len = s.length(b), rows = s.rows(b);
+    const int32_t *list = lists + (at / s.words * s.queries + w * 32) * s.count;
+    const int entries = min(32, s.queries - w * 32) * s.count;
+    for (int base = 0; base < s.blocks; base += kBitsChunk) {
+        const int n = min(kBitsChunk, s.blocks - base);
+        for (int j = threadIdx.x; j < n; j += kBitsThreads) row[j] = 0;
+        __syncthreads();
+        for (int e = threadIdx.x; e < entries; e += kBitsThreads) {
+            const int x = e / s.count, i = w * 32 + x, j = list[e] - base;
+            if (j >= 0 && j < n && i < rows && (int64_t)(base + j) * kBlock < s.end(i, len)) atomicOr(row + j, 1u << x);
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < n; j += kBitsThreads) bits[at * s.blocks + base + j] = row[j];
+        __syncthreads();
+    }
+}
+
+// ---- choosing -----------------------------------------------------------------------------------------------------
+// Score of block j for query i: (sum of the group's query heads) . (mean of the block's keys), everything in 64 bits: its order decides whole
+// numbers, and 32-bit sums in two orders disagree about blocks that are close.
+// Means: one CTA per (b, kv head, block), 8 dimensions to a thread, the tokens shared by groups of threads.
+constexpr int kMeanThreads = 128;
+template <typename T> __global__ void __launch_bounds__(kMeanThreads) means_kernel(const Shape s, const Operand k, double *means) {
+    __shared__ double part[kMeanThreads * 8];
+    const int64_t at = blockIdx.x;
+    const int j = (int)(at % s.blocks), h = (int)(at / s.blocks % s.kv_heads), b = (int)(at / s.blocks / s.kv_heads);
+    const int first = j * kBlock, n = min(kBlock, s.length(b) - first);
+    const int chunks = s.d / 8, groups = kMeanThreads / chunks, c = threadIdx.x % chunks, g = threadIdx.x / chunks;
+    double sum[8] = {};
+    if (g < groups) {
+        const T *p = static_cast<const T *>(k.at) + b * k.batch + first * k.token + h * k.head + c * 8;
+        for (int t = g; t < n; t += groups) {
+            float f[8];
+            load8(p + t * k.token, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += f[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[(g * chunks + c) * 8 + i] = sum[i];
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < s.d; x += kMeanThreads) {
+        double total = 0;
+        for (int y = 0; y < groups; ++y) total += part[y * s.d + x];
+        means[at * s.d + x] = n > 0 ? total / n : 0.0;
+    }
+}
+
+// Scores as whole numbers of the same order, above 0; what is no number counts as the lowest score.
+__device__ __forceinline__ uint64_t sortable(double x) {
+    x = x != x ? -DBL_MAX : fmin(fmax(x, -DBL_MAX), DBL_MAX);
+    const uint64_t u = (uint64_t)__double_as_longlong(x == 0.0 ? 0.0 : x);
+    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+// A warp takes the `want` highest of keys[0 .. n) (0: not to be had) into `taken` bits, ties to the lowest index.  keys lose what is taken.
+__device__ __forceinline__ void take_best(uint64_t *keys, int n, int want, uint32_t *taken) {
+    const int lane = threadIdx.x & 31;
+    uint64_t best = 0;
+    int at = 0x7fffffff;
+    auto scan = [&]() {
+        best = 0;
+        at = 0x7fffffff;
+        for (int j = lane; j < n; j += 32)
+            if (keys[j] > best) { best = keys[j]; at = j; }
+    };
+    scan();
+    for (int x = 0; x < want; ++x) {
+        const uint32_t hi = (uint32_t)(best >> 32), top = __reduce_max_sync(~0u, hi);
+        const uint32_t lo = hi == top ? (uint32_t)best : 0u, low = __reduce_max_sync(~0u, lo);
+        if (!(top | low)) break;
+        const int winner = __reduce_min_sync(~0u, hi == top && lo == low ? at : 0x7fffffff);
+        if (at == winner) {
+            keys[at] = 0;
+            taken[at >> 5] |= 1u << (at & 31);   // words are shared by lanes of a warp, but one lane writes at a time
+            scan();
+        }
+        __syncwarp();
+    }
+}
+// The set bits in ascending order, -1 behind them.
+__device__ __forceinline__ void write_list(const uint32_t *taken, int words, int count, int32_t *list) {
+    const int lane = threadIdx.x & 31;
+    int done = 0;
+    for (int base = 0; base < words; base += 32) {
+        uint32_t w = base + lane < words ? taken[base + lane] : 0u;
+        int before = __popc(w);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(~0u, before, o);
+            if (lane >= o) before += y;
+        }
+        const int total = __shfl_sync(~0u, before, 31);
+        int at = done + before - __popc(w);
+        for (; w; w &= w - 1) list[at++] = (base + lane) * 32 + __ffs(w) - 1;
+        done += total;
+    }
+    for (int x = done + lane; x < count; x += 32) list[x] = -1;
+}
+
+// One CTA scores QT queries of one head of keys against all their candidates, 64 blocks and 32 dimensions at a time, and each of its warps
+// then takes the best of one query after another.  Shared memory: the queries' sums, a piece of the means, the scores.
+constexpr int kScoreThreads = 256, kPiece = 32;
+template <int QT> constexpr int64_t score_bytes(int blocks, int d) {
+    return (int64_t)QT * (d + 1) * 8 + (int64_t)kBlock * (kPiece + 1) * 8 + (int64_t)QT * blocks * 8 + (int64_t)(kScoreThreads / 32) * ((blocks + 31) / 32) * 4;
+}
+template <typename T, int QT> __global__ void __launch_bounds__(kScoreThreads) score_kernel(const Shape s, const Operand q, const double *means, int32_t *lists) {
+    extern __shared__ double sm[];
+    double *sums = sm, *piece = sums + QT * (s.d + 1), *scores = piece + kBlock * (kPiece + 1);
+    uint32_t *taken_all = reinterpret_cast<uint32_t *>(scores + (int64_t)QT * s.blocks);
+    const int tiles = (s.queries + QT - 1) / QT;
+    const int64_t bh = blockIdx.x / tiles;
+    const int i0 = (int)(blockIdx.x % tiles) * QT, h = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
+    const int len = s.length(b), rows = s.rows(b), tid = threadIdx.x;
+    const int last = min(i0 + QT, rows) - 1;   // last query of the tile that is there
+    const int most = last < i0 ? 0 : s.causal ? s.position(last) / kBlock : (len + kBlock - 1) / kBlock;   // candidates of any of them
+
+    const T *qp = static_cast<const T *>(q.at) + b * q.batch + h * s.group * q.head;
+    for (int x = tid; x < QT * (s.d / 8); x += kScoreThreads) {
+        const int i = x / (s.d / 8), c = x % (s.d / 8) * 8;
+        double sum[8] = {};
+        if (i0 + i < rows)
+            for (int g = 0; g < s.group; ++g) {
+                float f[8];
+                load8(qp + (i0 + i) * q.token + g * q.head + c, f);
+#pragma unroll
+                for (int y = 0; y < 8; ++y) sum[y] += f[y];
+            }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) sums[i * (s.d + 1) + c + y] = sum[y];
+    }
+    constexpr int kRows = QT >= 16 ? QT / 16 : 1;   // queries of a thread; the 16 threads of a row of threads take 4 blocks each
+    const int tx = tid % 16, ty = tid / 16;
+    for (int base = 0; base < most; base += kBlock) {
+        double acc[kRows][4] = {};
+        for (int d0 = 0; d0 < s.d; d0 += kPiece) {
+            const int width = min(kPiece, s.d - d0);
+            __syncthreads();
+            for (int x = tid; x < kBlock * kPiece; x += kScoreThreads) {
+                const int j = x / kPiece, y = x % kPiece;
+                piece[j * (kPiece + 1) + y] = base + j < most && y < width ? means[(bh * s.blocks + base + j) * s.d + d0 + y] : 0.0;
+            }
+            __syncthreads();
+            if (ty * kRows < QT)
+                for (int y = 0; y < width; ++y) {
+                    double a[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) a[x] = piece[(tx + 16 * x) * (kPiece + 1) + y];
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) {
+                        const double v = sums[(ty * kRows + r) * (s.d + 1) + d0 + y];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[r][x] = fma(v, a[x], acc[r][x]);
+                    }
+                }
+        }
+        if (ty * kRows < QT)
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (base + tx + 16 * x < most) scores[(int64_t)(ty * kRows + r) * s.blocks + base + tx + 16 * x] = acc[r][x];
+    }
+    __syncthreads();
+    const int warp = tid >> 5, lane = tid & 31, words = (s.blocks + 31) / 32;
+    uint32_t *taken = taken_all + warp * words;
+    for (int r = warp; r < QT && i0 + r < s.queries; r += kScoreThreads / 32) {
+        const int i = i0 + r, own = s.causal ? s.position(i) / kBlock : -1;
+        int32_t *list = lists + (bh * s.queries + i) * s.count;
+        const int n = i >= rows ? 0 : s.causal ? own : most;
+        uint64_t *keys = reinterpret_cast<uint64_t *>(scores + (int64_t)r * s.blocks);
+        for (int j = lane; j < n; j += 32) keys[j] = sortable(__longlong_as_double((long long)keys[j]));
+        for (int x = lane; x < words; x += 32) taken[x] = i < rows && own >= 0 && own / 32 == x ? 1u << (own & 31) : 0u;
+        __syncwarp();
+        take_best(keys, n, s.count - (own >= 0), taken);
+        __syncwarp();
+        write_list(taken, words, s.count, list);
+        __syncwarp();
+    }
+}
+
+// ---- attention, row by row ------------------------------------------------------------------------------------------
+// The operators straight from their formulas, on the CUDA cores, in fp32: a warp takes a row (query, head), its lanes the keys of a block two by two for
+// the scores and then the dimensions for the sums.  Keys that a row does not attend to are not read, so what stands there cannot reach it, whatever it is.
+// `redo`: one word per tile of `tile` queries (forward, dQ) or per block of keys (dK, dV); only those with a word that is not 0 are computed.
+struct Args {
+    Shape s;
+    Operand q, k, v, out, grad_out;   // out and grad_out as q
+    const uint32_t *bits;
+    float *lse;           // [batch, heads, queries] base 2; +inf: the row attends to nothing
+    float *delta;         // the same shape: rowsum(out o grad_out)
+    const void *out_low;  // what rounding left of out, as out; or null
+    void *result;         // out or grad_q, contiguous
+    void *result_low;     // out_low or null
+    void *grad_k, *grad_v;
+    const uint32_t *redo;
+    int tile;
+    float scale;
+};
+constexpr int kRowThreads = 128, kRowWarps = kRowThreads / 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T> __device__ __forceinline__ float dot_row(const float *a, const T *p, int d) {
+    float sum = 0.f;
+    for (int c = 0; c < d; c += 8) {
+        float f[8];
+        load8(p + c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(a[c + i], f[i], sum);
+    }
+    return sum;
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+    return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return x;
+}
+
+template <typename T, bool kBackward> __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Args a) {
+    __shared__ float q_s[kRowWarps][kMaxD], g_s[kRowWarps][kMaxD];
+    if (a.redo && a.redo[blockIdx.x] == 0) return;
+    const Shape &s = a.s;
+    const int tiles = (s.queries + a.tile - 1) / a.tile;
+    const int64_t bh = blockIdx.x / tiles;
+    const int i0 = (int)(blockIdx.x % tiles) * a.tile, kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, len = s.length(b);
+    const T *kp = static_cast<const T *>(a.k.at) + b * a.k.batch + kvh * a.k.head;
+    const T *vp = static_cast<const T *>(a.v.at) + b * a.v.batch + kvh * a.v.head;
+    const float c = a.scale * kLog2e;
+    for (int r = warp; r < a.tile * s.group; r += kRowWarps) {
+        const int i = i0 + r / s.group, h = kvh * s.group + r % s.group;
+        if (i >= s.queries) break;
+        const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+        const T *qp = static_cast<const T *>(a.q.at) + b * a.q.batch + (int64_t)i * a.q.token + h * a.q.head;
+        const T *gp = kBackward ? static_cast<const T *>(a.grad_out.at) + b * a.grad_out.batch + (int64_t)i * a.grad_out.token + h * a.grad_out.head : nullptr;
+        __syncwarp();
+        for (int x = lane; x < s.d; x += 32) {
+            q_s[warp][x] = to_f32(qp[x]);
+            if (kBackward) g_s[warp][x] = to_f32(gp[x]);
+        }
+        __syncwarp();
+        const int end = s.end(i, len);
+        const uint32_t *bits = a.bits + (bh * s.words + (i >> 5)) * s.blocks;
+        float top = -INFINITY, total = 0.f, acc[kMaxD / 32] = {};
+        const float lse = kBackward ? a.lse[row] : 0.f, delta = kBackward ? a.delta[row] : 0.f;
+        for (int j = 0; j < s.blocks; ++j) {
+            if (!(bits[j] >> (i & 31) & 1u)) continue;
+            const int n = min(kBlock, end - j * kBlock);
+            float w[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int t = lane + 32 * x;
+                w[x] = -INFINITY;
+                if (t < n) w[x] = dot_row(q_s[warp], kp + (int64_t)(j * kBlock + t) * a.k.token, s.d) * c;
+            }
+            if (!kBackward) {
+                const float m = fmaxf(top, warp_max(fmaxf(w[0], w[1]))), base = m == -INFINITY ? 0.f : m;
+                const float shrink = exp2f(top - base);
+                w[0] = lane < n ? exp2f(w[0] - base) : 0.f;
+                w[1] = lane + 32 < n ? exp2f(w[1] - base) : 0.f;
+                total = total * shrink + warp_sum(w[0] + w[1]);
+                top = m;
+#pragma unroll
+                for (int x = 0; x < kMaxD / 32; ++x) acc[x] *= shrink;
+            } else {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int t = lane + 32 * x;
+                    float ds = 0.f;
+                    if (t < n) ds = exp2f(w[x] - lse) * (dot_row(g_s[warp], vp + (int64_t)(j * kBlock + t) * a.v.token, s.d) - delta) * a.scale;
+                    w[x] = ds;
+                }
+            }
+            for (int t = 0; t < n; ++t) {
+                const float p = __shfl_sync(~0u, t < 32 ? w[0] : w[1], t & 31);
+                const T *row_t = (kBackward ? kp : vp) + (int64_t)(j * kBlock + t) * (kBackward ? a.k.token : a.v.token);
+#pragma unroll
+                for (int x = 0; x < kMaxD / 32; ++x)
+                    if (lane + 32 * x < s.d) acc[x] = fmaf(p, to_f32(row_t[lane + 32 * x]), acc[x]);
+            }
+        }
+        const int64_t at = (((int64_t)b * s.queries + i) * s.heads + h) * s.d;
+#pragma unroll
+        for (int x = 0; x < kMaxD / 32; ++x)
+            if (lane + 32 * x < s.d) {
+                const float y = kBackward ? acc[x] : total == 0.f ? 0.f : acc[x] / total;
+                const T high = from_f32<T>(y);
+                static_cast<T *>(a.result)[at + lane + 32 * x] = high;
+                if (!kBackward && a.result_low) static_cast<T *>(a.result_low)[at + lane + 32 * x] = from_f32<T>(y - to_f32(high));
+            }
+        if (!kBackward && lane == 0) a.lse[row] = total == 0.f ? INFINITY : top + log2f(total);
+    }
+}
+
+// dK and dV of the keys of one block: a warp takes a key, its lanes the queries of a word for the scores and then the dimensions for the sums.
+template <typename T> __global__ void __launch_bounds__(kRowThreads) keys_kernel(const Args a) {
+    __shared__ float k_s[kRowWarps][kMaxD], v_s[kRowWarps][kMaxD];
+    if (a.redo && a.redo[blockIdx.x] == 0) return;
+    const Shape &s = a.s;
+    const int64_t bh = blockIdx.x / s.blocks;
+    const int j = (int)(blockIdx.x % s.blocks), kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, len = s.length(b);
+    const float c = a.scale * kLog2e;
+    for (int t = j * kBlock + warp; t < min(s.keys, (j + 1) * kBlock); t += kRowWarps) {
+        float dk[kMaxD / 32] = {}, dv[kMaxD / 32] = {};
+        if (t < len) {
+            const T *kp = static_cast<const T *>(a.k.at) + b * a.k.batch + (int64_t)t * a.k.token + kvh * a.k.head;
+            const T *vp = static_cast<const T *>(a.v.at) + b * a.v.batch + (int64_t)t * a.v.token + kvh * a.v.head;
+            __syncwarp();
+            for (int x = lane; x < s.d; x += 32) {
+                k_s[warp][x] = to_f32(kp[x]);
+                v_s[warp][x] = to_f32(vp[x]);
+            }
+            __syncwarp();
+            for (int w = 0; w < s.words; ++w) {
+                const int i = w * 32 + lane;
+                const bool here = (a.bits[(bh * s.words + w) * s.blocks + j] >> lane & 1u) && t < s.end(i, len);
+                const uint32_t rows = __ballot_sync(~0u, here);
+                if (!rows) continue;
+                for (int g = 0; g < s.group; ++g) {
+                    const int h = kvh * s.group + g;
+                    const T *qp = static_cast<const T *>(a.q.at) + b * a.q.batch + h * a.q.head;
+                    const T *gp = static_cast<const T *>(a.grad_out.at) + b * a.grad_out.batch + h * a.grad_out.head;
+                    float p = 0.f, ds = 0.f;
+                    if (here) {
+                        const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+                        p = exp2f(dot_row(k_s[warp], qp + (int64_t)i * a.q.token, s.d) * c - a.lse[row]);
+                        ds = p * (dot_row(v_s[warp], gp + (int64_t)i * a.grad_out.token, s.d) - a.delta[row]) * a.scale;
+                    }
+                    for (uint32_t left = rows; left; left &= left - 1) {
+                        const int x = __ffs(left) - 1;
+                        const float px = __shfl_sync(~0u, p, x), dx = __shfl_sync(~0u, ds, x);
+#pragma unroll
+                        for (int y = 0; y < kMaxD / 32; ++y) {
+                            const int e = lane + 32 * y;
+                            if (e < s.d) {
+                                dv[y] = fmaf(px, to_f32(gp[(int64_t)(w * 32 + x) * a.grad_out.token + e]), dv[y]);
+                                dk[y] = fmaf(dx, to_f32(qp[(int64_t)(w * 32 + x) * a.q.token + e]), dk[y]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        const int64_t at = (((int64_t)b * s.keys + t) * s.kv_heads + kvh) * s.d;
+#pragma unroll
+        for (int y = 0; y < kMaxD / 32; ++y)
+            if (lane + 32 * y < s.d) {
+                static_cast<T *>(a.grad_k)[at + lane + 32 * y] = from_f32<T>(dk[y]);
+                static_cast<T *>(a.grad_v)[at + lane + 32 * y] = from_f32<T>(dv[y]);
+            }
+    }
+}
+
+// rowsum(out o grad_out) of each row; 0 for rows behind a sequence's end.  Eight dimensions to a lane, 16 lanes to a row.
+template <typename T> __global__ void __launch_bounds__(256) delta_kernel(const Args a) {
+    const Shape &s = a.s;
+    const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, all = (int64_t)s.batch * s.queries * s.heads;
+    const int c = threadIdx.x % 16 * 8;
+    const int h = (int)(at % s.heads), i = (int)(at / s.heads % s.queries), b = (int)(at / s.heads / s.queries);
+    float sum = 0.f;
+    if (at < all && c < s.d && i < s.rows(b)) {
+        float o[8], g[8];
+        load8(static_cast<const T *>(a.out.at) + b * a.out.batch + (int64_t)i * a.out.token + h * a.out.head + c, o);
+        load8(static_cast<const T *>(a.grad_out.at) + b * a.grad_out.batch + (int64_t)i * a.grad_out.token + h * a.grad_out.head + c, g);
+        if (a.out_low) {
+            float low[8];
+            load8(static_cast<const T *>(a.out_low) + at * s.d + c, low);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) sum = fmaf(low[x], g[x], sum);
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sum = fmaf(o[x], g[x], sum);
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (at < all && c == 0) a.delta[((int64_t)b * s.heads + h) * s.queries + i] = sum;
+}
+
+}  // namespace blocks
+}  // namespace vs

@@ -25,6 +25,7 @@
 
 #include "vsparse_b200.h"
 #include "common.cuh"
+#include "host.h"
 #include "cuda_core.cuh"
 #include "attention.cuh"
 #include "spmm_tc.cuh"
@@ -128,6 +129,19 @@ int device_info(DeviceInfo **out) {
     *out = &d;
     return VS_OK;
 }
+
+}  // namespace
+
+int vs::current_device(int *sm_count, uint32_t **status) {
+    DeviceInfo *d = nullptr;
+    const int rc = device_info(&d);
+    if (rc != VS_OK) return rc;
+    *sm_count = d->sm_count;
+    *status = d->status;
+    return VS_OK;
+}
+
+namespace {
 
 // Set for the duration of an entry point that promises not to allocate: the tensor-core formulations that need
 // plan scratch are skipped on this thread, the kernels that need none take the call.
@@ -438,9 +452,6 @@ struct TimedLaunch {   // records the opening event on construction, the closing
 };
 
 // cuTensorMapEncodeTiled, fetched from the driver at first use (the library does not link libcuda).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn encode_tiled_fn() {
     static EncodeTiledFn fn = []() -> EncodeTiledFn {
         void *p = nullptr;
@@ -450,7 +461,11 @@ EncodeTiledFn encode_tiled_fn() {
     }();
     return fn;
 }
+}  // namespace
 
+vs::EncodeTiledFn vs::encode_tiled() { return encode_tiled_fn(); }
+
+namespace {
 // Tensor map of a row-major fp16 matrix [rows x cols] for row gathers: box = 64 columns x 1 row, 128-byte
 // swizzle, zero fill outside the matrix.
 int make_gather_map(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t cols) {

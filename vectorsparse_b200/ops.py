@@ -22,7 +22,7 @@ import types
 import torch
 
 from . import _lib
-from ._lib import VS_F16, VS_F32, VS_PATH_CUDA_CORE, VS_PATH_TENSOR
+from ._lib import VS_BF16, VS_F16, VS_F32, VS_PATH_CUDA_CORE, VS_PATH_TENSOR
 
 try:
     from . import _binding
@@ -376,3 +376,224 @@ def measure_fp32_fma() -> float:
     v = C.c_double(0.0)
     _lib.check(_lib.lib().vs_measure_fp32_fma(C.byref(v)), "vs_measure_fp32_fma")
     return float(v.value)
+
+
+# ---- attention over chosen blocks, and single tokens over a cache (no counterpart in the reference) ------------------------
+
+_DT16 = {torch.float16: VS_F16, torch.bfloat16: VS_BF16}
+BLOCK = 64          # keys of a block, tokens of a page
+RING = 2 * BLOCK    # tokens of a ring
+
+
+def _strided(t: torch.Tensor, name: str, dims: int, dtype=None):
+    """Pointer and host array of the strides of a tensor whose last dimension is contiguous."""
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got {t.dim()}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    return t.data_ptr(), (ctypes.c_int64 * (dims - 1))(*(t.stride(i) if t.shape[i] > 1 else 8 for i in range(dims - 1)))
+
+
+def _shaped(t: torch.Tensor, name: str, shape, dtype):
+    """Pointer of a contiguous tensor of exactly this shape and type; None stays None."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _workspace(t, nbytes: int):
+    """Pointer and size of a workspace of at least `nbytes`."""
+    if not nbytes:
+        return None, 0
+    if t is None or not t.is_contiguous() or t.numel() * t.element_size() < nbytes:
+        raise ValueError(f"the workspace must be a contiguous tensor of {nbytes} bytes or more")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _block_sizes(q, k, blocks):
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q and k must be [batch, tokens, heads, d]")
+    (batch, queries, heads, d), (_, keys, kv_heads, _) = q.shape, k.shape
+    if k.shape[0] != batch or k.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch and width")
+    if kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads cannot share {kv_heads} heads of keys")
+    if blocks.dim() != 4 or blocks.shape[:3] != (batch, kv_heads, queries) or blocks.shape[3] < 1:
+        raise ValueError(f"blocks must have the shape {(batch, kv_heads, queries)} and a count of at least 1, got {tuple(blocks.shape)}")
+    if q.dtype not in _DT16:
+        raise _lib.VsError(-2, "q")
+    return _DT16[q.dtype], batch, queries, keys, heads, kv_heads, d, blocks.shape[3]
+
+
+def select_blocks(q, k, blocks, workspace, causal=True, lengths=None):
+    """Writes the blocks of 64 keys that each query attends to into blocks [B, Hkv, Lq, count] int32 (ascending, -1 behind them): the query's own and the
+    count - 1 with the highest (sum of the group's queries) . (mean of the block's keys) before it; not causal: the count highest.  q [B, Lq, Hq, D], k
+    [B, Lk, Hkv, D], fp16 or bf16, any strides that keep 16-byte alignment; lengths [B] int32: tokens of each entry of a padded batch (Lq == Lk);
+    workspace: select_blocks_workspace(q, k) bytes.  See vs_select_blocks."""
+    sizes = _block_sizes(q, k, blocks)
+    device = _one_device(q=q, k=k, blocks=blocks, workspace=workspace, lengths=lengths)
+    ws, nbytes = _workspace(workspace, select_blocks_workspace(q, k))
+    with torch.cuda.device(device):
+        rc = _lib.lib().vs_select_blocks(*sizes, int(causal), *_strided(q, "q", 4), *_strided(k, "k", 4, q.dtype),
+                                         _shaped(lengths, "lengths", (sizes[1],), torch.int32), _shaped(blocks, "blocks", blocks.shape, torch.int32), ws, nbytes,
+                                         _stream())
+    _lib.check(rc, "vs_select_blocks")
+    return 0
+
+
+def select_blocks_workspace(q, k) -> int:
+    return _lib.lib().vs_select_blocks_workspace_bytes(k.shape[0], k.shape[1], k.shape[2], k.shape[3])
+
+
+def selected_attention_workspace(q, k, backward=False) -> int:
+    return _lib.lib().vs_selected_attention_workspace_bytes(*q.shape[:2], k.shape[1], q.shape[2], *k.shape[2:], int(backward))
+
+
+def selected_attention(q, k, v, blocks, out, lse, workspace, scale, causal=True, lengths=None, out_low=None):
+    """softmax(scale * q k^T) v over the keys of each query's listed blocks, into out (contiguous, as q); lse [B, Hq, Lq] fp32 and out_low (as out: what its
+    rounding left over; or None) are for the backward pass; workspace: selected_attention_workspace(q, k) bytes.  See vs_selected_attention."""
+    sizes = _block_sizes(q, k, blocks)
+    device = _one_device(q=q, k=k, v=v, blocks=blocks, out=out, lse=lse, workspace=workspace, lengths=lengths, out_low=out_low)
+    if v.shape != k.shape:
+        raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
+    ws, nbytes = _workspace(workspace, selected_attention_workspace(q, k))
+    with torch.cuda.device(device):
+        rc = _lib.lib().vs_selected_attention(*sizes, int(causal), *_strided(q, "q", 4), *_strided(k, "k", 4, q.dtype), *_strided(v, "v", 4, q.dtype),
+                                              _shaped(lengths, "lengths", (sizes[1],), torch.int32), _shaped(blocks, "blocks", blocks.shape, torch.int32),
+                                              _shaped(out, "out", q.shape, q.dtype), _shaped(out_low, "out_low", q.shape, q.dtype),
+                                              _shaped(lse, "lse", (q.shape[0], q.shape[2], q.shape[1]), torch.float32), float(scale), ws, nbytes, _stream())
+    _lib.check(rc, "vs_selected_attention")
+    return 0
+
+
+def selected_attention_backward(q, k, v, blocks, out, lse, grad_out, grad_q, grad_k, grad_v, workspace, scale, causal=True, lengths=None, out_low=None):
+    """Gradients of selected_attention (contiguous, as q, k and v) from its results out, lse and, unless None, out_low; workspace: selected_attention_workspace(q, k, True) bytes."""
+    sizes = _block_sizes(q, k, blocks)
+    device = _one_device(q=q, k=k, v=v, blocks=blocks, out=out, lse=lse, grad_out=grad_out, grad_q=grad_q, grad_k=grad_k, grad_v=grad_v, workspace=workspace,
+                         lengths=lengths, out_low=out_low)
+    if v.shape != k.shape or grad_out.shape != q.shape:
+        raise ValueError(f"v and grad_out must have the shapes of k {tuple(k.shape)} and q {tuple(q.shape)}, got {tuple(v.shape)} and {tuple(grad_out.shape)}")
+    ws, nbytes = _workspace(workspace, selected_attention_workspace(q, k, True))
+    with torch.cuda.device(device):
+        rc = _lib.lib().vs_selected_attention_backward(
+            *sizes, int(causal), *_strided(q, "q", 4), *_strided(k, "k", 4, q.dtype), *_strided(v, "v", 4, q.dtype),
+            _shaped(lengths, "lengths", (sizes[1],), torch.int32), _shaped(blocks, "blocks", blocks.shape, torch.int32), _shaped(out, "out", q.shape, q.dtype),
+            _shaped(out_low, "out_low", q.shape, q.dtype), _shaped(lse, "lse", (q.shape[0], q.shape[2], q.shape[1]), torch.float32), *_strided(grad_out, "grad_out", 4, q.dtype),
+            _shaped(grad_q, "grad_q", q.shape, q.dtype), _shaped(grad_k, "grad_k", k.shape, q.dtype), _shaped(grad_v, "grad_v", k.shape, q.dtype), float(scale),
+            ws, nbytes, _stream())
+    _lib.check(rc, "vs_selected_attention_backward")
+    return 0
+
+
+class BlockCache:
+    """Keys and values of many sequences for single-token attention: complete blocks of 64 tokens in 8 bits with a scale for each block and head, the newest
+    tokens in 16 bits.
+
+        k_codes, v_codes    int8  [pages, Hkv, 64, D]        k_scales, v_scales  float32 [pages, Hkv]
+        k_sums              int16 [pages, Hkv, D]            k_ring, v_ring      fp16 or bf16 [tails, Hkv, 128, D]
+
+    Which page holds which block of which sequence, which ring is whose and how long each sequence is, the caller keeps: table [n, max_blocks], tails [n],
+    lengths [n], int32 on the device."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales, k_sums, k_ring, v_ring):
+        if k_codes.dim() != 4 or k_ring.dim() != 4 or k_codes.shape[2] != BLOCK or k_ring.shape[2] != RING:
+            raise ValueError(f"codes must be [pages, heads, {BLOCK}, d] and rings [tails, heads, {RING}, d], got {tuple(k_codes.shape)} and {tuple(k_ring.shape)}")
+        pages, heads, _, d = k_codes.shape
+        if k_ring.dtype not in _DT16:
+            raise _lib.VsError(-2, "k_ring")
+        if k_ring.shape[1] != heads or k_ring.shape[3] != d:
+            raise ValueError(f"codes {tuple(k_codes.shape)} and rings {tuple(k_ring.shape)} must agree in heads and width")
+        for t, name, shape, dtype in ((k_codes, "k_codes", k_codes.shape, torch.int8), (v_codes, "v_codes", k_codes.shape, torch.int8),
+                                      (k_scales, "k_scales", (pages, heads), torch.float32), (v_scales, "v_scales", (pages, heads), torch.float32),
+                                      (k_sums, "k_sums", (pages, heads, d), torch.int16), (k_ring, "k_ring", k_ring.shape, k_ring.dtype),
+                                      (v_ring, "v_ring", k_ring.shape, k_ring.dtype)):
+            _shaped(t, name, shape, dtype)
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.k_sums, self.k_ring, self.v_ring = k_codes, v_codes, k_scales, v_scales, k_sums, k_ring, v_ring
+        self.pages, self.tails, self.kv_heads, self.d, self.dtype = pages, k_ring.shape[0], heads, d, k_ring.dtype
+
+    @classmethod
+    def empty(cls, pages, tails, kv_heads, d, dtype, device):
+        codes = [torch.zeros((pages, kv_heads, BLOCK, d), dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
+        rings = [torch.zeros((tails, kv_heads, RING, d), dtype=dtype, device=device) for _ in range(2)]
+        return cls(*codes, *scales, torch.zeros((pages, kv_heads, d), dtype=torch.int16, device=device), *rings)
+
+    def _tensors(self):
+        return dict(k_codes=self.k_codes, v_codes=self.v_codes, k_scales=self.k_scales, v_scales=self.v_scales, k_sums=self.k_sums, k_ring=self.k_ring,
+                    v_ring=self.v_ring)
+
+
+def _table(table, n):
+    if table.dim() != 2 or table.shape[0] != n:
+        raise ValueError(f"table must be [{n}, blocks], got {tuple(table.shape)}")
+    return _shaped(table, "table", table.shape, torch.int32), table.shape[1]
+
+
+def cache_append(cache, k, v, table, tails, lengths, counts=None):
+    """Appends k, v [n, T, Hkv, D] (counts[r] <= T tokens of sequence r; None: T) behind lengths [n]; blocks that become complete are rounded into their
+    pages.  lengths is the caller's to advance.  See vs_cache_append."""
+    device = _one_device(k=k, v=v, table=table, tails=tails, lengths=lengths, counts=counts, **cache._tensors())
+    if k.dim() != 4 or k.shape[2:] != (cache.kv_heads, cache.d) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [n, tokens, {cache.kv_heads}, {cache.d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    n, tokens = k.shape[:2]
+    c = cache
+    with torch.cuda.device(device):
+        rc = _lib.lib().vs_cache_append(
+            _DT16[c.dtype], c.pages, c.tails, c.kv_heads, c.d, c.k_codes.data_ptr(), c.v_codes.data_ptr(), c.k_scales.data_ptr(), c.v_scales.data_ptr(),
+            c.k_sums.data_ptr(), c.k_ring.data_ptr(), c.v_ring.data_ptr(), n, tokens, *_strided(k, "k", 4, c.dtype), *_strided(v, "v", 4, c.dtype),
+            *_table(table, n), _shaped(tails, "tails", (n,), torch.int32), _shaped(lengths, "lengths", (n,), torch.int32),
+            _shaped(counts, "counts", (n,), torch.int32), _stream())
+    _lib.check(rc, "vs_cache_append")
+    return 0
+
+
+def _token_sizes(q, cache):
+    if q.dim() != 3 or q.shape[2] != cache.d or q.shape[1] < cache.kv_heads or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"q must be [n, heads, {cache.d}] with a multiple of {cache.kv_heads} heads, got {tuple(q.shape)}")
+    return q.shape[:2]
+
+
+def cache_select(q, cache, table, lengths, blocks):
+    """Writes the complete blocks that the newest token of each sequence attends to into blocks [n, Hkv, count] int32: the newest and the count - 1 with the
+    highest (sum of the group's queries) . (sum of the block's codes) * scale.  q [n, Hq, D].  See vs_cache_select."""
+    device = _one_device(q=q, table=table, lengths=lengths, blocks=blocks, **cache._tensors())
+    n, heads = _token_sizes(q, cache)
+    if blocks.dim() != 3 or blocks.shape[:2] != (n, cache.kv_heads):
+        raise ValueError(f"blocks must be [{n}, {cache.kv_heads}, count], got {tuple(blocks.shape)}")
+    with torch.cuda.device(device):
+        rc = _lib.lib().vs_cache_select(_DT16[cache.dtype], cache.pages, heads, cache.kv_heads, cache.d, cache.k_scales.data_ptr(), cache.k_sums.data_ptr(), n,
+                                        *_strided(q, "q", 3, cache.dtype), *_table(table, n), _shaped(lengths, "lengths", (n,), torch.int32), blocks.shape[2],
+                                        _shaped(blocks, "blocks", blocks.shape, torch.int32), _stream())
+    _lib.check(rc, "vs_cache_select")
+    return 0
+
+
+def cache_attention_workspace(q, cache, table, blocks=None) -> int:
+    return _lib.lib().vs_cache_attention_workspace_bytes(q.shape[0], q.shape[1], cache.kv_heads, cache.d, table.shape[1] if blocks is None else blocks.shape[2])
+
+
+def cache_attention(q, cache, table, tails, lengths, out, workspace, scale, blocks=None):
+    """Attention of the newest token of each sequence, q [n, Hq, D], over its complete blocks (all, or those in blocks [n, Hkv, count]) and the tokens behind
+    them, into out (contiguous, as q); workspace: cache_attention_workspace(...) bytes or None where that is 0.  See vs_cache_attention."""
+    device = _one_device(q=q, table=table, tails=tails, lengths=lengths, out=out, workspace=workspace, blocks=blocks, **cache._tensors())
+    n, heads = _token_sizes(q, cache)
+    c = cache
+    if blocks is not None and (blocks.dim() != 3 or blocks.shape[:2] != (n, c.kv_heads)):
+        raise ValueError(f"blocks must be [{n}, {c.kv_heads}, count], got {tuple(blocks.shape)}")
+    ws, nbytes = _workspace(workspace, cache_attention_workspace(q, c, table, blocks))
+    with torch.cuda.device(device):
+        rc = _lib.lib().vs_cache_attention(
+            _DT16[c.dtype], c.pages, c.tails, heads, c.kv_heads, c.d, c.k_codes.data_ptr(), c.v_codes.data_ptr(), c.k_scales.data_ptr(), c.v_scales.data_ptr(),
+            c.k_ring.data_ptr(), c.v_ring.data_ptr(), n, *_strided(q, "q", 3, c.dtype), *_table(table, n), _shaped(tails, "tails", (n,), torch.int32),
+            _shaped(lengths, "lengths", (n,), torch.int32), None if blocks is None else _shaped(blocks, "blocks", blocks.shape, torch.int32),
+            0 if blocks is None else blocks.shape[2], _shaped(out, "out", q.shape, c.dtype), float(scale), ws, nbytes, _stream())
+    _lib.check(rc, "vs_cache_attention")
+    return 0

@@ -197,3 +197,114 @@ def _backward(which, mask, path, scale, saved, grad, wanted):
 
 
 ops._binding.bind_backward(_backward)
+
+
+# ---- attention over chosen blocks, and single tokens over a cache ------------------------------------------------------------
+
+BlockCache = ops.BlockCache
+
+_LIB.define("select_blocks(Tensor q, Tensor k, int count, bool causal, Tensor? lengths) -> Tensor")
+_LIB.define("selected_attention(Tensor q, Tensor k, Tensor v, Tensor blocks, float scale, bool causal, Tensor? lengths, bool low) -> (Tensor, Tensor, Tensor?)")
+_LIB.define("selected_attention_backward(Tensor q, Tensor k, Tensor v, Tensor blocks, Tensor out, Tensor? out_low, Tensor lse, Tensor grad_out, float scale, "
+            "bool causal, Tensor? lengths) -> (Tensor, Tensor, Tensor)")
+
+
+def _usable(t):
+    """t where the kernels take its layout, else a contiguous copy."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _scratch(nbytes, device):
+    return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _select_blocks(q, k, count, causal, lengths):
+    q, k = _usable(q), _usable(k)
+    blocks = torch.empty((q.shape[0], k.shape[2], q.shape[1], count), dtype=torch.int32, device=q.device)
+    ops.select_blocks(q, k, blocks, _scratch(ops.select_blocks_workspace(q, k), q.device), causal, lengths)
+    return blocks
+
+
+def _selected_attention(q, k, v, blocks, scale, causal, lengths, low):
+    q, k, v = _usable(q), _usable(k), _usable(v)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out_low = torch.empty_like(out) if low else None
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+    ops.selected_attention(q, k, v, blocks, out, lse, _scratch(ops.selected_attention_workspace(q, k), q.device), scale, causal, lengths, out_low)
+    return out, lse, out_low
+
+
+def _selected_attention_backward(q, k, v, blocks, out, out_low, lse, grad_out, scale, causal, lengths):
+    q, k, v, grad_out = _usable(q), _usable(k), _usable(v), _usable(grad_out)
+    gq, gk, gv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+    ops.selected_attention_backward(q, k, v, blocks, out, lse, grad_out, gq, gk, gv, _scratch(ops.selected_attention_workspace(q, k, True), q.device), scale,
+                                    causal, lengths, out_low)
+    return gq, gk, gv
+
+
+_LIB.impl("select_blocks", _select_blocks, "CUDA")
+_LIB.impl("selected_attention", _selected_attention, "CUDA")
+_LIB.impl("selected_attention_backward", _selected_attention_backward, "CUDA")
+
+
+def select_blocks(q, k, count, causal=True, lengths=None):
+    """[B, Hkv, Lq, count] int32: the blocks of 64 keys that each query attends to (see ops.select_blocks).  A choice has no gradient."""
+    with torch.no_grad():
+        return _through(_select_blocks, torch.ops.vsparse.select_blocks, (q, k), q, k, int(count), bool(causal), lengths)
+
+
+class SelectedAttention(torch.autograd.Function):
+    """softmax(scale * Q K^T at the chosen blocks) V and its gradients by the library's two operators."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, blocks, scale: float, causal: bool, lengths):
+        low = any(ctx.needs_input_grad[:2])   # what only the gradients of q and k read
+        out, lse, out_low = _through(_selected_attention, torch.ops.vsparse.selected_attention, (q, k, v, blocks), q, k, v, blocks, scale, causal, lengths, low)
+        ctx.save_for_backward(q, k, v, blocks, out, out_low, lse, lengths)
+        ctx.scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, blocks, out, out_low, lse, lengths = ctx.saved_tensors
+        grads = _through(_selected_attention_backward, torch.ops.vsparse.selected_attention_backward, (q, k, v, grad_out), q, k, v, blocks, out, out_low, lse, grad_out,
+                         ctx.scale, ctx.causal, lengths)
+        return (*grads, None, None, None, None)
+
+
+def selected_attention(q, k, v, blocks, scale, causal=True, lengths=None):
+    """Attention of q [B, Lq, Hq, D] over the keys of each query's blocks [B, Hkv, Lq, count]; k, v [B, Lk, Hkv, D]; fp16 or bf16; differentiable in q, k, v.
+
+        blocks = select_blocks(q, k, 16)
+        out = selected_attention(q, k, v, blocks, D ** -0.5)
+
+    lengths [B] int32: tokens of each entry of a padded batch (Lq == Lk).  See ops.selected_attention."""
+    return SelectedAttention.apply(q, k, v, blocks, float(scale), bool(causal), lengths)
+
+
+def cache_append(cache, k, v, table, tails, lengths, counts=None):
+    """Appends k, v [n, T, Hkv, D] to the cache behind lengths [n] (see ops.cache_append); advancing lengths is the caller's."""
+    with torch.no_grad():
+        ops.cache_append(cache, _usable(k), _usable(v), table, tails, lengths, counts)
+
+
+def cache_select(q, cache, table, lengths, count):
+    """[n, Hkv, count] int32: the complete blocks that the newest token of each sequence attends to (see ops.cache_select)."""
+    with torch.no_grad():
+        q = _usable(q)
+        blocks = torch.empty((q.shape[0], cache.kv_heads, count), dtype=torch.int32, device=q.device)
+        ops.cache_select(q, cache, table, lengths, blocks)
+        return blocks
+
+
+def cache_attention(q, cache, table, tails, lengths, scale, blocks=None):
+    """Attention of the newest token of each sequence, q [n, Hq, D], over the cache: all of it, or the chosen blocks (see ops.cache_attention).  For inference: no
+    gradient is recorded."""
+    with torch.no_grad():
+        q = _usable(q)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ops.cache_attention(q, cache, table, tails, lengths, out, _scratch(ops.cache_attention_workspace(q, cache, table, blocks), q.device), scale, blocks)
+        return out
