@@ -9,12 +9,14 @@
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 #include <utility>
 
 #include "vsparse_b200.h"
 #include "common.cuh"
 #include "host.h"
 #include "blocks.cuh"
+#include "blocks_tc.cuh"
 #include "cache.cuh"
 
 #define VS_EXPORT extern "C" __attribute__((visibility("default")))
@@ -97,6 +99,8 @@ void contiguous(blocks::Operand &o, const void *at, int64_t tokens, int64_t head
 inline int64_t up256(int64_t bytes) { return (bytes + 255) & ~255ll; }
 inline int64_t bits_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * s.words * s.blocks * 4); }
 
+inline int64_t redo_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * ((int64_t)s.queries + s.blocks) * 4); }   // a word per tile and block
+
 // Queries of a tile: the largest power of two whose rows (queries x heads of the group) fit 128.
 inline int tile_queries(int group) {
     int t = 128;
@@ -131,11 +135,55 @@ int make_bits(const blocks::Shape &s, const int32_t *lists, uint32_t *bits, cuda
     return (int)cudaGetLastError();
 }
 
-template <typename T> int attention(blocks::Args a, cudaStream_t st) {
+// {d, heads, tokens, batch} of an operand, for copies of 64 dimensions of `heads` heads of `tokens` tokens, 128-byte swizzle; zeros outside.
+template <typename T> int make_map(CUtensorMap *map, const blocks::Operand &o, int64_t batch, int64_t tokens, int64_t heads, int64_t d, int box_heads, int box_tokens) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return VS_ERR_DEVICE;
+    auto bytes = [](int64_t stride, int64_t extent) { return (cuuint64_t)(extent > 1 ? stride * 2 : 16); };   // of one, any will do
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
+    const cuuint64_t strides[3] = {bytes(o.head, heads), bytes(o.token, tokens), bytes(o.batch, batch)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens, 1}, unit[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return fn(map, type, 4, const_cast<void *>(o.at), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? VS_OK
+               : VS_ERR_ARG;
+}
+// Tiles of a call and the words that say which of them are to be computed again, one by one.
+inline int64_t query_tiles(const blocks::Shape &s) {
+    const int tile = tile_queries(s.group);
+    return (int64_t)s.batch * s.kv_heads * ((s.queries + tile - 1) / tile);
+}
+inline unsigned again_grid(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 4 * 148); }
+
+template <typename T, int DP> int forward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
     const blocks::Shape &s = a.s;
-    a.tile = 1;
-    blocks::rows_kernel<T, false><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.queries), blocks::kRowThreads, 0, st>>>(a);
-    return (int)cudaGetLastError();
+    using Smem = blocks::tcore::ForwardSmem<DP>;
+    CUtensorMap q, k, v;
+    a.tile = tile_queries(s.group);
+    int rc = make_map<T>(&q, a.q, s.batch, s.queries, s.heads, s.d, s.group, a.tile);
+    if (rc == VS_OK) rc = make_map<T>(&k, a.k, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
+    if (rc == VS_OK) rc = make_map<T>(&v, a.v, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
+    if (rc == VS_OK) rc = allow_smem<blocks::tcore::forward_kernel<T, DP>>(Smem::kBytes + 1024);
+    if (rc != VS_OK) return rc;
+    const int64_t tiles = query_tiles(s);
+    cudaError_t e = launch_behind(blocks::tcore::forward_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kForwardThreads, Smem::kBytes + 1024, st, a, q, k, v, redo, status);
+    if (e != cudaSuccess) return (int)e;
+    a.redo = redo;
+    return (int)launch_behind(blocks::rows_kernel<T, false>, again_grid(tiles), blocks::kRowThreads, 0, st, a);
+}
+template <typename T> int attention(blocks::Args a, uint32_t *redo, cudaStream_t st) {
+    const blocks::Shape &s = a.s;
+    if (s.keys == 0) {   // no key to attend to
+        a.tile = tile_queries(s.group);
+        blocks::rows_kernel<T, false><<<again_grid(query_tiles(s)), blocks::kRowThreads, 0, st>>>(a);
+        return (int)cudaGetLastError();
+    }
+    int sms = 0;
+    uint32_t *status = nullptr;
+    const int rc = current_device(&sms, &status);
+    if (rc != VS_OK) return rc;
+    return s.d <= 64 ? forward<T, 64>(a, redo, status, st) : forward<T, 128>(a, redo, status, st);
 }
 template <typename T> int attention_backward(blocks::Args a, void *grad_q, cudaStream_t st) {
     const blocks::Shape &s = a.s;
@@ -143,9 +191,9 @@ template <typename T> int attention_backward(blocks::Args a, void *grad_q, cudaS
     blocks::delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
-    a.tile = 1;
+    a.tile = tile_queries(s.group);
     a.result = grad_q;
-    blocks::rows_kernel<T, true><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.queries), blocks::kRowThreads, 0, st>>>(a);
+    blocks::rows_kernel<T, true><<<(unsigned)query_tiles(s), blocks::kRowThreads, 0, st>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
     blocks::keys_kernel<T><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.blocks), blocks::kRowThreads, 0, st>>>(a);
@@ -182,7 +230,7 @@ VS_EXPORT int vs_select_blocks(int dtype, int batch, int queries, int keys, int 
 VS_EXPORT int64_t vs_selected_attention_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int d, int backward) {
     blocks::Shape s;
     if (check_shape(VS_F16, batch, queries, keys, heads, kv_heads, d, 1, 0, nullptr, s) != VS_OK) return 0;
-    return bits_bytes(s) + (backward ? up256((int64_t)batch * heads * queries * 4) : 0);
+    return bits_bytes(s) + redo_bytes(s) + (backward ? up256((int64_t)batch * heads * queries * 4) : 0);
 }
 
 VS_EXPORT int vs_selected_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const void *q,
@@ -203,7 +251,8 @@ VS_EXPORT int vs_selected_attention(int dtype, int batch, int queries, int keys,
     uint32_t *bits = static_cast<uint32_t *>(workspace);
     if ((rc = make_bits(a.s, lists, bits, st)) != VS_OK) return rc;
     a.bits = bits; a.lse = lse; a.result = out; a.result_low = out_low; a.scale = scale;
-    return dtype == VS_F16 ? attention<__half>(a, st) : attention<__nv_bfloat16>(a, st);
+    uint32_t *redo = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + bits_bytes(a.s));
+    return dtype == VS_F16 ? attention<__half>(a, redo, st) : attention<__nv_bfloat16>(a, redo, st);
 }
 
 VS_EXPORT int vs_selected_attention_backward(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal,
@@ -237,7 +286,7 @@ VS_EXPORT int vs_selected_attention_backward(int dtype, int batch, int queries, 
     uint32_t *bits = static_cast<uint32_t *>(workspace);
     if ((rc = make_bits(a.s, lists, bits, st)) != VS_OK) return rc;
     a.bits = bits; a.lse = const_cast<float *>(lse); a.scale = scale;
-    a.delta = reinterpret_cast<float *>(static_cast<char *>(workspace) + bits_bytes(a.s));
+    a.delta = reinterpret_cast<float *>(static_cast<char *>(workspace) + bits_bytes(a.s) + redo_bytes(a.s));
     a.grad_k = grad_k; a.grad_v = grad_v;
     return dtype == VS_F16 ? attention_backward<__half>(a, grad_q, st) : attention_backward<__nv_bfloat16>(a, grad_q, st);
 }

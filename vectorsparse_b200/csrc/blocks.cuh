@@ -13,6 +13,10 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <type_traits>
+
+#include "common.cuh"
+
 namespace vs {
 namespace blocks {
 
@@ -59,6 +63,7 @@ template <typename T> __device__ __forceinline__ void load8(const T *p, float (&
 constexpr int kBitsThreads = 128, kBitsChunk = 4096;
 __global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const int32_t *lists, uint32_t *bits) {
     __shared__ uint32_t row[kBitsChunk];
+    pdl_launch_dependents();
     const int64_t at = blockIdx.x;
     const int w = (int)(at % s.words);
     const int b = (int)(at / s.words / s.kv_heads);
@@ -286,137 +291,142 @@ __device__ __forceinline__ float warp_sum(float x) {
 
 template <typename T, bool kBackward> __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Args a) {
     __shared__ float q_s[kRowWarps][kMaxD], g_s[kRowWarps][kMaxD];
-    if (a.redo && a.redo[blockIdx.x] == 0) return;
+    pdl_wait();
     const Shape &s = a.s;
-    const int tiles = (s.queries + a.tile - 1) / a.tile;
-    const int64_t bh = blockIdx.x / tiles;
-    const int i0 = (int)(blockIdx.x % tiles) * a.tile, kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, len = s.length(b);
-    const T *kp = static_cast<const T *>(a.k.at) + b * a.k.batch + kvh * a.k.head;
-    const T *vp = static_cast<const T *>(a.v.at) + b * a.v.batch + kvh * a.v.head;
-    const float c = a.scale * kLog2e;
-    for (int r = warp; r < a.tile * s.group; r += kRowWarps) {
-        const int i = i0 + r / s.group, h = kvh * s.group + r % s.group;
-        if (i >= s.queries) break;
-        const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
-        const T *qp = static_cast<const T *>(a.q.at) + b * a.q.batch + (int64_t)i * a.q.token + h * a.q.head;
-        const T *gp = kBackward ? static_cast<const T *>(a.grad_out.at) + b * a.grad_out.batch + (int64_t)i * a.grad_out.token + h * a.grad_out.head : nullptr;
-        __syncwarp();
-        for (int x = lane; x < s.d; x += 32) {
-            q_s[warp][x] = to_f32(qp[x]);
-            if (kBackward) g_s[warp][x] = to_f32(gp[x]);
-        }
-        __syncwarp();
-        const int end = s.end(i, len);
-        const uint32_t *bits = a.bits + (bh * s.words + (i >> 5)) * s.blocks;
-        float top = -INFINITY, total = 0.f, acc[kMaxD / 32] = {};
-        const float lse = kBackward ? a.lse[row] : 0.f, delta = kBackward ? a.delta[row] : 0.f;
-        for (int j = 0; j < s.blocks; ++j) {
-            if (!(bits[j] >> (i & 31) & 1u)) continue;
-            const int n = min(kBlock, end - j * kBlock);
-            float w[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int t = lane + 32 * x;
-                w[x] = -INFINITY;
-                if (t < n) w[x] = dot_row(q_s[warp], kp + (int64_t)(j * kBlock + t) * a.k.token, s.d) * c;
+    const int tiles = (s.queries + a.tile - 1) / a.tile, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int64_t index = blockIdx.x; index < (int64_t)s.batch * s.kv_heads * tiles; index += gridDim.x) {
+        if (a.redo && a.redo[index] == 0) continue;
+        const int64_t bh = index / tiles;
+        const int i0 = (int)(index % tiles) * a.tile, kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads), len = s.length(b);
+        const T *kp = static_cast<const T *>(a.k.at) + b * a.k.batch + kvh * a.k.head;
+        const T *vp = static_cast<const T *>(a.v.at) + b * a.v.batch + kvh * a.v.head;
+        const float c = a.scale * kLog2e;
+        for (int r = warp; r < a.tile * s.group; r += kRowWarps) {
+            const int i = i0 + r / s.group, h = kvh * s.group + r % s.group;
+            if (i >= s.queries) break;
+            const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+            const T *qp = static_cast<const T *>(a.q.at) + b * a.q.batch + (int64_t)i * a.q.token + h * a.q.head;
+            const T *gp = kBackward ? static_cast<const T *>(a.grad_out.at) + b * a.grad_out.batch + (int64_t)i * a.grad_out.token + h * a.grad_out.head : nullptr;
+            __syncwarp();
+            for (int x = lane; x < s.d; x += 32) {
+                q_s[warp][x] = to_f32(qp[x]);
+                if (kBackward) g_s[warp][x] = to_f32(gp[x]);
             }
-            if (!kBackward) {
-                const float m = fmaxf(top, warp_max(fmaxf(w[0], w[1]))), base = m == -INFINITY ? 0.f : m;
-                const float shrink = exp2f(top - base);
-                w[0] = lane < n ? exp2f(w[0] - base) : 0.f;
-                w[1] = lane + 32 < n ? exp2f(w[1] - base) : 0.f;
-                total = total * shrink + warp_sum(w[0] + w[1]);
-                top = m;
-#pragma unroll
-                for (int x = 0; x < kMaxD / 32; ++x) acc[x] *= shrink;
-            } else {
+            __syncwarp();
+            const int end = s.end(i, len);
+            const uint32_t *bits = a.bits + (bh * s.words + (i >> 5)) * s.blocks;
+            float top = -INFINITY, total = 0.f, acc[kMaxD / 32] = {};
+            const float lse = kBackward ? a.lse[row] : 0.f, delta = kBackward ? a.delta[row] : 0.f;
+            for (int j = 0; j < s.blocks; ++j) {
+                if (!(bits[j] >> (i & 31) & 1u)) continue;
+                const int n = min(kBlock, end - j * kBlock);
+                float w[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int t = lane + 32 * x;
-                    float ds = 0.f;
-                    if (t < n) ds = exp2f(w[x] - lse) * (dot_row(g_s[warp], vp + (int64_t)(j * kBlock + t) * a.v.token, s.d) - delta) * a.scale;
-                    w[x] = ds;
+                    w[x] = -INFINITY;
+                    if (t < n) w[x] = dot_row(q_s[warp], kp + (int64_t)(j * kBlock + t) * a.k.token, s.d) * c;
+                }
+                if (!kBackward) {
+                    const float m = fmaxf(top, warp_max(fmaxf(w[0], w[1]))), base = m == -INFINITY ? 0.f : m;
+                    const float shrink = exp2f(top - base);
+                    w[0] = lane < n ? exp2f(w[0] - base) : 0.f;
+                    w[1] = lane + 32 < n ? exp2f(w[1] - base) : 0.f;
+                    total = total * shrink + warp_sum(w[0] + w[1]);
+                    top = m;
+#pragma unroll
+                    for (int x = 0; x < kMaxD / 32; ++x) acc[x] *= shrink;
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int t = lane + 32 * x;
+                        float ds = 0.f;
+                        if (t < n) ds = exp2f(w[x] - lse) * (dot_row(g_s[warp], vp + (int64_t)(j * kBlock + t) * a.v.token, s.d) - delta) * a.scale;
+                        w[x] = ds;
+                    }
+                }
+                for (int t = 0; t < n; ++t) {
+                    const float p = __shfl_sync(~0u, t < 32 ? w[0] : w[1], t & 31);
+                    const T *row_t = (kBackward ? kp : vp) + (int64_t)(j * kBlock + t) * (kBackward ? a.k.token : a.v.token);
+#pragma unroll
+                    for (int x = 0; x < kMaxD / 32; ++x)
+                        if (lane + 32 * x < s.d) acc[x] = fmaf(p, to_f32(row_t[lane + 32 * x]), acc[x]);
                 }
             }
-            for (int t = 0; t < n; ++t) {
-                const float p = __shfl_sync(~0u, t < 32 ? w[0] : w[1], t & 31);
-                const T *row_t = (kBackward ? kp : vp) + (int64_t)(j * kBlock + t) * (kBackward ? a.k.token : a.v.token);
+            const int64_t at = (((int64_t)b * s.queries + i) * s.heads + h) * s.d;
 #pragma unroll
-                for (int x = 0; x < kMaxD / 32; ++x)
-                    if (lane + 32 * x < s.d) acc[x] = fmaf(p, to_f32(row_t[lane + 32 * x]), acc[x]);
-            }
+            for (int x = 0; x < kMaxD / 32; ++x)
+                if (lane + 32 * x < s.d) {
+                    const float y = kBackward ? acc[x] : total == 0.f ? 0.f : acc[x] / total;
+                    const T high = from_f32<T>(y);
+                    static_cast<T *>(a.result)[at + lane + 32 * x] = high;
+                    if (!kBackward && a.result_low) static_cast<T *>(a.result_low)[at + lane + 32 * x] = from_f32<T>(y - to_f32(high));
+                }
+            if (!kBackward && lane == 0) a.lse[row] = total == 0.f ? INFINITY : top + log2f(total);
         }
-        const int64_t at = (((int64_t)b * s.queries + i) * s.heads + h) * s.d;
-#pragma unroll
-        for (int x = 0; x < kMaxD / 32; ++x)
-            if (lane + 32 * x < s.d) {
-                const float y = kBackward ? acc[x] : total == 0.f ? 0.f : acc[x] / total;
-                const T high = from_f32<T>(y);
-                static_cast<T *>(a.result)[at + lane + 32 * x] = high;
-                if (!kBackward && a.result_low) static_cast<T *>(a.result_low)[at + lane + 32 * x] = from_f32<T>(y - to_f32(high));
-            }
-        if (!kBackward && lane == 0) a.lse[row] = total == 0.f ? INFINITY : top + log2f(total);
     }
 }
 
 // dK and dV of the keys of one block: a warp takes a key, its lanes the queries of a word for the scores and then the dimensions for the sums.
 template <typename T> __global__ void __launch_bounds__(kRowThreads) keys_kernel(const Args a) {
     __shared__ float k_s[kRowWarps][kMaxD], v_s[kRowWarps][kMaxD];
-    if (a.redo && a.redo[blockIdx.x] == 0) return;
+    pdl_wait();
     const Shape &s = a.s;
-    const int64_t bh = blockIdx.x / s.blocks;
-    const int j = (int)(blockIdx.x % s.blocks), kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, len = s.length(b);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float c = a.scale * kLog2e;
-    for (int t = j * kBlock + warp; t < min(s.keys, (j + 1) * kBlock); t += kRowWarps) {
-        float dk[kMaxD / 32] = {}, dv[kMaxD / 32] = {};
-        if (t < len) {
-            const T *kp = static_cast<const T *>(a.k.at) + b * a.k.batch + (int64_t)t * a.k.token + kvh * a.k.head;
-            const T *vp = static_cast<const T *>(a.v.at) + b * a.v.batch + (int64_t)t * a.v.token + kvh * a.v.head;
-            __syncwarp();
-            for (int x = lane; x < s.d; x += 32) {
-                k_s[warp][x] = to_f32(kp[x]);
-                v_s[warp][x] = to_f32(vp[x]);
-            }
-            __syncwarp();
-            for (int w = 0; w < s.words; ++w) {
-                const int i = w * 32 + lane;
-                const bool here = (a.bits[(bh * s.words + w) * s.blocks + j] >> lane & 1u) && t < s.end(i, len);
-                const uint32_t rows = __ballot_sync(~0u, here);
-                if (!rows) continue;
-                for (int g = 0; g < s.group; ++g) {
-                    const int h = kvh * s.group + g;
-                    const T *qp = static_cast<const T *>(a.q.at) + b * a.q.batch + h * a.q.head;
-                    const T *gp = static_cast<const T *>(a.grad_out.at) + b * a.grad_out.batch + h * a.grad_out.head;
-                    float p = 0.f, ds = 0.f;
-                    if (here) {
-                        const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
-                        p = exp2f(dot_row(k_s[warp], qp + (int64_t)i * a.q.token, s.d) * c - a.lse[row]);
-                        ds = p * (dot_row(v_s[warp], gp + (int64_t)i * a.grad_out.token, s.d) - a.delta[row]) * a.scale;
-                    }
-                    for (uint32_t left = rows; left; left &= left - 1) {
-                        const int x = __ffs(left) - 1;
-                        const float px = __shfl_sync(~0u, p, x), dx = __shfl_sync(~0u, ds, x);
+    for (int64_t index = blockIdx.x; index < (int64_t)s.batch * s.kv_heads * s.blocks; index += gridDim.x) {
+        if (a.redo && a.redo[index] == 0) continue;
+        const int64_t bh = index / s.blocks;
+        const int j = (int)(index % s.blocks), kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads), len = s.length(b);
+        for (int t = j * kBlock + warp; t < min(s.keys, (j + 1) * kBlock); t += kRowWarps) {
+            float dk[kMaxD / 32] = {}, dv[kMaxD / 32] = {};
+            if (t < len) {
+                const T *kp = static_cast<const T *>(a.k.at) + b * a.k.batch + (int64_t)t * a.k.token + kvh * a.k.head;
+                const T *vp = static_cast<const T *>(a.v.at) + b * a.v.batch + (int64_t)t * a.v.token + kvh * a.v.head;
+                __syncwarp();
+                for (int x = lane; x < s.d; x += 32) {
+                    k_s[warp][x] = to_f32(kp[x]);
+                    v_s[warp][x] = to_f32(vp[x]);
+                }
+                __syncwarp();
+                for (int w = 0; w < s.words; ++w) {
+                    const int i = w * 32 + lane;
+                    const bool here = (a.bits[(bh * s.words + w) * s.blocks + j] >> lane & 1u) && t < s.end(i, len);
+                    const uint32_t rows = __ballot_sync(~0u, here);
+                    if (!rows) continue;
+                    for (int g = 0; g < s.group; ++g) {
+                        const int h = kvh * s.group + g;
+                        const T *qp = static_cast<const T *>(a.q.at) + b * a.q.batch + h * a.q.head;
+                        const T *gp = static_cast<const T *>(a.grad_out.at) + b * a.grad_out.batch + h * a.grad_out.head;
+                        float p = 0.f, ds = 0.f;
+                        if (here) {
+                            const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+                            p = exp2f(dot_row(k_s[warp], qp + (int64_t)i * a.q.token, s.d) * c - a.lse[row]);
+                            ds = p * (dot_row(v_s[warp], gp + (int64_t)i * a.grad_out.token, s.d) - a.delta[row]) * a.scale;
+                        }
+                        for (uint32_t left = rows; left; left &= left - 1) {
+                            const int x = __ffs(left) - 1;
+                            const float px = __shfl_sync(~0u, p, x), dx = __shfl_sync(~0u, ds, x);
 #pragma unroll
-                        for (int y = 0; y < kMaxD / 32; ++y) {
-                            const int e = lane + 32 * y;
-                            if (e < s.d) {
-                                dv[y] = fmaf(px, to_f32(gp[(int64_t)(w * 32 + x) * a.grad_out.token + e]), dv[y]);
-                                dk[y] = fmaf(dx, to_f32(qp[(int64_t)(w * 32 + x) * a.q.token + e]), dk[y]);
+                            for (int y = 0; y < kMaxD / 32; ++y) {
+                                const int e = lane + 32 * y;
+                                if (e < s.d) {
+                                    dv[y] = fmaf(px, to_f32(gp[(int64_t)(w * 32 + x) * a.grad_out.token + e]), dv[y]);
+                                    dk[y] = fmaf(dx, to_f32(qp[(int64_t)(w * 32 + x) * a.q.token + e]), dk[y]);
+                                }
                             }
                         }
                     }
                 }
             }
-        }
-        const int64_t at = (((int64_t)b * s.keys + t) * s.kv_heads + kvh) * s.d;
+            const int64_t at = (((int64_t)b * s.keys + t) * s.kv_heads + kvh) * s.d;
 #pragma unroll
-        for (int y = 0; y < kMaxD / 32; ++y)
-            if (lane + 32 * y < s.d) {
-                static_cast<T *>(a.grad_k)[at + lane + 32 * y] = from_f32<T>(dk[y]);
-                static_cast<T *>(a.grad_v)[at + lane + 32 * y] = from_f32<T>(dv[y]);
-            }
+            for (int y = 0; y < kMaxD / 32; ++y)
+                if (lane + 32 * y < s.d) {
+                    static_cast<T *>(a.grad_k)[at + lane + 32 * y] = from_f32<T>(dk[y]);
+                    static_cast<T *>(a.grad_v)[at + lane + 32 * y] = from_f32<T>(dv[y]);
+                }
+        }
     }
 }
 

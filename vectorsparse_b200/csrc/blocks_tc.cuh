@@ -1,0 +1,409 @@
+// Attention over chosen blocks on the tensor cores (tcgen05).
+//
+// A tile is 128 rows: `tile` consecutive queries times the heads of a group, one head of keys.  It goes through the union of its queries' lists, a
+// block of 64 keys at a time; a row that has not listed a block gets weights of 0 there.  Neighbouring queries choose mostly alike, so the union is not
+// much longer than a list, and tiles of full height are what the tensor cores need: gathering each query's own blocks instead reads 32 KB of keys and values
+// (d = 128) for a product of `group` rows, and is bound by L2 many times over.
+//
+// A multiplied tile knows nothing of single keys: 0 * Inf in it is a NaN that the operator does not have.  So a tile whose result is not finite says so in its
+// word of `redo`, and the row kernels behind compute it again; they read only what a row attends to.
+#pragma once
+#include <cuda.h>
+
+#include "blocks.cuh"
+#include "common.cuh"
+#include "tc_ptx.cuh"
+
+namespace vs {
+namespace blocks {
+namespace tcore {
+
+constexpr uint32_t kStatusForward = 512u, kStatusGradQ = 1024u, kStatusGradKV = 2048u;   // bits raised in the status word when a bounded wait ran out
+constexpr int kRows = 128;
+constexpr uint32_t kBf16Operands = (1u << 7) | (1u << 10);
+template <typename T> __host__ __device__ constexpr uint32_t idesc(int n, int a_mn, int b_mn) {
+    return tc::make_idesc_f16(kRows, n, a_mn, b_mn) | (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? kBf16Operands : 0u);
+}
+
+// Waits for a phase, or until another role of the CTA has given up; gives up itself after as many polls as the other tensor kernels.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
+    for (uint32_t i = 0; i < tc::kMaxPolls; ++i) {
+        if (tc::mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ bool finite(float x) { return x * 0.f == 0.f; }
+
+// A block that a tile goes through: its number (-1: no more) and which of the tile's queries have listed it.
+struct __align__(16) Entry {
+    uint32_t rows[4];
+    int32_t block;
+    int32_t pad[3];
+};
+constexpr int kEntries = 8;   // in a ring: more than there are blocks between the loader and the softmax
+
+struct Tile {   // where a CTA's tile lies
+    int b, kvh, i0;
+    int64_t bh, index;   // index: among all tiles, in the order of the queries
+};
+__device__ __forceinline__ Tile tile_of(const Shape &s, int tile, int64_t index) {
+    const int tiles = (s.queries + tile - 1) / tile;
+    Tile t;
+    t.bh = index / tiles;
+    t.i0 = (tiles - 1 - (int)(index % tiles)) * tile;   // the last queries have most keys before them: they go first
+    t.kvh = (int)(t.bh % s.kv_heads);
+    t.b = (int)(t.bh / s.kv_heads);
+    t.index = t.bh * tiles + t.i0 / tile;
+    return t;
+}
+
+// The blocks that a tile of queries has listed, in ascending order, found by a warp 32 at a time.
+struct Scan {
+    const uint32_t *bits;
+    int blocks, end, words, shift;
+    uint32_t mask;
+    int base = 0;
+    uint32_t now[4], then[4];
+
+    __device__ __forceinline__ void fetch(int from, uint32_t (&to)[4]) const {
+        const int j = from + (threadIdx.x & 31);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to[k] = k < words && j < end ? (__ldg(bits + (int64_t)k * blocks + j) >> shift) & mask : 0u;
+    }
+    __device__ __forceinline__ Scan(const Shape &s, const uint32_t *all, const Tile &t, int tile) {
+        blocks = s.blocks;
+        const int w = t.i0 >> 5;
+        bits = all + (t.bh * s.words + w) * s.blocks;
+        words = tile <= 32 ? 1 : min(tile / 32, s.words - w);
+        shift = t.i0 & 31;
+        mask = tile >= 32 ? ~0u : (1u << tile) - 1;
+        const int last = min(t.i0 + tile, s.queries) - 1, len = s.length(t.b);
+        end = min(s.blocks, (s.end(last, len) + kBlock - 1) / kBlock);
+        fetch(0, then);
+    }
+    // the lanes' next 32 blocks: false where there are no more
+    __device__ __forceinline__ bool next(uint32_t &some) {
+        if (base >= end) return false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) now[k] = then[k];
+        fetch(base + 32, then);
+        some = __ballot_sync(~0u, (now[0] | now[1] | now[2] | now[3]) != 0);
+        base += 32;
+        return true;
+    }
+    __device__ __forceinline__ void entry(int lane, Entry &e) const {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e.rows[k] = __shfl_sync(~0u, now[k], lane);
+        e.block = base - 32 + lane;
+    }
+};
+
+// Writes 32 rows of the warp, one to a lane, so that a row's bytes leave together: `value(g, v)` gives the lane's elements 32 g .. 32 g + 31 as
+// four 16-byte pieces.  They pass through `stage`, 32 rows of 128 bytes in each of DP / 64 slabs `slab` bytes apart, the pieces swizzled by the row.
+template <typename T, int DP, typename F> __device__ __forceinline__ void write_rows(uint8_t *stage, int slab, T *out, int64_t row_at, bool there, int d, F value) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < DP / 32; ++g) {
+        uint4 v[4];
+        value(g, v);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(stage + g / 2 * slab + lane * 128 + ((((g % 2) * 4 + c) ^ (lane & 7)) << 4)) = v[c];
+    }
+    __syncwarp();
+    constexpr int kLanes = DP / 8;   // to a row
+#pragma unroll 4
+    for (int r0 = 0; r0 < 32; r0 += 32 / kLanes) {
+        const int r = r0 + lane / kLanes, c = lane % kLanes;
+        const int64_t at = __shfl_sync(~0u, row_at, r);
+        const bool live = __shfl_sync(~0u, (int)there, r);
+        if (live && c * 8 < d)
+            *reinterpret_cast<uint4 *>(out + at + c * 8) = *reinterpret_cast<const uint4 *>(stage + c / 8 * slab + r * 128 + (((c % 8) ^ (r & 7)) << 4));
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack8(const float *f) {
+    return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------------
+// A barrier tells a phase from the next but not from the one after that, so what may be two products ahead or behind has two barriers, one for either buffer of S.
+// Per block: S[128 x 64] = Q K^T (operands in shared memory), the softmax's step by one thread per row out of tensor memory, P (16 bits) back into S's place,
+// O[128 x d] += P V with P as the operand in tensor memory.  S is double buffered; 256 columns of tensor memory and ~100 KB of shared memory, so that
+// two CTAs share an SM and one's products run under the other's exponentials.
+// The maximum that weights are taken relative to follows the true one only when that has grown by 2^8: weights then stay below 256, exact enough in
+// either type, and O is seldom rescaled.
+constexpr float kSlack = 8.f;
+template <int DP> struct ForwardSmem {
+    static constexpr int kSlots = DP == 128 ? 4 : 6;
+    static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
+    static constexpr int kQ = 1024, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // the first 1024 bytes: entries, barriers
+    static constexpr int kEntriesAt = 0, kBars = kEntries * sizeof(Entry);
+    static constexpr int kBarQ = kBars, kFull = kBarQ + 8, kEmpty = kFull + 8 * kSlots, kS = kEmpty + 8 * kSlots, kP = kS + 16, kPv = kP + 16, kE = kPv + 16, kDrain = kE + 8 * kEntries, kAbort = kDrain + 8,
+                         kHolder = kAbort + 4;
+    static_assert(kHolder + 4 <= 1024, "head");
+};
+constexpr int kForwardThreads = 192;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_v, uint32_t *redo, uint32_t *status) {
+    using M = ForwardSmem<DP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = tc::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t *sm = smem_raw + (base - raw);
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(sm + M::kAbort);
+    const Shape &s = a.s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Tile t = tile_of(s, a.tile, blockIdx.x);
+    const int len = s.length(t.b);
+
+    if (threadIdx.x == 0) {
+        tc::mbar_init(base + M::kBarQ, 1);
+        for (int i = 0; i < M::kSlots; ++i) {
+            tc::mbar_init(base + M::kFull + 8 * i, 1);
+            tc::mbar_init(base + M::kEmpty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(base + M::kS + 8 * i, 1);
+            tc::mbar_init(base + M::kP + 8 * i, 4);
+            tc::mbar_init(base + M::kPv + 8 * i, 1);
+        }
+        tc::mbar_init(base + M::kDrain, 1);
+        for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+    }
+    if (warp == 5) {
+        tc::tmem_alloc(base + M::kHolder, 256);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder);
+    const uint32_t tmem_o = tmem + 128;
+    bool bad = false;
+    pdl_launch_dependents();
+
+    if (warp == 4) {
+        // loader: position 2 x holds the keys, 2 x + 1 the values of the x-th block
+        pdl_wait();   // the bits are the kernel's before
+        const uint32_t q_bytes = (uint32_t)(a.tile * s.group * 128 * (DP / 64));
+        if (lane == 0) {
+            tc::mbar_expect_tx(base + M::kBarQ, q_bytes);
+            for (int x = 0; x < DP / 64; ++x) tc::tma_load_4d(base + M::kQ + x * kRows * 128, &map_q, base + M::kBarQ, x * 64, t.kvh * s.group, t.i0, t.b);
+        }
+        uint32_t at = 0;
+        bool ok = true;
+        auto slot_free = [&]() {   // lane 0: the slot of position `at`
+            return at < (uint32_t)M::kSlots || wait(base + M::kEmpty + 8 * (at % M::kSlots), (at / M::kSlots - 1) & 1, abort_flag);
+        };
+        auto load = [&](const CUtensorMap *map, int j) {
+            const uint32_t slot = at % M::kSlots, bar = base + M::kFull + 8 * slot;
+            tc::mbar_expect_tx(bar, M::kSlotBytes);
+            for (int x = 0; x < DP / 64; ++x) tc::tma_load_4d(base + M::kRing + slot * M::kSlotBytes + x * kBlock * 128, map, bar, x * 64, t.kvh, j * kBlock, t.b);
+            ++at;
+        };
+        Scan scan(s, a.bits, t, a.tile);
+        uint32_t some;
+        while (ok && scan.next(some)) {
+            for (; some && ok; some &= some - 1) {
+                Entry e;
+                scan.entry(__ffs(some) - 1, e);
+                if (lane == 0) {
+                    ok = slot_free();
+                    if (ok) {
+                        Entry *to = reinterpret_cast<Entry *>(sm + M::kEntriesAt) + (at / 2) % kEntries;
+                        *reinterpret_cast<uint4 *>(to->rows) = make_uint4(e.rows[0], e.rows[1], e.rows[2], e.rows[3]);
+                        to->block = e.block;
+                        tc::mbar_arrive(base + M::kE + 8 * ((at / 2) % kEntries));
+                        load(&map_k, e.block);
+                        ok = slot_free();
+                        if (ok) load(&map_v, e.block);
+                    }
+                }
+                ok = __shfl_sync(~0u, (int)ok, 0);
+            }
+        }
+        if (lane == 0) {
+            if (ok && slot_free()) {
+                reinterpret_cast<Entry *>(sm + M::kEntriesAt)[(at / 2) % kEntries].block = -1;
+                tc::mbar_arrive(base + M::kE + 8 * ((at / 2) % kEntries));
+                tc::mbar_arrive(base + M::kFull + 8 * (at % M::kSlots));
+            }
+            if (*abort_flag)   // copies in flight end before the shared memory is given back
+                for (uint32_t x = at > (uint32_t)M::kSlots ? at - M::kSlots : 0; x < at; ++x)
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (x % M::kSlots), (x / M::kSlots) & 1); ++y) {}
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescO = idesc<T>(DP, 0, 1);
+            const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
+            const uint32_t q_lo = tc::smem_desc_lo(base + M::kQ, 16), k_lo = tc::smem_desc_lo(base + M::kRing, 16);
+            const uint32_t v_lo = tc::smem_desc_lo(base + M::kRing, kBlock * 128);   // 64-dimension slabs
+            bool ok = wait(base + M::kBarQ, 0, abort_flag);
+            uint32_t x = 0;
+            auto values = [&](uint32_t y) {   // O += P V of the y-th block
+                const uint32_t at = 2 * y + 1, slot = at % M::kSlots;
+                if (!(ok = ok && wait(base + M::kP + 8 * (y & 1), (y >> 1) & 1, abort_flag) && wait(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag))) return;
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < kBlock / 16; ++k)
+                    tc::mma_f16_ts(tmem_o, tmem + (y & 1) * 64 + 8 * k, tc::desc64(v_lo + slot * (M::kSlotBytes >> 4) + 128 * k, hi), kIdescO, y > 0 || k > 0);
+                tc::mma_commit(base + M::kPv + 8 * (y & 1));
+                tc::mma_commit(base + M::kEmpty + 8 * slot);
+            };
+            for (; ok; ++x) {
+                const uint32_t at = 2 * x, slot = at % M::kSlots;
+                ok = wait(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag);
+                if (!ok || reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries].block < 0) break;
+                // S goes where the P of two blocks ago stood: its product has ended
+                if (x >= 2 && !(ok = wait(base + M::kPv + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) break;
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    tc::mma_f16_ss(tmem + (x & 1) * 64, tc::desc64(q_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
+                                   tc::desc64(k_lo + slot * (M::kSlotBytes >> 4) + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
+                tc::mma_commit(base + M::kS + 8 * (x & 1));
+                tc::mma_commit(base + M::kEmpty + 8 * slot);
+                if (x > 0) values(x - 1);
+            }
+            if (ok && x > 0) values(x - 1);
+            // what was issued ends before tensor memory is given back; normally the softmax has waited for it already
+            tc::mma_commit(base + M::kDrain);
+            for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
+        }
+    } else {
+        const int r = threadIdx.x, qx = r / s.group, i = t.i0 + qx;
+        const bool there = r < a.tile * s.group && i < s.queries;
+        const int h = t.kvh * s.group + r % s.group, end = there ? s.end(i, len) : 0;
+        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        const float c = a.scale * kLog2e;
+        float top = -INFINITY, total = 0.f;   // what the weights are relative to, and their sum
+        uint32_t x = 0;
+        bool ok = true;
+        for (;; ++x) {
+            ok = __all_sync(~0u, wait(base + M::kE + 8 * (x % kEntries), (x / kEntries) & 1, abort_flag));
+            if (!ok) break;
+            const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries];
+            const int block = e.block;
+            if (block < 0) break;
+            const bool listed = there && (e.rows[qx >> 5] >> (qx & 31) & 1u);
+            const int n = listed ? min(kBlock, end - block * kBlock) : 0;   // keys of the row
+            ok = __all_sync(~0u, wait(base + M::kS + 8 * (x & 1), (x >> 1) & 1, abort_flag));
+            if (!ok) break;
+            tc::tc_fence_after_sync();
+            uint32_t u[2][32];
+            tc::tmem_ld_x32_issue(mine + (x & 1) * 64, u[0]);
+            tc::tmem_ld_x32_issue(mine + (x & 1) * 64 + 32, u[1]);
+            tc::tmem_ld_x32_wait(u[0]);
+            tc::tmem_ld_x32_wait(u[1]);
+            if (!__all_sync(~0u, n == kBlock)) {
+#pragma unroll
+                for (int k = 0; k < kBlock; ++k)
+                    if (k >= n) u[k / 32][k % 32] = __float_as_uint(-INFINITY);
+            }
+            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int k = 0; k < kBlock; ++k) m[k % 4] = fmaxf(m[k % 4], __uint_as_float(u[k / 32][k % 32]));
+            const float high = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c;
+            if (__any_sync(~0u, high > top + kSlack)) {
+                const float to = fmaxf(top, high), shrink = to == -INFINITY ? 1.f : ex2(top - to);
+                top = to;
+                total *= shrink;
+                if (x > 0) {
+                    ok = __all_sync(~0u, wait(base + M::kPv + 8 * ((x - 1) & 1), ((x - 1) >> 1) & 1, abort_flag));
+                    if (!ok) break;
+                    tc::tc_fence_after_sync();
+#pragma unroll 1
+                    for (int k = 0; k < DP; k += 32) {
+                        uint32_t o[32];
+                        tc::tmem_ld_x32(mine + 128 + k, o);
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * shrink);
+                        tc::tmem_st_x32(mine + 128 + k, o);
+                    }
+                }
+            }
+            const float off = top == -INFINITY ? 0.f : -top;
+            float sum[4] = {};
+            uint32_t p[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+                const float y = ex2(fmaf(__uint_as_float(u[k / 16][2 * k % 32]), c, off)), z = ex2(fmaf(__uint_as_float(u[k / 16][2 * k % 32 + 1]), c, off));
+                sum[2 * k % 4] += y;
+                sum[2 * k % 4 + 1] += z;
+                p[k] = pack2<T>(y, z);
+            }
+            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc::tmem_st_x32(mine + (x & 1) * 64, p);
+            tc::tmem_st_wait();
+            tc::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(base + M::kP + 8 * (x & 1));
+        }
+        // the last product, and with it all before it; without any, the copy of Q ends before its place takes the result
+        if (ok) ok = __all_sync(~0u, x > 0 ? wait(base + M::kPv + 8 * ((x - 1) & 1), ((x - 1) >> 1) & 1, abort_flag) : wait(base + M::kBarQ, 0, abort_flag));
+        if (ok) {
+            tc::tc_fence_after_sync();
+            const int64_t row = (((int64_t)t.b * s.queries + i) * s.heads + h) * s.d;
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            auto result = [&](int g, float (&f)[32]) {
+                uint32_t o[32];
+                if (x > 0) tc::tmem_ld_x32(mine + 128 + 32 * g, o);
+#pragma unroll
+                for (int y = 0; y < 32; ++y) f[y] = x > 0 && total != 0.f ? __uint_as_float(o[y]) * inv : 0.f;
+            };
+            uint8_t *stage = sm + M::kQ + warp * 32 * 128;
+            write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result), row, there, s.d, [&](int g, uint4 (&v)[4]) {
+                float f[32];
+                result(g, f);
+#pragma unroll
+                for (int y = 0; y < 32; ++y) bad |= there && !finite(f[y]);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
+            });
+            if (a.result_low)
+                write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result_low), row, there, s.d, [&](int g, uint4 (&v)[4]) {
+                    float f[32];
+                    result(g, f);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) f[y] -= to_f32(from_f32<T>(f[y]));
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
+                });
+            bad |= there && total != total;
+            if (there) a.lse[((int64_t)t.b * s.heads + h) * s.queries + i] = total == 0.f ? INFINITY : top + log2f(total);
+        }
+    }
+    tc::tc_fence_before_sync();
+    const bool again = __syncthreads_or(bad);
+    if (threadIdx.x == 0) {
+        redo[t.index] = again;
+        if (*abort_flag) atomicOr(status, kStatusForward);
+    }
+    if (warp == 5) {
+        tc::tc_fence_after_sync();
+        tc::tmem_dealloc(tmem, 256);
+    }
+}
+
+}  // namespace tcore
+}  // namespace blocks
+}  // namespace vs
