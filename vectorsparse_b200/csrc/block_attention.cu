@@ -129,9 +129,9 @@ template <typename T> int select(const blocks::Shape &s, const blocks::Operand &
 }
 static_assert(blocks::score_bytes<1>(blocks::kMaxBlocks, blocks::kMaxD) <= kMaxSmem, "scores of one query");
 
-int make_bits(const blocks::Shape &s, const int32_t *lists, uint32_t *bits, cudaStream_t st) {
+int make_bits(const blocks::Shape &s, const int32_t *lists, uint32_t *bits, uint32_t *zero, cudaStream_t st) {
     if (s.blocks == 0) return VS_OK;
-    blocks::bits_kernel<<<(unsigned)((int64_t)s.batch * s.kv_heads * s.words), blocks::kBitsThreads, 0, st>>>(s, lists, bits);
+    blocks::bits_kernel<<<(unsigned)((int64_t)s.batch * s.kv_heads * s.words), blocks::kBitsThreads, 0, st>>>(s, lists, bits, zero);
     return (int)cudaGetLastError();
 }
 
@@ -185,19 +185,39 @@ template <typename T> int attention(blocks::Args a, uint32_t *redo, cudaStream_t
     if (rc != VS_OK) return rc;
     return s.d <= 64 ? forward<T, 64>(a, redo, status, st) : forward<T, 128>(a, redo, status, st);
 }
-template <typename T> int attention_backward(blocks::Args a, void *grad_q, cudaStream_t st) {
+template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
     const blocks::Shape &s = a.s;
-    const int64_t rows = (int64_t)s.batch * s.queries * s.heads;
-    blocks::delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return (int)e;
+    using SmemQ = blocks::tcore::GradQSmem<DP>;
+    using SmemKV = blocks::tcore::GradKVSmem<DP>;
+    CUtensorMap q, g, k, v;
     a.tile = tile_queries(s.group);
-    a.result = grad_q;
-    blocks::rows_kernel<T, true><<<(unsigned)query_tiles(s), blocks::kRowThreads, 0, st>>>(a);
-    e = cudaGetLastError();
+    int rc = make_map<T>(&q, a.q, s.batch, s.queries, s.heads, s.d, s.group, a.tile);
+    if (rc == VS_OK) rc = make_map<T>(&g, a.grad_out, s.batch, s.queries, s.heads, s.d, s.group, a.tile);
+    if (rc == VS_OK) rc = make_map<T>(&k, a.k, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
+    if (rc == VS_OK) rc = make_map<T>(&v, a.v, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
+    if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_q_kernel<T, DP>>(SmemQ::kBytes);
+    if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_kv_kernel<T, DP>>(SmemKV::kBytes + 1024);
+    if (rc != VS_OK) return rc;
+    const int64_t rows = (int64_t)s.batch * s.queries * s.heads, tiles = query_tiles(s), blocks_all = (int64_t)s.batch * s.kv_heads * s.blocks;
+    uint32_t *redo_kv = redo + tiles;
+    cudaError_t e = launch_behind(blocks::delta_kernel<T>, (unsigned)((rows + 15) / 16), 256, 0, st, a);
+    if (e == cudaSuccess)
+        e = launch_behind(blocks::tcore::grad_q_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kForwardThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
+    if (e == cudaSuccess)
+        e = launch_behind(blocks::tcore::grad_kv_kernel<T, DP>, (unsigned)blocks_all, blocks::tcore::kGradKVThreads, SmemKV::kBytes + 1024, st, a, q, g, k, v, redo_kv, status);
     if (e != cudaSuccess) return (int)e;
-    blocks::keys_kernel<T><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.blocks), blocks::kRowThreads, 0, st>>>(a);
-    return (int)cudaGetLastError();
+    a.redo = redo;
+    e = launch_behind(blocks::rows_kernel<T, true>, again_grid(tiles), blocks::kRowThreads, 0, st, a);
+    if (e != cudaSuccess) return (int)e;
+    a.redo = redo_kv;
+    return (int)launch_behind(blocks::keys_kernel<T>, again_grid(blocks_all), blocks::kRowThreads, 0, st, a);
+}
+template <typename T> int attention_backward(blocks::Args a, uint32_t *redo, cudaStream_t st) {
+    int sms = 0;
+    uint32_t *status = nullptr;
+    const int rc = current_device(&sms, &status);
+    if (rc != VS_OK) return rc;
+    return a.s.d <= 64 ? backward<T, 64>(a, redo, status, st) : backward<T, 128>(a, redo, status, st);
 }
 
 inline bool scale_ok(float scale) { return scale > 0.f && std::isfinite(scale); }
@@ -230,7 +250,7 @@ VS_EXPORT int vs_select_blocks(int dtype, int batch, int queries, int keys, int 
 VS_EXPORT int64_t vs_selected_attention_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int d, int backward) {
     blocks::Shape s;
     if (check_shape(VS_F16, batch, queries, keys, heads, kv_heads, d, 1, 0, nullptr, s) != VS_OK) return 0;
-    return bits_bytes(s) + redo_bytes(s) + (backward ? up256((int64_t)batch * heads * queries * 4) : 0);
+    return bits_bytes(s) + redo_bytes(s) + (backward ? up256((int64_t)batch * heads * queries * 4) + 256 : 0);   // the words of its rows, one of the call
 }
 
 VS_EXPORT int vs_selected_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const void *q,
@@ -249,7 +269,7 @@ VS_EXPORT int vs_selected_attention(int dtype, int batch, int queries, int keys,
     if (workspace_bytes < vs_selected_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, d, 0)) return VS_ERR_SHAPE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     uint32_t *bits = static_cast<uint32_t *>(workspace);
-    if ((rc = make_bits(a.s, lists, bits, st)) != VS_OK) return rc;
+    if ((rc = make_bits(a.s, lists, bits, nullptr, st)) != VS_OK) return rc;
     a.bits = bits; a.lse = lse; a.result = out; a.result_low = out_low; a.scale = scale;
     uint32_t *redo = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + bits_bytes(a.s));
     return dtype == VS_F16 ? attention<__half>(a, redo, st) : attention<__nv_bfloat16>(a, redo, st);
@@ -283,12 +303,13 @@ VS_EXPORT int vs_selected_attention_backward(int dtype, int batch, int queries, 
     if (workspace_bytes < vs_selected_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, d, 1)) return VS_ERR_SHAPE;
     contiguous(a.out, out, queries, heads, d);
     a.out_low = out_low;
-    uint32_t *bits = static_cast<uint32_t *>(workspace);
-    if ((rc = make_bits(a.s, lists, bits, st)) != VS_OK) return rc;
-    a.bits = bits; a.lse = const_cast<float *>(lse); a.scale = scale;
-    a.delta = reinterpret_cast<float *>(static_cast<char *>(workspace) + bits_bytes(a.s) + redo_bytes(a.s));
-    a.grad_k = grad_k; a.grad_v = grad_v;
-    return dtype == VS_F16 ? attention_backward<__half>(a, grad_q, st) : attention_backward<__nv_bfloat16>(a, grad_q, st);
+    char *at = static_cast<char *>(workspace);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(at), *redo = reinterpret_cast<uint32_t *>(at + bits_bytes(a.s));
+    a.bits = bits; a.lse = const_cast<float *>(lse); a.scale = scale; a.result = grad_q; a.grad_k = grad_k; a.grad_v = grad_v;
+    a.delta = reinterpret_cast<float *>(at + bits_bytes(a.s) + redo_bytes(a.s));
+    a.most = reinterpret_cast<uint32_t *>(at + bits_bytes(a.s) + redo_bytes(a.s) + up256((int64_t)batch * heads * queries * 4));
+    if ((rc = make_bits(a.s, lists, bits, a.most, st)) != VS_OK) return rc;
+    return dtype == VS_F16 ? attention_backward<__half>(a, redo, st) : attention_backward<__nv_bfloat16>(a, redo, st);
 }
 
 // ---- the cache ----------------------------------------------------------------------------------------------------------

@@ -61,10 +61,11 @@ template <typename T> __device__ __forceinline__ void load8(const T *p, float (&
 // One CTA takes a word of 32 queries: it collects their bits in shared memory and writes the word's row for all blocks, so that nothing has to
 // be cleared beforehand.  Bound by the reading of the lists.
 constexpr int kBitsThreads = 128, kBitsChunk = 4096;
-__global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const int32_t *lists, uint32_t *bits) {
+__global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const int32_t *lists, uint32_t *bits, uint32_t *zero) {
     __shared__ uint32_t row[kBitsChunk];
     pdl_launch_dependents();
     const int64_t at = blockIdx.x;
+    if (zero && at == 0 && threadIdx.x == 0) *zero = 0;
     const int w = (int)(at % s.words);
     const int b = (int)(at / s.words / s.kv_heads);
     const int len = s.length(b), rows = s.rows(b);
@@ -257,6 +258,7 @@ struct Args {
     const uint32_t *bits;
     float *lse;           // [batch, heads, queries] base 2; +inf: the row attends to nothing
     float *delta;         // the same shape: rowsum(out o grad_out)
+    uint32_t *most;       // largest magnitude in grad_out, as the bits of a float
     const void *out_low;  // what rounding left of out, as out; or null
     void *result;         // out or grad_q, contiguous
     void *result_low;     // out_low or null
@@ -430,13 +432,16 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads) keys_kernel
     }
 }
 
-// rowsum(out o grad_out) of each row; 0 for rows behind a sequence's end.  Eight dimensions to a lane, 16 lanes to a row.
+// rowsum(out o grad_out) of each row and the largest magnitude in grad_out; nothing of rows behind a sequence's end.  Eight dimensions to a lane, 16 lanes
+// to a row.
 template <typename T> __global__ void __launch_bounds__(256) delta_kernel(const Args a) {
     const Shape &s = a.s;
     const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, all = (int64_t)s.batch * s.queries * s.heads;
     const int c = threadIdx.x % 16 * 8;
     const int h = (int)(at % s.heads), i = (int)(at / s.heads % s.queries), b = (int)(at / s.heads / s.queries);
-    float sum = 0.f;
+    pdl_wait();
+    pdl_launch_dependents();
+    float sum = 0.f, most = 0.f;
     if (at < all && c < s.d && i < s.rows(b)) {
         float o[8], g[8];
         load8(static_cast<const T *>(a.out.at) + b * a.out.batch + (int64_t)i * a.out.token + h * a.out.head + c, o);
@@ -448,7 +453,19 @@ template <typename T> __global__ void __launch_bounds__(256) delta_kernel(const 
             for (int x = 0; x < 8; ++x) sum = fmaf(low[x], g[x], sum);
         }
 #pragma unroll
-        for (int x = 0; x < 8; ++x) sum = fmaf(o[x], g[x], sum);
+        for (int x = 0; x < 8; ++x) {
+            sum = fmaf(o[x], g[x], sum);
+            most = fmaxf(most, fabsf(g[x]));
+        }
+    }
+    const uint32_t all_most = __reduce_max_sync(~0u, __float_as_uint(most));
+    __shared__ uint32_t warps_most[8];
+    if (threadIdx.x % 32 == 0) warps_most[threadIdx.x / 32] = all_most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t top = 0;
+        for (int x = 0; x < 8; ++x) top = max(top, warps_most[x]);
+        if (top > *reinterpret_cast<volatile uint32_t *>(a.most)) atomicMax(a.most, top);   // a maximum: the order does not count
     }
 #pragma unroll
     for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);

@@ -247,9 +247,11 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 tc::mbar_arrive(base + M::kE + 8 * ((at / 2) % kEntries));
                 tc::mbar_arrive(base + M::kFull + 8 * (at % M::kSlots));
             }
-            if (*abort_flag)   // copies in flight end before the shared memory is given back
+            if (*abort_flag) {   // copies in flight end before the shared memory is given back
+                for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kBarQ, 0); ++y) {}
                 for (uint32_t x = at > (uint32_t)M::kSlots ? at - M::kSlots : 0; x < at; ++x)
                     for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (x % M::kSlots), (x / M::kSlots) & 1); ++y) {}
+            }
         }
     } else if (warp == 5) {
         if (lane == 0) {
@@ -401,6 +403,502 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
     if (warp == 5) {
         tc::tc_fence_after_sync();
         tc::tmem_dealloc(tmem, 256);
+    }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------
+// Weights and the scores' gradients are rounded to 16 bits for their products.  fp16 keeps its precision only above 2^-14, so there both are multiplied by powers of
+// two first: the weights, at most 1, by 2^14; the gradients by the one that brings the largest element of grad_out to 1 .. 2 (found by the delta kernel).
+template <typename T> struct Lift {
+    static constexpr float kWeight = std::is_same<T, __half>::value ? 14.f : 0.f;   // exponent
+    static __device__ __forceinline__ float grad(const uint32_t *most) {
+        if (!std::is_same<T, __half>::value) return 1.f;
+        const uint32_t e = __ldcg(most) >> 23;
+        return e < 6 || e >= 253 ? 1.f : __uint_as_float((259u - e) << 23);   // 2^(5 - (e - 127))
+    }
+};
+__device__ __forceinline__ float exp2i(float e) { return __uint_as_float((uint32_t)((int)e + 127) << 23); }   // a whole exponent
+
+// dQ: a tile of queries through the union of its lists, as forward.  Per block S = Q K^T and dP = dO V^T, dS = P (dP - delta) back into S's place as an operand,
+// dQ += dS K with the same keys, now contracted over.  Keys are double buffered, values not: their place is free once dP is there, long before the
+// next ones are needed.  256 columns of tensor memory, 113 KB of shared memory (d = 128): two CTAs an SM, one's products under the other's exponentials.
+template <int DP> struct GradQSmem {
+    static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
+    static constexpr int kQ = 1024, kG = kQ + kQBytes, kK = kG + kQBytes, kV = kK + 2 * kSlotBytes, kBytes = kV + kSlotBytes;
+    static constexpr int kBars = kEntries * sizeof(Entry);
+    static constexpr int kBarQ = kBars, kKFull = kBarQ + 8, kKEmpty = kKFull + 16, kVFull = kKEmpty + 16, kVEmpty = kVFull + 8, kSP = kVEmpty + 8, kDs = kSP + 8, kDq = kDs + 8,
+                         kE = kDq + 8, kDrain = kE + 8 * kEntries, kAbort = kDrain + 8, kHolder = kAbort + 4;
+    static_assert(kHolder + 4 <= 1024, "head");
+    static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs an SM");
+};
+template <typename T, int DP>
+__global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
+                                                                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, uint32_t *redo,
+                                                                    uint32_t *status) {
+    using M = GradQSmem<DP>;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    const uint32_t base = tc::smem_u32(sm);
+    const Shape &s = a.s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Tile t = tile_of(s, a.tile, blockIdx.x);
+    pdl_launch_dependents();
+    if (base & 1023u) {   // there is no room for a margin: a tile whose memory does not start where the swizzle needs it is left to the kernel behind
+        pdl_wait();
+        if (threadIdx.x == 0) redo[t.index] = 1;
+        return;
+    }
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(sm + M::kAbort);
+    const int len = s.length(t.b);
+
+    if (threadIdx.x == 0) {
+        for (int bar : {M::kBarQ, M::kKFull, M::kKFull + 8, M::kKEmpty, M::kKEmpty + 8, M::kVFull, M::kVEmpty, M::kSP, M::kDq, M::kDrain}) tc::mbar_init(base + bar, 1);
+        tc::mbar_init(base + M::kDs, 4);
+        for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+    }
+    if (warp == 5) {
+        tc::tmem_alloc(base + M::kHolder, 256);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder);
+    bool bad = false;
+
+    if (warp == 4) {
+        pdl_wait();
+        const uint32_t q_bytes = (uint32_t)(a.tile * s.group * 128 * (DP / 64));
+        if (lane == 0) {
+            tc::mbar_expect_tx(base + M::kBarQ, 2 * q_bytes);
+            for (int x = 0; x < DP / 64; ++x) {
+                tc::tma_load_4d(base + M::kQ + x * kRows * 128, &map_q, base + M::kBarQ, x * 64, t.kvh * s.group, t.i0, t.b);
+                tc::tma_load_4d(base + M::kG + x * kRows * 128, &map_g, base + M::kBarQ, x * 64, t.kvh * s.group, t.i0, t.b);
+            }
+        }
+        uint32_t x = 0;
+        bool ok = true;
+        auto load = [&](const CUtensorMap *map, uint32_t to, uint32_t bar, int j) {
+            tc::mbar_expect_tx(bar, M::kSlotBytes);
+            for (int y = 0; y < DP / 64; ++y) tc::tma_load_4d(to + y * kBlock * 128, map, bar, y * 64, t.kvh, j * kBlock, t.b);
+        };
+        Scan scan(s, a.bits, t, a.tile);
+        uint32_t some;
+        while (ok && scan.next(some)) {
+            for (; some && ok; some &= some - 1) {
+                Entry e;
+                scan.entry(__ffs(some) - 1, e);
+                if (lane == 0) {
+                    ok = x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
+                    if (ok) {
+                        Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
+                        *reinterpret_cast<uint4 *>(to->rows) = make_uint4(e.rows[0], e.rows[1], e.rows[2], e.rows[3]);
+                        to->block = e.block;
+                        tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
+                        load(&map_k, base + M::kK + (x & 1) * M::kSlotBytes, base + M::kKFull + 8 * (x & 1), e.block);
+                        ok = x < 1 || wait(base + M::kVEmpty, (x - 1) & 1, abort_flag);
+                        if (ok) load(&map_v, base + M::kV, base + M::kVFull, e.block);
+                    }
+                }
+                ok = __shfl_sync(~0u, (int)ok, 0);
+                ++x;
+            }
+        }
+        if (lane == 0) {
+            if (ok && (x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
+                reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
+                tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
+                tc::mbar_arrive(base + M::kKFull + 8 * (x & 1));
+            }
+            if (*abort_flag) {   // copies in flight end before the shared memory is given back
+                for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kBarQ, 0); ++y) {}
+                for (uint32_t z = x > 2 ? x - 2 : 0; z < x; ++z) {
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kKFull + 8 * (z & 1), (z >> 1) & 1); ++y) {}
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kVFull, z & 1); ++y) {}
+                }
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescQ = idesc<T>(DP, 0, 1);
+            const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
+            const uint32_t q_lo = tc::smem_desc_lo(base + M::kQ, 16), g_lo = tc::smem_desc_lo(base + M::kG, 16), k_lo = tc::smem_desc_lo(base + M::kK, 16);
+            const uint32_t v_lo = tc::smem_desc_lo(base + M::kV, 16), kt_lo = tc::smem_desc_lo(base + M::kK, kBlock * 128);
+            bool ok = wait(base + M::kBarQ, 0, abort_flag);
+            for (uint32_t x = 0; ok; ++x) {
+                const uint32_t slot = x & 1, at = slot * (M::kSlotBytes >> 4);
+                ok = wait(base + M::kKFull + 8 * slot, (x >> 1) & 1, abort_flag);
+                if (!ok || reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0) break;
+                if (x > 0 && !(ok = wait(base + M::kDq, (x - 1) & 1, abort_flag))) break;   // S goes where dS stood
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    tc::mma_f16_ss(tmem, tc::desc64(q_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
+                                   tc::desc64(k_lo + at + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
+                if (!(ok = wait(base + M::kVFull, x & 1, abort_flag))) break;
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    tc::mma_f16_ss(tmem + 64, tc::desc64(g_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
+                                   tc::desc64(v_lo + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
+                tc::mma_commit(base + M::kSP);
+                tc::mma_commit(base + M::kVEmpty);
+                if (!(ok = wait(base + M::kDs, x & 1, abort_flag))) break;
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < kBlock / 16; ++k)
+                    tc::mma_f16_ts(tmem + 128, tmem + 8 * k, tc::desc64(kt_lo + at + 128 * k, hi), kIdescQ, x > 0 || k > 0);
+                tc::mma_commit(base + M::kDq);
+                tc::mma_commit(base + M::kKEmpty + 8 * slot);
+            }
+            tc::mma_commit(base + M::kDrain);
+            for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
+        }
+    } else {
+        const int r = threadIdx.x, qx = r / s.group, i = t.i0 + qx;
+        const bool there = r < a.tile * s.group && i < s.queries;
+        const int h = t.kvh * s.group + r % s.group, end = there ? s.end(i, len) : 0;
+        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        const float c = a.scale * kLog2e;
+        float lse = INFINITY, lift = 1.f, minus_delta = 0.f;
+        uint32_t x = 0;
+        bool ok = true;
+        for (;; ++x) {
+            ok = __all_sync(~0u, wait(base + M::kE + 8 * (x % kEntries), (x / kEntries) & 1, abort_flag));
+            if (!ok) break;
+            const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm)[x % kEntries];
+            const int block = e.block;
+            if (block < 0) break;
+            const bool listed = there && (e.rows[qx >> 5] >> (qx & 31) & 1u);
+            const int n = listed ? min(kBlock, end - block * kBlock) : 0;   // keys of the row
+            if (x == 0) {   // the loader has waited for the kernels that wrote these
+                lift = Lift<T>::grad(a.most);
+                if (there) {
+                    const int64_t row = ((int64_t)t.b * s.heads + h) * s.queries + i;
+                    lse = __ldcg(a.lse + row);
+                    minus_delta = -__ldcg(a.delta + row) * lift;
+                }
+            }
+            ok = __all_sync(~0u, wait(base + M::kSP, x & 1, abort_flag));
+            if (!ok) break;
+            tc::tc_fence_after_sync();
+            const bool whole = __all_sync(~0u, n == kBlock);
+            uint32_t ds[32];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t u[32], d[32];
+                tc::tmem_ld_x32_issue(mine + 32 * half, u);
+                tc::tmem_ld_x32_issue(mine + 64 + 32 * half, d);
+                tc::tmem_ld_x32_wait(u);
+                tc::tmem_ld_x32_wait(d);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    float f[2];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        f[y] = ex2(fmaf(__uint_as_float(u[2 * k + y]), c, -lse)) * fmaf(__uint_as_float(d[2 * k + y]), lift, minus_delta);
+                        if (!whole && 32 * half + 2 * k + y >= n) f[y] = 0.f;
+                    }
+                    ds[16 * half + k] = pack2<T>(f[0], f[1]);
+                }
+            }
+            tc::tmem_st_x32(mine, ds);
+            tc::tmem_st_wait();
+            tc::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(base + M::kDs);
+        }
+        if (ok) ok = __all_sync(~0u, x > 0 ? wait(base + M::kDq, (x - 1) & 1, abort_flag) : wait(base + M::kBarQ, 0, abort_flag));
+        if (ok) {
+            tc::tc_fence_after_sync();
+            const int64_t row = (((int64_t)t.b * s.queries + i) * s.heads + h) * s.d;
+            const float back = a.scale / lift;
+            write_rows<T, DP>(sm + M::kQ + warp * 32 * 128, kRows * 128, static_cast<T *>(a.result), row, there, s.d, [&](int g, uint4 (&v)[4]) {
+                uint32_t o[32];
+                float f[32];
+                if (x > 0) tc::tmem_ld_x32(mine + 128 + 32 * g, o);
+#pragma unroll
+                for (int y = 0; y < 32; ++y) {
+                    f[y] = x > 0 ? __uint_as_float(o[y]) * back : 0.f;
+                    bad |= there && !finite(f[y]);
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
+            });
+        }
+    }
+    tc::tc_fence_before_sync();
+    const bool again = __syncthreads_or(bad);
+    if (threadIdx.x == 0) {
+        redo[t.index] = again;
+        if (*abort_flag) atomicOr(status, kStatusGradQ);
+    }
+    if (warp == 5) {
+        tc::tc_fence_after_sync();
+        tc::tmem_dealloc(tmem, 256);
+    }
+}
+
+// dK, dV: a block of 64 keys of one head through the tiles of queries in which any has listed it.  Per tile S = Q K^T and dP = dO V^T as above, rows in lanes;
+// P and dS go to shared memory, where they are the operands of dV^T[d x 64] += dO^T P and dK^T += Q^T dS: contracted over the rows, all heads of the group
+// summed on the way, in the order of the tiles.  d <= 64: both at once, [dO Q]^T [P dS], whose other two quarters are not used.
+// Q and dO are double buffered (192 KB of shared memory, one CTA an SM), and so are S and dP in tensor memory: the products of the next tile run under this
+// one's exponentials.  The softmax has eight warps, two to a quarter of the rows, 32 keys each.
+template <int DP> struct GradKVSmem {
+    static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2, kPBytes = kRows * kBlock * 2;
+    static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes, kBytes = kStage + 4 * kQBytes;   // P, dS; twice Q, dO
+    static constexpr int kBars = kEntries * sizeof(Entry);
+    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 16, kSP = kEmpty + 16, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
+                         kAbort = kDrain + 8, kHolder = kAbort + 4;
+    static_assert(kHolder + 4 <= 1024 && kBytes + 1024 <= 227 * 1024, "shared memory");
+};
+constexpr int kGradKVThreads = 320;
+template <typename T, int DP>
+__global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
+                                                                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, uint32_t *redo,
+                                                                    uint32_t *status) {
+    using M = GradKVSmem<DP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = tc::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t *sm = smem_raw + (base - raw);
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(sm + M::kAbort);
+    const Shape &s = a.s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t bh = blockIdx.x % ((int64_t)s.batch * s.kv_heads);   // the first blocks have most queries behind them: they go first, of all heads
+    const int j = (int)(blockIdx.x / ((int64_t)s.batch * s.kv_heads)), kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
+    const int len = s.length(b), live = a.tile * s.group;
+    pdl_launch_dependents();
+
+    if (threadIdx.x == 0) {
+        for (int bar : {M::kKV, M::kFull, M::kFull + 8, M::kEmpty, M::kEmpty + 8, M::kSP, M::kSP + 8, M::kDone, M::kDrain}) tc::mbar_init(base + bar, 1);
+        tc::mbar_init(base + M::kPds, 8);
+        for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+    }
+    if (warp == 9) {
+        tc::tmem_alloc(base + M::kHolder, 512);
+        tc::tmem_relinquish();
+    }
+    // rows of the last places, which no copy fills, are contracted over too: zeros
+    for (int x = threadIdx.x; x < (kRows - live) * 8 * 4 * (DP / 64); x += kGradKVThreads)
+        *reinterpret_cast<uint4 *>(sm + M::kStage + x / ((kRows - live) * 8) * (kRows * 128) + live * 128 + x % ((kRows - live) * 8) * 16) = make_uint4(0, 0, 0, 0);
+    tc::fence_proxy_async();
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder), tmem_acc = tmem + 256;
+    bool bad = false;
+
+    if (warp == 8) {
+        pdl_wait();
+        if (lane == 0) {
+            tc::mbar_expect_tx(base + M::kKV, 2 * M::kSlotBytes);
+            for (int y = 0; y < DP / 64; ++y) {
+                tc::tma_load_4d(base + M::kK + y * kBlock * 128, &map_k, base + M::kKV, y * 64, kvh, j * kBlock, b);
+                tc::tma_load_4d(base + M::kV + y * kBlock * 128, &map_v, base + M::kKV, y * 64, kvh, j * kBlock, b);
+            }
+        }
+        const uint32_t q_bytes = (uint32_t)(live * 128 * (DP / 64));
+        const int tiles = (s.queries + a.tile - 1) / a.tile;
+        const int shown = j * kBlock >= len ? tiles : s.causal ? max(0, j * kBlock - (s.keys - s.queries)) / a.tile : 0;   // no tile before can have the block
+        const uint32_t mask = a.tile >= 32 ? ~0u : (1u << a.tile) - 1;
+        const uint32_t *bits = a.bits + bh * s.words * s.blocks + j;
+        uint32_t then[4], now[4];
+        auto fetch = [&](int from) {
+            const int i0 = (from + lane) * a.tile;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                then[k] = from + lane < tiles && (k == 0 || 32 * k < a.tile) && (i0 >> 5) + k < s.words
+                              ? (__ldcg(bits + (int64_t)((i0 >> 5) + k) * s.blocks) >> (i0 & 31)) & mask
+                              : 0u;
+        };
+        uint32_t x = 0;
+        bool ok = true;
+        fetch(shown);
+        for (int from = shown; ok && from < tiles; from += 32) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) now[k] = then[k];
+            fetch(from + 32);
+            for (uint32_t some = __ballot_sync(~0u, (now[0] | now[1] | now[2] | now[3]) != 0); some && ok; some &= some - 1) {
+                const int src = __ffs(some) - 1;
+                uint32_t rows[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(~0u, now[k], src);
+                if (lane == 0) {
+                    ok = x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
+                    if (ok) {
+                        const int i0 = (from + src) * a.tile;
+                        Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
+                        *reinterpret_cast<uint4 *>(to->rows) = make_uint4(rows[0], rows[1], rows[2], rows[3]);
+                        to->block = i0;
+                        tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
+                        const uint32_t bar = base + M::kFull + 8 * (x & 1), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
+                        tc::mbar_expect_tx(bar, 2 * q_bytes);
+                        for (int y = 0; y < DP / 64; ++y) {
+                            tc::tma_load_4d(at + y * kRows * 128, &map_q, bar, y * 64, kvh * s.group, i0, b);
+                            tc::tma_load_4d(at + M::kQBytes + y * kRows * 128, &map_g, bar, y * 64, kvh * s.group, i0, b);
+                        }
+                    }
+                }
+                ok = __shfl_sync(~0u, (int)ok, 0);
+                ++x;
+            }
+        }
+        if (lane == 0) {
+            if (ok && (x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
+                reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
+                tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
+                tc::mbar_arrive(base + M::kFull + 8 * (x & 1));
+            }
+            if (*abort_flag)   // copies in flight end before the shared memory is given back
+                for (uint32_t z = x > 2 ? x - 2 : 0; z < x; ++z)
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (z & 1), (z >> 1) & 1); ++y) {}
+            for (uint32_t y = 0; y < tc::kMaxPolls && !tc::mbar_try_wait(base + M::kKV, 0); ++y) {}   // nobody else waits for these where no tile has the block
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescG = idesc<T>(DP == 64 ? 2 * kBlock : kBlock, 1, 1);
+            const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
+            const uint32_t k_lo = tc::smem_desc_lo(base + M::kK, 16), v_lo = tc::smem_desc_lo(base + M::kV, 16);
+            const uint32_t q_lo = tc::smem_desc_lo(base + M::kStage, 16), g_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, 16);
+            // contracted over the rows: 64-dimension slabs; at d <= 64 Q's slab and dO's are the two halves of one operand, P and dS of the other
+            const uint32_t qt_lo = tc::smem_desc_lo(base + M::kStage, kRows * 128), gt_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, kRows * 128);
+            const uint32_t p_lo = tc::smem_desc_lo(base + M::kP, M::kPBytes), ds_lo = tc::smem_desc_lo(base + M::kP + M::kPBytes, M::kPBytes);
+            bool ok = wait(base + M::kKV, 0, abort_flag);
+            uint32_t x = 0;
+            auto grads = [&](uint32_t y) {
+                const uint32_t at = (y & 1) * (2 * M::kQBytes >> 4);
+                if (!(ok = ok && wait(base + M::kPds, y & 1, abort_flag))) return;
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < kRows / 16; ++k) {
+                    if constexpr (DP == 64) {   // rows of the result: Q's dimensions, then dO's; columns: with P, then with dS
+                        tc::mma_f16_ss(tmem_acc, tc::desc64(qt_lo + at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, y > 0 || k > 0);
+                    } else {
+                        tc::mma_f16_ss(tmem_acc, tc::desc64(gt_lo + at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, y > 0 || k > 0);
+                        tc::mma_f16_ss(tmem_acc + 64, tc::desc64(qt_lo + at + 128 * k, hi), tc::desc64(ds_lo + 128 * k, hi), kIdescG, y > 0 || k > 0);
+                    }
+                }
+                tc::mma_commit(base + M::kDone);
+                tc::mma_commit(base + M::kEmpty + 8 * (y & 1));
+            };
+            for (; ok; ++x) {
+                const uint32_t at = (x & 1) * (2 * M::kQBytes >> 4), to = tmem + (x & 1) * 128;
+                ok = wait(base + M::kFull + 8 * (x & 1), (x >> 1) & 1, abort_flag);
+                if (!ok || reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0) break;
+                tc::tc_fence_after_sync();   // S and dP go where those of two tiles ago stood: read before P and dS were said to be there
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    tc::mma_f16_ss(to, tc::desc64(q_lo + at + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
+                                   tc::desc64(k_lo + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    tc::mma_f16_ss(to + 64, tc::desc64(g_lo + at + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
+                                   tc::desc64(v_lo + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
+                tc::mma_commit(base + M::kSP + 8 * (x & 1));
+                if (x > 0) grads(x - 1);
+            }
+            if (ok && x > 0) grads(x - 1);
+            tc::mma_commit(base + M::kDrain);
+            for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
+        }
+    } else {
+        const int quarter = warp & 3, half = warp >> 2;
+        const int r = quarter * 32 + lane, qx = r / s.group, g = r % s.group, h = kvh * s.group + g;
+        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + 32 * half;
+        const float c = a.scale * kLog2e;
+        float lift = 1.f;
+        uint32_t x = 0;
+        bool ok = true;
+        for (;; ++x) {
+            ok = __all_sync(~0u, wait(base + M::kE + 8 * (x % kEntries), (x / kEntries) & 1, abort_flag));
+            if (!ok) break;
+            const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm)[x % kEntries];
+            const int i0 = e.block, i = i0 + qx;
+            if (i0 < 0) break;
+            if (x == 0) lift = Lift<T>::grad(a.most) * exp2i(-Lift<T>::kWeight);   // the loader has waited for the kernels that wrote it
+            const bool listed = r < live && i < s.queries && (e.rows[qx >> 5] >> (qx & 31) & 1u);
+            const int n = listed ? min(kBlock, s.end(i, len) - j * kBlock) - 32 * half : 0;   // keys of the row from this warp's first on
+            float base2 = INFINITY, minus_delta = 0.f;
+            if (listed) {
+                const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+                base2 = __ldcg(a.lse + row) - Lift<T>::kWeight;
+                minus_delta = -__ldcg(a.delta + row) * lift;
+            }
+            ok = __all_sync(~0u, wait(base + M::kSP + 8 * (x & 1), (x >> 1) & 1, abort_flag));
+            if (!ok) break;
+            tc::tc_fence_after_sync();
+            const bool whole = __all_sync(~0u, n >= 32);
+            uint32_t u[32], d[32], p[16], ds[16];
+            tc::tmem_ld_x32_issue(mine + (x & 1) * 128, u);
+            tc::tmem_ld_x32_issue(mine + (x & 1) * 128 + 64, d);
+            tc::tmem_ld_x32_wait(u);
+            tc::tmem_ld_x32_wait(d);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                float w[2], f[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    w[y] = ex2(fmaf(__uint_as_float(u[2 * k + y]), c, -base2));
+                    f[y] = w[y] * fmaf(__uint_as_float(d[2 * k + y]), lift, minus_delta);
+                    if (!whole && 2 * k + y >= n) w[y] = f[y] = 0.f;
+                }
+                p[k] = pack2<T>(w[0], w[1]);
+                ds[k] = pack2<T>(f[0], f[1]);
+            }
+            if (x > 0 && !(ok = __all_sync(~0u, wait(base + M::kDone, (x - 1) & 1, abort_flag)))) break;   // P and dS of the tile before have been read
+            uint8_t *to = sm + M::kP + r * 128;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int at = ((4 * half + y) ^ (r & 7)) << 4;
+                *reinterpret_cast<uint4 *>(to + at) = make_uint4(p[4 * y], p[4 * y + 1], p[4 * y + 2], p[4 * y + 3]);
+                *reinterpret_cast<uint4 *>(to + M::kPBytes + at) = make_uint4(ds[4 * y], ds[4 * y + 1], ds[4 * y + 2], ds[4 * y + 3]);
+            }
+            tc::fence_proxy_async();
+            tc::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(base + M::kPds);
+        }
+        if (ok && x > 0) ok = __all_sync(~0u, wait(base + M::kDone, (x - 1) & 1, abort_flag));
+        if (ok) {
+            // accumulators: a dimension to a lane, keys in columns.  d > 64: dV in columns 0 .. 63, dK in 64 ..; d <= 64: dK in lanes 0 .. 63 of columns 64 ..,
+            // dV in lanes 64 .. of columns 0 ..  The two halves of the warps take one of the two each, or 32 keys each.
+            tc::tc_fence_after_sync();
+            const float back_v = exp2i(-Lift<T>::kWeight), back_k = x > 0 ? a.scale / (lift * exp2i(Lift<T>::kWeight)) : 0.f;
+            const uint32_t lanes = tmem_acc + ((uint32_t)(quarter * 32) << 16);
+            const bool is_k = DP == 64 ? quarter < 2 : half == 1;
+            const int dim = (DP == 64 ? quarter % 2 : quarter) * 32 + lane;
+            const float back = is_k ? back_k : back_v;
+            T *out = static_cast<T *>(is_k ? a.grad_k : a.grad_v) + (((int64_t)b * s.keys + j * kBlock) * s.kv_heads + kvh) * s.d + dim;
+            const int64_t pitch = (int64_t)s.kv_heads * s.d;
+            const int keys = min(kBlock, s.keys - j * kBlock);
+#pragma unroll
+            for (int part = 0; part < (DP == 64 ? 1 : 2); ++part) {
+                const int first = DP == 64 ? 32 * half : 32 * part;
+                uint32_t o[32];
+                if (x > 0) tc::tmem_ld_x32(lanes + (is_k ? 64 : 0) + first, o);
+#pragma unroll
+                for (int y = 0; y < 32; ++y) {
+                    const float f = x > 0 ? __uint_as_float(o[y]) * back : 0.f;
+                    if (dim < s.d && first + y < keys) {
+                        bad |= !finite(f);
+                        out[(first + y) * pitch] = from_f32<T>(f);
+                    }
+                }
+            }
+        }
+    }
+    tc::tc_fence_before_sync();
+    const bool again = __syncthreads_or(bad);
+    if (threadIdx.x == 0) {
+        redo[bh * s.blocks + j] = again;
+        if (*abort_flag) atomicOr(status, kStatusGradKV);
+    }
+    if (warp == 9) {
+        tc::tc_fence_after_sync();
+        tc::tmem_dealloc(tmem, 512);
     }
 }
 
