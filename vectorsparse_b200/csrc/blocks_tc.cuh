@@ -39,6 +39,34 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two at a time: one instruction each on this part.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float2 pair(uint32_t x, uint32_t y) { return make_float2(__uint_as_float(x), __uint_as_float(y)); }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -311,20 +339,21 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             ok = __all_sync(~0u, wait(base + M::kS + 8 * (x & 1), (x >> 1) & 1, abort_flag));
             if (!ok) break;
             tc::tc_fence_after_sync();
-            uint32_t u[2][32];
-            tc::tmem_ld_x32_issue(mine + (x & 1) * 64, u[0]);
-            tc::tmem_ld_x32_issue(mine + (x & 1) * 64 + 32, u[1]);
-            tc::tmem_ld_x32_wait(u[0]);
-            tc::tmem_ld_x32_wait(u[1]);
-            if (!__all_sync(~0u, n == kBlock)) {
+            uint32_t u[64];
+            uint32_t (&lo)[32] = *reinterpret_cast<uint32_t (*)[32]>(u), (&hi)[32] = *reinterpret_cast<uint32_t (*)[32]>(u + 32);
+            tc::tmem_ld_x32_issue(mine + (x & 1) * 64, lo);
+            tc::tmem_ld_x32_issue(mine + (x & 1) * 64 + 32, hi);
+            tc::tmem_ld_x32_wait(lo);
+            tc::tmem_ld_x32_wait(hi);
+            if (__any_sync(~0u, n > 0 && n < kBlock)) {   // a block that ends inside: the queries' own, mostly
 #pragma unroll
                 for (int k = 0; k < kBlock; ++k)
-                    if (k >= n) u[k / 32][k % 32] = __float_as_uint(-INFINITY);
+                    if (k >= n) u[k] = __float_as_uint(-INFINITY);
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 0; k < kBlock; ++k) m[k % 4] = fmaxf(m[k % 4], __uint_as_float(u[k / 32][k % 32]));
-            const float high = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c;
+            for (int k = 0; k < kBlock; k += 2) m[k / 2 % 4] = max3(m[k / 2 % 4], __uint_as_float(u[k]), __uint_as_float(u[k + 1]));
+            const float high = n > 0 ? fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c : -INFINITY;
             if (__any_sync(~0u, high > top + kSlack)) {
                 const float to = fmaxf(top, high), shrink = to == -INFINITY ? 1.f : ex2(top - to);
                 top = to;
@@ -343,17 +372,20 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                     }
                 }
             }
-            const float off = top == -INFINITY ? 0.f : -top;
-            float sum[4] = {};
+            // a row that has not listed the block has no weight there: its scores, finite ones, all end at -inf
+            const float off = n <= 0 ? -INFINITY : top == -INFINITY ? 0.f : -top;
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             uint32_t p[32];
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
-                const float y = ex2(fmaf(__uint_as_float(u[k / 16][2 * k % 32]), c, off)), z = ex2(fmaf(__uint_as_float(u[k / 16][2 * k % 32 + 1]), c, off));
-                sum[2 * k % 4] += y;
-                sum[2 * k % 4 + 1] += z;
-                p[k] = pack2<T>(y, z);
+                float2 y = fma2(pair(u[2 * k], u[2 * k + 1]), make_float2(c, c), make_float2(off, off));
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+                sum[k % 2] = add2(sum[k % 2], y);
+                p[k] = pack2<T>(y.x, y.y);
             }
-            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            sum[0] = add2(sum[0], sum[1]);
+            total += sum[0].x + sum[0].y;
             tc::tmem_st_x32(mine + (x & 1) * 64, p);
             tc::tmem_st_wait();
             tc::tc_fence_before_sync();
@@ -583,7 +615,8 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
             ok = __all_sync(~0u, wait(base + M::kSP, x & 1, abort_flag));
             if (!ok) break;
             tc::tc_fence_after_sync();
-            const bool whole = __all_sync(~0u, n == kBlock);
+            const bool whole = __all_sync(~0u, n <= 0 || n == kBlock);
+            const float off = n > 0 ? -lse : -INFINITY;   // a row that has not listed the block has no weight there
             uint32_t ds[32];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -594,13 +627,15 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
                 tc::tmem_ld_x32_wait(d);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    float f[2];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        f[y] = ex2(fmaf(__uint_as_float(u[2 * k + y]), c, -lse)) * fmaf(__uint_as_float(d[2 * k + y]), lift, minus_delta);
-                        if (!whole && 32 * half + 2 * k + y >= n) f[y] = 0.f;
+                    float2 w = fma2(pair(u[2 * k], u[2 * k + 1]), make_float2(c, c), make_float2(off, off));
+                    w.x = ex2(w.x);
+                    w.y = ex2(w.y);
+                    float2 f = mul2(w, fma2(pair(d[2 * k], d[2 * k + 1]), make_float2(lift, lift), make_float2(minus_delta, minus_delta)));
+                    if (!whole) {
+                        if (32 * half + 2 * k >= n) f.x = 0.f;
+                        if (32 * half + 2 * k + 1 >= n) f.y = 0.f;
                     }
-                    ds[16 * half + k] = pack2<T>(f[0], f[1]);
+                    ds[16 * half + k] = pack2<T>(f.x, f.y);
                 }
             }
             tc::tmem_st_x32(mine, ds);
@@ -830,7 +865,7 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
             ok = __all_sync(~0u, wait(base + M::kSP + 8 * (x & 1), (x >> 1) & 1, abort_flag));
             if (!ok) break;
             tc::tc_fence_after_sync();
-            const bool whole = __all_sync(~0u, n >= 32);
+            const bool whole = __all_sync(~0u, !listed || n >= 32);   // a row that has not listed the block has no weight there: base2
             uint32_t u[32], d[32], p[16], ds[16];
             tc::tmem_ld_x32_issue(mine + (x & 1) * 128, u);
             tc::tmem_ld_x32_issue(mine + (x & 1) * 128 + 64, d);
@@ -838,15 +873,16 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
             tc::tmem_ld_x32_wait(d);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                float w[2], f[2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    w[y] = ex2(fmaf(__uint_as_float(u[2 * k + y]), c, -base2));
-                    f[y] = w[y] * fmaf(__uint_as_float(d[2 * k + y]), lift, minus_delta);
-                    if (!whole && 2 * k + y >= n) w[y] = f[y] = 0.f;
+                float2 w = fma2(pair(u[2 * k], u[2 * k + 1]), make_float2(c, c), make_float2(-base2, -base2));
+                w.x = ex2(w.x);
+                w.y = ex2(w.y);
+                float2 f = mul2(w, fma2(pair(d[2 * k], d[2 * k + 1]), make_float2(lift, lift), make_float2(minus_delta, minus_delta)));
+                if (!whole) {
+                    if (2 * k >= n) w.x = f.x = 0.f;
+                    if (2 * k + 1 >= n) w.y = f.y = 0.f;
                 }
-                p[k] = pack2<T>(w[0], w[1]);
-                ds[k] = pack2<T>(f[0], f[1]);
+                p[k] = pack2<T>(w.x, w.y);
+                ds[k] = pack2<T>(f.x, f.y);
             }
             if (x > 0 && !(ok = __all_sync(~0u, wait(base + M::kDone, (x - 1) & 1, abort_flag)))) break;   // P and dS of the tile before have been read
             uint8_t *to = sm + M::kP + r * 128;
