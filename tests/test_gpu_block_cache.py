@@ -293,3 +293,35 @@ def test_refusals():
     odd = torch_ops.BlockCache.empty(2, 2, 1, 24, torch.float16, DEV)
     with pytest.raises(VsError):
         torch_ops.cache_append(odd, *(torch.zeros((1, 1, 1, 24), dtype=torch.float16, device=DEV),) * 2, m.dev[0][:1], m.dev[1][:1], n[:1])
+
+
+def test_a_dispatch_mode_sees_the_operators():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func.namespace == "vsparse":
+                self.seen.append(func.overloadpacket.__name__)
+            return func(*args, **(kwargs or {}))
+
+    m = filled(2, [70, 130], 1, 64, torch.float16, room=1)
+    q = randn(2, 4, 64, dtype=torch.float16, seed=0)
+    lists = torch_ops.cache_select(q, m.cache, m.dev[0], m.lengths(), 2)
+    out = torch_ops.cache_attention(q, m.cache, *m.dev, m.lengths(), 0.125, lists)
+    x = q[None]
+    leaf = x.clone().requires_grad_()
+    blocks = torch_ops.select_blocks(x, x[:, :, :2], 1)
+    with Names() as mode:
+        assert torch.equal(torch_ops.cache_select(q, m.cache, m.dev[0], m.lengths(), 2), lists)
+        assert torch.equal(torch_ops.cache_attention(q, m.cache, *m.dev, m.lengths(), 0.125, lists), out)
+        m.append(randn(2, 3, 1, 64, dtype=torch.float16, seed=1), randn(2, 3, 1, 64, dtype=torch.float16, seed=2))
+        assert torch.equal(torch_ops.select_blocks(x, x[:, :, :2], 1), blocks)
+        torch_ops.selected_attention(leaf, x[:, :, :2], x[:, :, :2], blocks, 0.125).sum().backward()
+        torch_ops.selected_attention(x, x[:, :, :2], x[:, :, :2], blocks, 0.125)
+    m.check()
+    assert mode.seen == ["cache_select", "cache_attention", "cache_append", "select_blocks", "selected_attention", "selected_attention_backward", "selected_attention"]
+    assert torch.isfinite(leaf.grad).all()

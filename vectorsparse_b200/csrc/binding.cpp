@@ -50,6 +50,18 @@ struct Library {
     decltype(&vs_attention_cvse_backward) attention_backward;
 } g_lib;
 
+struct BlockLibrary {   // attention over chosen blocks, the cache
+    decltype(&vs_select_blocks_workspace_bytes) select_blocks_workspace;
+    decltype(&vs_select_blocks) select_blocks;
+    decltype(&vs_selected_attention_workspace_bytes) selected_attention_workspace;
+    decltype(&vs_selected_attention) selected_attention;
+    decltype(&vs_selected_attention_backward) selected_attention_backward;
+    decltype(&vs_cache_append) cache_append;
+    decltype(&vs_cache_select) cache_select;
+    decltype(&vs_cache_attention_workspace_bytes) cache_attention_workspace;
+    decltype(&vs_cache_attention) cache_attention;
+} g_blocks;
+
 // The arguments of one call: `ok` turns false at the first one the fast path does not take.
 struct Args {
     PyObject *const *argv;
@@ -93,6 +105,44 @@ struct Args {
         if (device < 0) device = dev;
         if (dev != device) ok = false;
         return &t;
+    }
+    // a CUDA tensor of `dims` dimensions in a layout that the block operators take, and the strides of all but its last dimension
+    const at::Tensor *strided(int i, int dims, int64_t *strides) {
+        if (!ok || !THPVariable_Check(argv[i])) {
+            ok = false;
+            return nullptr;
+        }
+        const at::Tensor &t = THPVariable_Unpack(argv[i]);
+        if (!t.is_cuda() || t.dim() != dims || t.stride(dims - 1) != 1 || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u)) {
+            ok = false;
+            return nullptr;
+        }
+        for (int d = 0; d < dims - 1; ++d) {
+            strides[d] = t.size(d) > 1 ? t.stride(d) : 8;
+            if (strides[d] <= 0 || strides[d] % 8 != 0 || t.size(d) > INT_MAX) ok = false;
+        }
+        const int dev = t.get_device();
+        if (device < 0) device = dev;
+        if (dev != device) ok = false;
+        return &t;
+    }
+    bool flag(int i) {
+        if (argv[i] != Py_True && argv[i] != Py_False) ok = false;
+        return argv[i] == Py_True;
+    }
+    int dtype16(const at::Tensor *t) {
+        if (ok && t->scalar_type() == at::kHalf) return VS_F16;
+        if (ok && t->scalar_type() == at::kBFloat16) return VS_BF16;
+        ok = false;
+        return -1;
+    }
+    // a contiguous int32 tensor of exactly this many elements, or null for None
+    const int32_t *exactly(int i, int64_t numel) {
+        if (none(i)) return nullptr;
+        const at::Tensor *t = tensor(i);
+        type(t, at::kInt);
+        if (ok && t->numel() != numel) ok = false;
+        return ok ? static_cast<const int32_t *>(t->const_data_ptr()) : nullptr;
     }
     void need(const at::Tensor *t, int64_t numel) {
         if (!ok || t->numel() < numel) ok = false;
@@ -515,6 +565,268 @@ PyObject *differentiable(PyObject *, PyObject *const *argv, Py_ssize_t n_args) {
     }
 }
 
+// ---- attention over chosen blocks, the cache ------------------------------------------------------------------------------
+// These allocate their results and workspaces and answer with the results, or None (the Python operator then makes its checks and the call).
+
+struct On {   // makes a device current for the allocations and the call
+    c10::cuda::OptionalCUDAGuard guard;
+    void *stream;
+    explicit On(int device) {
+        if (c10::cuda::current_device() != device) guard.set_index((c10::DeviceIndex)device);
+        stream = (void *)c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    }
+};
+at::Tensor scratch(const at::Tensor &like, int64_t bytes) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+PyObject *wrap(std::initializer_list<at::Tensor> list) {
+    PyObject *out = PyTuple_New((Py_ssize_t)list.size());
+    Py_ssize_t i = 0;
+    for (const at::Tensor &t : list) {
+        PyObject *x = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
+        if (!x) {
+            Py_XDECREF(out);
+            return nullptr;
+        }
+        if (out) PyTuple_SET_ITEM(out, i++, x);
+    }
+    return out;
+}
+
+struct Sizes {
+    int batch, queries, keys, heads, kv_heads, d;
+    bool of(const at::Tensor *q, const at::Tensor *k) {
+        if (k->size(0) != q->size(0) || k->size(3) != q->size(3) || q->size(3) > INT_MAX || k->scalar_type() != q->scalar_type()) return false;
+        batch = (int)q->size(0); queries = (int)q->size(1); heads = (int)q->size(2); d = (int)q->size(3);
+        keys = (int)k->size(1); kv_heads = (int)k->size(2);
+        return true;
+    }
+    bool lists(const at::Tensor *b) const {
+        return b->dim() == 4 && b->size(0) == batch && b->size(1) == kv_heads && b->size(2) == queries && b->size(3) >= 1 && b->size(3) <= INT_MAX;
+    }
+};
+
+// select_blocks(q, k, count, causal, lengths | None) -> blocks
+VS_FAST_CALL(select_blocks, 5) {
+    int64_t sq[3], sk[3];
+    const at::Tensor *q = a.strided(0, 4, sq), *k = a.strided(1, 4, sk);
+    const int count = a.integer(2), causal = a.flag(3);
+    Sizes z;
+    if (!a.ok || count < 1 || !z.of(q, k)) Py_RETURN_NONE;
+    const int32_t *lengths = a.exactly(4, z.batch);
+    const int t = a.dtype16(q);
+    if (!a.ok) Py_RETURN_NONE;
+    On on(a.device);
+    at::Tensor blocks = at::empty({z.batch, z.kv_heads, z.queries, count}, q->options().dtype(at::kInt));
+    const int64_t bytes = g_blocks.select_blocks_workspace(z.batch, z.keys, z.kv_heads, z.d);
+    at::Tensor ws = scratch(*q, bytes);
+    const void *pq = q->const_data_ptr(), *pk = k->const_data_ptr();
+    int32_t *pb = static_cast<int32_t *>(blocks.mutable_data_ptr());
+    void *pw = ws.mutable_data_ptr();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_blocks.select_blocks(t, z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.d, count, causal, pq, sq, pk, sk, lengths, pb, pw, bytes, on.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(blocks));
+}
+
+// selected_attention(q, k, v, blocks, scale, causal, lengths | None, low) -> (out, lse, out_low | None)
+VS_FAST_CALL(selected_attention, 8) {
+    int64_t sq[3], sk[3], sv[3];
+    const at::Tensor *q = a.strided(0, 4, sq), *k = a.strided(1, 4, sk), *v = a.strided(2, 4, sv), *blocks = a.tensor(3);
+    const double scale = a.number(4);
+    const int causal = a.flag(5);
+    const bool low = a.flag(7);
+    a.type(blocks, at::kInt);
+    Sizes z;
+    if (!a.ok || !z.of(q, k) || v->sizes() != k->sizes() || v->scalar_type() != q->scalar_type() || !z.lists(blocks)) Py_RETURN_NONE;
+    const int32_t *lengths = a.exactly(6, z.batch);
+    const int t = a.dtype16(q);
+    if (!a.ok) Py_RETURN_NONE;
+    On on(a.device);
+    at::Tensor out = at::empty(q->sizes(), q->options()), lse = at::empty({z.batch, z.heads, z.queries}, q->options().dtype(at::kFloat)), out_low;
+    if (low) out_low = at::empty(q->sizes(), q->options());
+    const int64_t bytes = g_blocks.selected_attention_workspace(z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.d, 0);
+    at::Tensor ws = scratch(*q, bytes);
+    const void *pq = q->const_data_ptr(), *pk = k->const_data_ptr(), *pv = v->const_data_ptr();
+    const int32_t *pb = static_cast<const int32_t *>(blocks->const_data_ptr());
+    const int count = (int)blocks->size(3);
+    void *po = out.mutable_data_ptr(), *pl = low ? out_low.mutable_data_ptr() : nullptr, *pw = ws.mutable_data_ptr();
+    float *ps = static_cast<float *>(lse.mutable_data_ptr());
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_blocks.selected_attention(t, z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.d, count, causal, pq, sq, pk, sk, pv, sv, lengths, pb, po, pl, ps, (float)scale,
+                                  pw, bytes, on.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return wrap({out, lse, out_low});
+}
+
+// selected_attention_backward(q, k, v, blocks, out, out_low | None, lse, grad_out, scale, causal, lengths | None) -> (grad_q, grad_k, grad_v)
+VS_FAST_CALL(selected_attention_backward, 11) {
+    int64_t sq[3], sk[3], sv[3], sg[3];
+    const at::Tensor *q = a.strided(0, 4, sq), *k = a.strided(1, 4, sk), *v = a.strided(2, 4, sv), *blocks = a.tensor(3), *out = a.tensor(4);
+    const at::Tensor *low = a.none(5) ? nullptr : a.tensor(5), *lse = a.tensor(6), *g = a.strided(7, 4, sg);
+    const double scale = a.number(8);
+    const int causal = a.flag(9);
+    a.type(blocks, at::kInt);
+    a.type(lse, at::kFloat);
+    Sizes z;
+    if (!a.ok || !z.of(q, k) || v->sizes() != k->sizes() || v->scalar_type() != q->scalar_type() || !z.lists(blocks)) Py_RETURN_NONE;
+    for (const at::Tensor *x : {out, low, g})
+        if (x && (x->sizes() != q->sizes() || x->scalar_type() != q->scalar_type())) Py_RETURN_NONE;
+    if (lse->numel() != (int64_t)z.batch * z.heads * z.queries) Py_RETURN_NONE;
+    const int32_t *lengths = a.exactly(10, z.batch);
+    const int t = a.dtype16(q);
+    if (!a.ok) Py_RETURN_NONE;
+    On on(a.device);
+    at::Tensor gq = at::empty(q->sizes(), q->options()), gk = at::empty(k->sizes(), k->options()), gv = at::empty(k->sizes(), k->options());
+    const int64_t bytes = g_blocks.selected_attention_workspace(z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.d, 1);
+    at::Tensor ws = scratch(*q, bytes);
+    const void *pq = q->const_data_ptr(), *pk = k->const_data_ptr(), *pv = v->const_data_ptr(), *po = out->const_data_ptr(), *pg = g->const_data_ptr();
+    const void *pl = low ? low->const_data_ptr() : nullptr;
+    const int32_t *pb = static_cast<const int32_t *>(blocks->const_data_ptr());
+    const float *ps = static_cast<const float *>(lse->const_data_ptr());
+    const int count = (int)blocks->size(3);
+    void *dq = gq.mutable_data_ptr(), *dk = gk.mutable_data_ptr(), *dv = gv.mutable_data_ptr(), *pw = ws.mutable_data_ptr();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_blocks.selected_attention_backward(t, z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.d, count, causal, pq, sq, pk, sk, pv, sv, lengths, pb, po, pl, ps, pg,
+                                           sg, dq, dk, dv, (float)scale, pw, bytes, on.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return wrap({gq, gk, gv});
+}
+
+// The tensors of a BlockCache, whose shapes and types it has checked itself: (k_codes, v_codes, k_scales, v_scales, k_sums, k_ring, v_ring)
+struct Cache {
+    const at::Tensor *t[7];
+    int pages, tails, kv_heads, d, type;
+    bool of(Args &a, int i) {
+        if (!PyTuple_CheckExact(a.argv[i]) || PyTuple_GET_SIZE(a.argv[i]) != 7) return false;
+        for (int x = 0; x < 7; ++x) {
+            PyObject *o = PyTuple_GET_ITEM(a.argv[i], x);
+            if (!THPVariable_Check(o)) return false;
+            t[x] = &THPVariable_Unpack(o);
+            if (!t[x]->is_cuda()) return false;
+            const int dev = t[x]->get_device();
+            if (a.device < 0) a.device = dev;
+            if (dev != a.device) return false;
+        }
+        if (t[0]->size(0) > INT_MAX || t[5]->size(0) > INT_MAX) return false;
+        pages = (int)t[0]->size(0); kv_heads = (int)t[0]->size(1); d = (int)t[0]->size(3); tails = (int)t[5]->size(0);
+        type = a.dtype16(t[5]);
+        return a.ok;
+    }
+    template <typename T> T *at(int x) const { return static_cast<T *>(t[x]->data_ptr()); }
+};
+// [n, max_blocks] int32
+const int32_t *table_of(Args &a, int i, int64_t n, int &max_blocks) {
+    const at::Tensor *t = a.tensor(i);
+    a.type(t, at::kInt);
+    if (!a.ok || t->dim() != 2 || t->size(0) != n || t->size(1) > INT_MAX) {
+        a.ok = false;
+        return nullptr;
+    }
+    max_blocks = (int)t->size(1);
+    return static_cast<const int32_t *>(t->const_data_ptr());
+}
+
+// cache_append(parts, k, v, table, tails, lengths, counts | None) -> 0
+VS_FAST_CALL(cache_append, 7) {
+    Cache c;
+    int64_t sk[3], sv[3];
+    if (!c.of(a, 0)) Py_RETURN_NONE;
+    const at::Tensor *k = a.strided(1, 4, sk), *v = a.strided(2, 4, sv);
+    if (!a.ok || k->size(2) != c.kv_heads || k->size(3) != c.d || v->sizes() != k->sizes() || a.dtype16(k) != c.type || a.dtype16(v) != c.type) Py_RETURN_NONE;
+    const int n = (int)k->size(0), tokens = (int)k->size(1);
+    int max_blocks = 0;
+    const int32_t *table = table_of(a, 3, n, max_blocks), *tails = a.exactly(4, n), *lengths = a.exactly(5, n), *counts = a.exactly(6, n);
+    if (!a.ok || a.none(4) || a.none(5)) Py_RETURN_NONE;
+    const void *pk = k->const_data_ptr(), *pv = v->const_data_ptr();
+    On on(a.device);
+    int8_t *kc = c.at<int8_t>(0), *vc = c.at<int8_t>(1);
+    float *ks = c.at<float>(2), *vs = c.at<float>(3);
+    int16_t *sums = c.at<int16_t>(4);
+    void *kr = c.at<void>(5), *vr = c.at<void>(6);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_blocks.cache_append(c.type, c.pages, c.tails, c.kv_heads, c.d, kc, vc, ks, vs, sums, kr, vr, n, tokens, pk, sk, pv, sv, table, max_blocks, tails, lengths, counts,
+                            on.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return PyLong_FromLong(0);
+}
+
+// q [n, heads, d] of a call on a cache
+const at::Tensor *token_of(Args &a, int i, const Cache &c, int64_t *strides) {
+    const at::Tensor *q = a.strided(i, 3, strides);
+    if (!a.ok || q->size(2) != c.d || q->size(1) < c.kv_heads || c.kv_heads < 1 || q->size(1) % c.kv_heads != 0 || a.dtype16(q) != c.type) a.ok = false;
+    return q;
+}
+
+// cache_select(parts, q, table, lengths, count) -> blocks
+VS_FAST_CALL(cache_select, 5) {
+    Cache c;
+    int64_t sq[2];
+    if (!c.of(a, 0)) Py_RETURN_NONE;
+    const at::Tensor *q = token_of(a, 1, c, sq);
+    const int count = a.integer(4);
+    if (!a.ok || count < 1) Py_RETURN_NONE;
+    const int n = (int)q->size(0), heads = (int)q->size(1);
+    int max_blocks = 0;
+    const int32_t *table = table_of(a, 2, n, max_blocks), *lengths = a.exactly(3, n);
+    if (!a.ok || a.none(3)) Py_RETURN_NONE;
+    On on(a.device);
+    at::Tensor blocks = at::empty({n, c.kv_heads, count}, q->options().dtype(at::kInt));
+    const void *pq = q->const_data_ptr();
+    const float *ks = c.at<float>(2);
+    const int16_t *sums = c.at<int16_t>(4);
+    int32_t *pb = static_cast<int32_t *>(blocks.mutable_data_ptr());
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_blocks.cache_select(c.type, c.pages, heads, c.kv_heads, c.d, ks, sums, n, pq, sq, table, max_blocks, lengths, count, pb, on.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(blocks));
+}
+
+// cache_attention(parts, q, table, tails, lengths, scale, blocks | None) -> out
+VS_FAST_CALL(cache_attention, 7) {
+    Cache c;
+    int64_t sq[2];
+    if (!c.of(a, 0)) Py_RETURN_NONE;
+    const at::Tensor *q = token_of(a, 1, c, sq);
+    const double scale = a.number(5);
+    if (!a.ok) Py_RETURN_NONE;
+    const int n = (int)q->size(0), heads = (int)q->size(1);
+    int max_blocks = 0, count = 0;
+    const int32_t *table = table_of(a, 2, n, max_blocks), *tails = a.exactly(3, n), *lengths = a.exactly(4, n), *lists = nullptr;
+    if (!a.none(6)) {
+        const at::Tensor *b = a.tensor(6);
+        a.type(b, at::kInt);
+        if (!a.ok || b->dim() != 3 || b->size(0) != n || b->size(1) != c.kv_heads || b->size(2) < 1 || b->size(2) > INT_MAX) Py_RETURN_NONE;
+        lists = static_cast<const int32_t *>(b->const_data_ptr());
+        count = (int)b->size(2);
+        if (n == 0) lists = nullptr;
+    }
+    if (!a.ok || a.none(3) || a.none(4)) Py_RETURN_NONE;
+    On on(a.device);
+    at::Tensor out = at::empty(q->sizes(), q->options()), ws;
+    const int64_t bytes = g_blocks.cache_attention_workspace(n, heads, c.kv_heads, c.d, lists ? count : max_blocks);
+    if (bytes) ws = scratch(*q, bytes);
+    const void *pq = q->const_data_ptr(), *kr = c.at<void>(5), *vr = c.at<void>(6);
+    const int8_t *kc = c.at<int8_t>(0), *vc = c.at<int8_t>(1);
+    const float *ks = c.at<float>(2), *vs = c.at<float>(3);
+    void *po = out.mutable_data_ptr(), *pw = bytes ? ws.mutable_data_ptr() : nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_blocks.cache_attention(c.type, c.pages, c.tails, heads, c.kv_heads, c.d, kc, vc, ks, vs, kr, vr, n, pq, sq, table, max_blocks, tails, lengths, lists, count, po,
+                               (float)scale, pw, bytes, on.stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+}
+
 PyObject *bind_backward(PyObject *, PyObject *const *argv, Py_ssize_t n) {
     if (n != 1 || !PyCallable_Check(argv[0])) {
         PyErr_SetString(PyExc_TypeError, "bind_backward: a function");
@@ -525,14 +837,13 @@ PyObject *bind_backward(PyObject *, PyObject *const *argv, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
-// bind(addresses): the library's functions in the order of struct Library
-PyObject *bind(PyObject *, PyObject *const *argv, Py_ssize_t n) {
-    constexpr Py_ssize_t kCount = sizeof(Library) / sizeof(void *);
+template <typename L> PyObject *bind_to(L &lib, PyObject *const *argv, Py_ssize_t n) {
+    constexpr Py_ssize_t kCount = sizeof(L) / sizeof(void *);
     if (n != kCount) {
         PyErr_SetString(PyExc_TypeError, "bind: wrong number of addresses");
         return nullptr;
     }
-    void **slot = reinterpret_cast<void **>(&g_lib);
+    void **slot = reinterpret_cast<void **>(&lib);
     for (Py_ssize_t i = 0; i < n; ++i) {
         slot[i] = PyLong_AsVoidPtr(argv[i]);
         if (!slot[i]) {
@@ -542,11 +853,15 @@ PyObject *bind(PyObject *, PyObject *const *argv, Py_ssize_t n) {
     }
     Py_RETURN_NONE;
 }
+// bind(addresses), bind_blocks(addresses): the library's functions in the order of struct Library and struct BlockLibrary
+PyObject *bind(PyObject *, PyObject *const *argv, Py_ssize_t n) { return bind_to(g_lib, argv, n); }
+PyObject *bind_blocks(PyObject *, PyObject *const *argv, Py_ssize_t n) { return bind_to(g_blocks, argv, n); }
 
 #define VS_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {
-    VS_METHOD(bind), VS_METHOD(spmm), VS_METHOD(spmm_t), VS_METHOD(sddmm), VS_METHOD(softmax), VS_METHOD(softmax_backward),
-    VS_METHOD(attention), VS_METHOD(attention_backward), VS_METHOD(differentiable), VS_METHOD(bind_backward), {nullptr, nullptr, 0, nullptr},
+    VS_METHOD(bind), VS_METHOD(bind_blocks), VS_METHOD(spmm), VS_METHOD(spmm_t), VS_METHOD(sddmm), VS_METHOD(softmax), VS_METHOD(softmax_backward),
+    VS_METHOD(attention), VS_METHOD(attention_backward), VS_METHOD(differentiable), VS_METHOD(bind_backward), VS_METHOD(select_blocks),
+    VS_METHOD(selected_attention), VS_METHOD(selected_attention_backward), VS_METHOD(cache_append), VS_METHOD(cache_select), VS_METHOD(cache_attention), {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_binding", "torch tensors to the C ABI of libvsparse_b200", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};

@@ -34,10 +34,15 @@ _DT = {torch.float16: VS_F16, torch.float32: VS_F32}
 
 
 def _bind() -> None:
-    """Hands the binding the functions of the library that _lib has loaded, in the order of its `Library` struct."""
-    names = ("vs_spmm_batched", "vs_spmm_t_batched", "vs_sddmm_batched", "vs_softmax_cvse", "vs_softmax_cvse_backward",
-             "vs_attention_cvse", "vs_attention_cvse_backward")
-    _binding.bind(*(ctypes.cast(getattr(_lib.lib(), n), ctypes.c_void_p).value for n in names))
+    """Hands the binding the functions of the library that _lib has loaded, in the order of its `Library` and `BlockLibrary` structs."""
+    def addresses(*names):
+        return (ctypes.cast(getattr(_lib.lib(), n), ctypes.c_void_p).value for n in names)
+
+    _binding.bind(*addresses("vs_spmm_batched", "vs_spmm_t_batched", "vs_sddmm_batched", "vs_softmax_cvse", "vs_softmax_cvse_backward",
+                             "vs_attention_cvse", "vs_attention_cvse_backward"))
+    _binding.bind_blocks(*addresses("vs_select_blocks_workspace_bytes", "vs_select_blocks", "vs_selected_attention_workspace_bytes",
+                                    "vs_selected_attention", "vs_selected_attention_backward", "vs_cache_append", "vs_cache_select",
+                                    "vs_cache_attention_workspace_bytes", "vs_cache_attention"))
 
 
 _bind()
@@ -516,8 +521,10 @@ class BlockCache:
                                       (k_sums, "k_sums", (pages, heads, d), torch.int16), (k_ring, "k_ring", k_ring.shape, k_ring.dtype),
                                       (v_ring, "v_ring", k_ring.shape, k_ring.dtype)):
             _shaped(t, name, shape, dtype)
-        self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.k_sums, self.k_ring, self.v_ring = k_codes, v_codes, k_scales, v_scales, k_sums, k_ring, v_ring
+        self._parts = (k_codes, v_codes, k_scales, v_scales, k_sums, k_ring, v_ring)
         self.pages, self.tails, self.kv_heads, self.d, self.dtype = pages, k_ring.shape[0], heads, d, k_ring.dtype
+
+    k_codes, v_codes, k_scales, v_scales, k_sums, k_ring, v_ring = (property(lambda self, i=i: self._parts[i]) for i in range(7))
 
     @classmethod
     def empty(cls, pages, tails, kv_heads, d, dtype, device):
@@ -527,8 +534,7 @@ class BlockCache:
         return cls(*codes, *scales, torch.zeros((pages, kv_heads, d), dtype=torch.int16, device=device), *rings)
 
     def _tensors(self):
-        return dict(k_codes=self.k_codes, v_codes=self.v_codes, k_scales=self.k_scales, v_scales=self.v_scales, k_sums=self.k_sums, k_ring=self.k_ring,
-                    v_ring=self.v_ring)
+        return dict(zip(("k_codes", "v_codes", "k_scales", "v_scales", "k_sums", "k_ring", "v_ring"), self._parts))
 
 
 def _table(table, n):

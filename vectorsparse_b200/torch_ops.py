@@ -82,11 +82,14 @@ def _through(kernel, op, operands, *args):
     """The registered operator `op`, whose CUDA kernel is `kernel`.  The dispatcher's way there and back costs the host ~10 us
     a call, so plain CUDA tensors with nobody listening go to the kernel at once; modes of either kind (tracers, fake tensors, user
     modes), torch.jit.trace, a running profiler, tensor subclasses and a backward pass that is itself differentiated see the operator."""
+    return kernel(*args) if not torch.is_grad_enabled() and _quiet(operands) else op(*args)
+
+
+def _quiet(operands):
+    """Whether nobody listens to the dispatcher and the operands are plain CUDA tensors."""
     heard = (torch._C._len_torch_dispatch_stack() or _len_pre_dispatch() or torch._C._len_torch_function_stack()
-             or torch._C._get_tracing_state() is not None or torch.autograd.profiler._is_profiler_enabled or torch.is_grad_enabled())
-    if not heard and all((type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and t.is_cuda for t in operands):
-        return kernel(*args)
-    return op(*args)
+             or torch._C._get_tracing_state() is not None or torch.autograd.profiler._is_profiler_enabled)
+    return not heard and all((type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and t.is_cuda for t in operands)
 
 
 _LIB.impl("spmm", _spmm, "CUDA")
@@ -221,6 +224,9 @@ def _scratch(nbytes, device):
 
 
 def _select_blocks(q, k, count, causal, lengths):
+    blocks = ops._binding.select_blocks(q, k, count, causal, lengths)
+    if blocks is not None:
+        return blocks
     q, k = _usable(q), _usable(k)
     blocks = torch.empty((q.shape[0], k.shape[2], q.shape[1], count), dtype=torch.int32, device=q.device)
     ops.select_blocks(q, k, blocks, _scratch(ops.select_blocks_workspace(q, k), q.device), causal, lengths)
@@ -228,6 +234,9 @@ def _select_blocks(q, k, count, causal, lengths):
 
 
 def _selected_attention(q, k, v, blocks, scale, causal, lengths, low):
+    results = ops._binding.selected_attention(q, k, v, blocks, scale, causal, lengths, low)
+    if results is not None:
+        return results
     q, k, v = _usable(q), _usable(k), _usable(v)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     out_low = torch.empty_like(out) if low else None
@@ -237,6 +246,9 @@ def _selected_attention(q, k, v, blocks, scale, causal, lengths, low):
 
 
 def _selected_attention_backward(q, k, v, blocks, out, out_low, lse, grad_out, scale, causal, lengths):
+    grads = ops._binding.selected_attention_backward(q, k, v, blocks, out, out_low, lse, grad_out, scale, causal, lengths)
+    if grads is not None:
+        return grads
     q, k, v, grad_out = _usable(q), _usable(k), _usable(v), _usable(grad_out)
     gq, gk, gv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
     ops.selected_attention_backward(q, k, v, blocks, out, lse, grad_out, gq, gk, gv, _scratch(ops.selected_attention_workspace(q, k, True), q.device), scale,
@@ -282,29 +294,65 @@ def selected_attention(q, k, v, blocks, scale, causal=True, lengths=None):
         out = selected_attention(q, k, v, blocks, D ** -0.5)
 
     lengths [B] int32: tokens of each entry of a padded batch (Lq == Lk).  See ops.selected_attention."""
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) and torch.autograd.forward_ad._current_level < 0:
+        with torch.no_grad():
+            return _through(_selected_attention, torch.ops.vsparse.selected_attention, (q, k, v, blocks), q, k, v, blocks, float(scale), bool(causal), lengths, False)[0]
     return SelectedAttention.apply(q, k, v, blocks, float(scale), bool(causal), lengths)
+
+
+_PARTS = "Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, Tensor k_sums, Tensor k_ring, Tensor v_ring"
+_LIB.define("cache_append(Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor(e!) k_sums, Tensor(f!) k_ring, Tensor(g!) v_ring, "
+            "Tensor k, Tensor v, Tensor table, Tensor tails, Tensor lengths, Tensor? counts) -> ()")
+_LIB.define(f"cache_select({_PARTS}, Tensor q, Tensor table, Tensor lengths, int count) -> Tensor")
+_LIB.define(f"cache_attention({_PARTS}, Tensor q, Tensor table, Tensor tails, Tensor lengths, float scale, Tensor? blocks) -> Tensor")
+
+
+def _cache_append(*args):
+    ops.cache_append(BlockCache(*args[:7]), _usable(args[7]), _usable(args[8]), *args[9:])
+
+
+def _cache_select(*args):
+    cache, (q, table, lengths, count) = BlockCache(*args[:7]), args[7:]
+    q = _usable(q)
+    blocks = torch.empty((q.shape[0], cache.kv_heads, count), dtype=torch.int32, device=q.device)
+    ops.cache_select(q, cache, table, lengths, blocks)
+    return blocks
+
+
+def _cache_attention(*args):
+    cache, (q, table, tails, lengths, scale, blocks) = BlockCache(*args[:7]), args[7:]
+    q = _usable(q)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ops.cache_attention(q, cache, table, tails, lengths, out, _scratch(ops.cache_attention_workspace(q, cache, table, blocks), q.device), scale, blocks)
+    return out
+
+
+for _name, _kernel in (("cache_append", _cache_append), ("cache_select", _cache_select), ("cache_attention", _cache_attention)):
+    _LIB.impl(_name, _kernel, "CUDA")
 
 
 def cache_append(cache, k, v, table, tails, lengths, counts=None):
     """Appends k, v [n, T, Hkv, D] to the cache behind lengths [n] (see ops.cache_append); advancing lengths is the caller's."""
+    if _quiet((k, v)) and ops._binding.cache_append(cache._parts, k, v, table, tails, lengths, counts) is not None:
+        return
     with torch.no_grad():
-        ops.cache_append(cache, _usable(k), _usable(v), table, tails, lengths, counts)
+        _through(_cache_append, torch.ops.vsparse.cache_append, (k, v), *cache._parts, k, v, table, tails, lengths, counts)
 
 
 def cache_select(q, cache, table, lengths, count):
     """[n, Hkv, count] int32: the complete blocks that the newest token of each sequence attends to (see ops.cache_select)."""
-    with torch.no_grad():
-        q = _usable(q)
-        blocks = torch.empty((q.shape[0], cache.kv_heads, count), dtype=torch.int32, device=q.device)
-        ops.cache_select(q, cache, table, lengths, blocks)
+    blocks = ops._binding.cache_select(cache._parts, q, table, lengths, count) if _quiet((q,)) else None
+    if blocks is not None:
         return blocks
+    with torch.no_grad():
+        return _through(_cache_select, torch.ops.vsparse.cache_select, (q,), *cache._parts, q, table, lengths, int(count))
 
 
 def cache_attention(q, cache, table, tails, lengths, scale, blocks=None):
     """Attention of the newest token of each sequence, q [n, Hq, D], over the cache: all of it, or the chosen blocks (see ops.cache_attention).  For inference: no
     gradient is recorded."""
-    with torch.no_grad():
-        q = _usable(q)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ops.cache_attention(q, cache, table, tails, lengths, out, _scratch(ops.cache_attention_workspace(q, cache, table, blocks), q.device), scale, blocks)
+    out = ops._binding.cache_attention(cache._parts, q, table, tails, lengths, float(scale), blocks) if _quiet((q,)) else None
+    if out is not None:
         return out
+    with torch.no_grad():
+        return _through(_cache_attention, torch.ops.vsparse.cache_attention, (q,), *cache._parts, q, table, tails, lengths, float(scale), blocks)
