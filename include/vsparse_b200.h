@@ -298,7 +298,7 @@ int vs_device_status(int clear, uint32_t *status);
  * vs_selected_attention_backward: gradients of q, k and v (all three written whole) for grad_out; the gradients of a head of keys are summed over its group,
  * in the same order in every call.  Both take a workspace of vs_selected_attention_workspace_bytes(..., backward).
  * ---------------------------------------------------------------------------------------------------- */
-int64_t vs_select_blocks_workspace_bytes(int batch, int keys, int kv_heads, int d);
+int64_t vs_select_blocks_workspace_bytes(int batch, int queries, int keys, int kv_heads, int d);
 int vs_select_blocks(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal,
                      const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const int32_t *lengths,
                      int32_t *lists, void *workspace, int64_t workspace_bytes, void *stream);

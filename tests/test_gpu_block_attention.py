@@ -180,9 +180,33 @@ def test_selection_of_padded_batches_ties_and_what_is_no_number():
                 assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), count, causal, lengths)), (causal, count)
 
 
+@pytest.mark.parametrize("count", [2, 5, 40, 127, 129, 200])
+def test_selection_of_scores_that_32_bits_cannot_tell_apart(count):
+    """Blocks whose scores differ in the last places of 64 bits, or not at all; queries of zeros; more candidates than are ranked again at once."""
+    q, k, _, _ = tensors(1, 70, 64 * 300, 2, 1, 64, torch.float16, 11)
+    base = k[:, :64].clone()
+    k[:, :64 * 290] = base.repeat(1, 290, 1, 1)                              # all alike
+    k[:, 64 * 100 + 3, 0, 0] += 2.0 ** -9                                    # but for one element of some
+    k[:, 64 * 150 + 3, 0, 1] -= 2.0 ** -9
+    k[:, 64 * 200 + 7, 0, 0] += 2.0 ** -9
+    q[:, 5], q[:, 60] = 0, 2.0 ** -24
+    k[:, 64 * 250:64 * 251] *= 2
+    for causal in (True, False):
+        got = torch_ops.select_blocks(q, k, count, causal).cpu().numpy()
+        assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), count, causal, None)), causal
+
+
+@pytest.mark.parametrize("scale", [1e-20, 1e-38, 1e15, 3e38])
+def test_selection_beyond_the_range_of_32_bits(scale):
+    q, k, _, _ = tensors(1, 40, 64 * 40, 4, 2, 64, torch.float32, 12)
+    q, k = (q * min(scale, 1e37)).bfloat16(), (k.clamp(-1, 1) * scale).bfloat16()
+    got = torch_ops.select_blocks(q, k, 6).cpu().numpy()
+    assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), 6, True, None))
+
+
 def test_many_blocks():
     """Lists over more blocks than one CTA keeps scores for 32, and for 8, queries of."""
-    for keys in (64 * 700 + 5, 64 * 4000):
+    for keys in (64 * 700 + 5, 64 * 1024, 64 * 1025, 64 * 4000):
         q, k, v, _ = tensors(1, 3, keys, 2, 1, 64, torch.float16, 2)
         got = torch_ops.select_blocks(q, k, 6)
         assert np.array_equal(got.cpu().numpy(), plain.select(plain.f64(q), plain.f64(k), 6, True, None))

@@ -45,7 +45,7 @@ SIGNATURES = {
     "vs_softmax_cvse_backward": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _f, _i, _i64, _vp]),
     "vs_attention_cvse_backward": (_i, [_i, _i, _i, _i, _i, _i] + [_vp] * 15 + [_f, _i, _vp]),
     "vs_attention_cvse_static": (_i, [_i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp]),
-    "vs_select_blocks_workspace_bytes": (_i64, [_i] * 4),
+    "vs_select_blocks_workspace_bytes": (_i64, [_i] * 5),
     "vs_select_blocks": (_i, [_i] * 9 + [_vp] * 7 + [_i64, _vp]),
     "vs_selected_attention_workspace_bytes": (_i64, [_i] * 7),
     "vs_selected_attention": (_i, [_i] * 9 + [_vp] * 11 + [_f, _vp, _i64, _vp]),

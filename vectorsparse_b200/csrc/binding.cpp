@@ -616,7 +616,7 @@ VS_FAST_CALL(select_blocks, 5) {
     if (!a.ok) Py_RETURN_NONE;
     On on(a.device);
     at::Tensor blocks = at::empty({z.batch, z.kv_heads, z.queries, count}, q->options().dtype(at::kInt));
-    const int64_t bytes = g_blocks.select_blocks_workspace(z.batch, z.keys, z.kv_heads, z.d);
+    const int64_t bytes = g_blocks.select_blocks_workspace(z.batch, z.queries, z.keys, z.kv_heads, z.d);
     at::Tensor ws = scratch(*q, bytes);
     const void *pq = q->const_data_ptr(), *pk = k->const_data_ptr();
     int32_t *pb = static_cast<int32_t *>(blocks.mutable_data_ptr());

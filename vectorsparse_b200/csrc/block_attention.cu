@@ -116,17 +116,55 @@ template <typename T, int QT> int launch_scores(const blocks::Shape &s, const bl
     blocks::score_kernel<T, QT><<<(unsigned)grid, blocks::kScoreThreads, smem, st>>>(s, q, means, lists);
     return (int)cudaGetLastError();
 }
-template <typename T> int select(const blocks::Shape &s, const blocks::Operand &q, const blocks::Operand &k, int32_t *lists, double *means, cudaStream_t st) {
+// The workspace of a choice: means in 64 and in 32 bits and the norms of the latter, then the scores of a slab and the norms of its queries.  Slabs of 48 MB stay in
+// L2 between the two kernels that share them.
+struct SelectSpace {
+    int64_t means, blocks, tiles, slab;   // elements of the means, blocks of keys, tiles of queries, tiles of a slab
+    bool fast;
+    int64_t bytes() const { return up256(means * 8) + up256(means * 4) + up256(blocks * 4) + slab * blocks::kFastQueries * 4 * (per_query + 1); }
+    int64_t per_query;
+    SelectSpace(int64_t pairs, int64_t queries, int64_t keys, int64_t d) {
+        per_query = (keys + blocks::kBlock - 1) / blocks::kBlock;
+        blocks = pairs * per_query;
+        means = blocks * d;
+        tiles = pairs * ((queries + blocks::kFastQueries - 1) / blocks::kFastQueries);
+        fast = per_query > 0 && per_query <= blocks::kFastMost;
+        slab = fast ? std::max<int64_t>(1, std::min(tiles, (int64_t(48) << 20) / (blocks::kFastQueries * 4 * per_query))) : 0;
+    }
+};
+template <typename T> int select(const blocks::Shape &s, const blocks::Operand &q, const blocks::Operand &k, int32_t *lists, void *workspace, cudaStream_t st) {
+    const SelectSpace space((int64_t)s.batch * s.kv_heads, s.queries, s.keys, s.d);
+    char *at = static_cast<char *>(workspace);
+    double *means = reinterpret_cast<double *>(at);
+    float *means32 = reinterpret_cast<float *>(at += up256(space.means * 8)), *norms = reinterpret_cast<float *>(at += up256(space.means * 4));
     if (s.blocks > 0) {
-        blocks::means_kernel<T><<<(unsigned)((int64_t)s.batch * s.kv_heads * s.blocks), blocks::kMeanThreads, 0, st>>>(s, k, means);
+        blocks::means_kernel<T><<<(unsigned)space.blocks, blocks::kMeanThreads, 0, st>>>(s, k, means, means32, norms);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return (int)e;
+    }
+    if (space.fast && s.count <= blocks::kFastCount) {
+        const int smem = blocks::fast_bytes(s.d);
+        const int rc = allow_smem<blocks::fast_score_kernel<T>>(smem);
+        if (rc != VS_OK) return rc;
+        blocks::Slab slab;
+        slab.scores = reinterpret_cast<float *>(at + up256(space.blocks * 4));
+        slab.norms = slab.scores + space.slab * blocks::kFastQueries * s.blocks;
+        for (slab.first = 0; slab.first < space.tiles; slab.first += space.slab) {
+            slab.tiles = std::min(space.slab, space.tiles - slab.first);
+            cudaError_t e = launch_behind(blocks::fast_score_kernel<T>, (unsigned)slab.tiles, blocks::kFastThreads, smem, st, s, q, (const float *)means32, slab);
+            if (e == cudaSuccess)
+                e = launch_behind(blocks::fast_rank_kernel<T>, (unsigned)(slab.tiles * blocks::kFastQueries / (blocks::kFastThreads / 32)), blocks::kFastThreads, 0, st, s, q,
+                                  (const double *)means, (const float *)norms, slab, lists);
+            if (e != cudaSuccess) return (int)e;
+        }
+        return VS_OK;
     }
     // as many queries to a CTA as their scores leave room for
     if (blocks::score_bytes<32>(s.blocks, s.d) <= kMaxSmem) return launch_scores<T, 32>(s, q, means, lists, st);
     if (blocks::score_bytes<8>(s.blocks, s.d) <= kMaxSmem) return launch_scores<T, 8>(s, q, means, lists, st);
     return launch_scores<T, 1>(s, q, means, lists, st);
 }
+static_assert(2 * (blocks::fast_bytes(blocks::kMaxD) + 1024) <= 228 * 1024, "two CTAs an SM");
 static_assert(blocks::score_bytes<1>(blocks::kMaxBlocks, blocks::kMaxD) <= kMaxSmem, "scores of one query");
 
 int make_bits(const blocks::Shape &s, const int32_t *lists, uint32_t *bits, uint32_t *zero, cudaStream_t st) {
@@ -224,9 +262,9 @@ inline bool scale_ok(float scale) { return scale > 0.f && std::isfinite(scale); 
 
 }  // namespace
 
-VS_EXPORT int64_t vs_select_blocks_workspace_bytes(int batch, int keys, int kv_heads, int d) {
-    if (batch < 1 || keys < 1 || kv_heads < 1 || d < 1) return 0;
-    return up256((int64_t)batch * kv_heads * ((keys + blocks::kBlock - 1) / blocks::kBlock) * d * 8);
+VS_EXPORT int64_t vs_select_blocks_workspace_bytes(int batch, int queries, int keys, int kv_heads, int d) {
+    if (batch < 1 || queries < 1 || keys < 1 || kv_heads < 1 || d < 1) return 0;
+    return SelectSpace((int64_t)batch * kv_heads, queries, keys, d).bytes();
 }
 
 VS_EXPORT int vs_select_blocks(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const void *q,
@@ -241,10 +279,9 @@ VS_EXPORT int vs_select_blocks(int dtype, int batch, int queries, int keys, int 
     if (keys > 0 && (rc = operand(ok, k, k_strides, batch, keys, kv_heads)) != VS_OK) return rc;
     if (!lists || (keys > 0 && !workspace)) return VS_ERR_NULL;
     if (!aligned16(workspace) || !aligned4(lists)) return VS_ERR_ALIGN;
-    if (workspace_bytes < vs_select_blocks_workspace_bytes(batch, keys, kv_heads, d)) return VS_ERR_SHAPE;
+    if (workspace_bytes < vs_select_blocks_workspace_bytes(batch, queries, keys, kv_heads, d)) return VS_ERR_SHAPE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    double *means = static_cast<double *>(workspace);
-    return dtype == VS_F16 ? select<__half>(s, oq, ok, lists, means, st) : select<__nv_bfloat16>(s, oq, ok, lists, means, st);
+    return dtype == VS_F16 ? select<__half>(s, oq, ok, lists, workspace, st) : select<__nv_bfloat16>(s, oq, ok, lists, workspace, st);
 }
 
 VS_EXPORT int64_t vs_selected_attention_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int d, int backward) {

@@ -57,6 +57,15 @@ template <typename T> __device__ __forceinline__ void load8(const T *p, float (&
     for (int i = 0; i < 8; ++i) f[i] = to_f32(h[i]);
 }
 
+// Two fused multiply-adds: one instruction on this part.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
 // ---- lists as bits ------------------------------------------------------------------------------------------------
 // One CTA takes a word of 32 queries: it collects their bits in shared memory and writes the word's row for all blocks, so that nothing has to
 // be cleared beforehand.  Bound by the reading of the lists.
@@ -88,10 +97,13 @@ __global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const
 // ---- choosing -----------------------------------------------------------------------------------------------------
 // Score of block j for query i: (sum of the group's query heads) . (mean of the block's keys), everything in 64 bits: its order decides whole
 // numbers, and 32-bit sums in two orders disagree about blocks that are close.
-// Means: one CTA per (b, kv head, block), 8 dimensions to a thread, the tokens shared by groups of threads.
+// Means: one CTA per (b, kv head, block), 8 dimensions to a thread, the tokens shared by groups of threads; in 64 bits, and in 32 with a bound on their norm.
 constexpr int kMeanThreads = 128;
-template <typename T> __global__ void __launch_bounds__(kMeanThreads) means_kernel(const Shape s, const Operand k, double *means) {
+template <typename T> __global__ void __launch_bounds__(kMeanThreads) means_kernel(const Shape s, const Operand k, double *means, float *means32, float *norms) {
     __shared__ double part[kMeanThreads * 8];
+    __shared__ float squares;
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) squares = 0.f;
     const int64_t at = blockIdx.x;
     const int j = (int)(at % s.blocks), h = (int)(at / s.blocks % s.kv_heads), b = (int)(at / s.blocks / s.kv_heads);
     const int first = j * kBlock, n = min(kBlock, s.length(b) - first);
@@ -112,8 +124,14 @@ template <typename T> __global__ void __launch_bounds__(kMeanThreads) means_kern
     for (int x = threadIdx.x; x < s.d; x += kMeanThreads) {
         double total = 0;
         for (int y = 0; y < groups; ++y) total += part[y * s.d + x];
-        means[at * s.d + x] = n > 0 ? total / n : 0.0;
+        total = n > 0 ? total / n : 0.0;
+        means[at * s.d + x] = total;
+        const float rounded = (float)total;
+        means32[at * s.d + x] = rounded;
+        atomicAdd(&squares, rounded * rounded);   // a bound, with room for the order of its sum
     }
+    __syncthreads();
+    if (threadIdx.x == 0) norms[at] = sqrtf(squares) * 1.001f;
 }
 
 // Scores as whole numbers of the same order, above 0; what is no number counts as the lowest score.
@@ -167,6 +185,294 @@ __device__ __forceinline__ void write_list(const uint32_t *taken, int words, int
     for (int x = done + lane; x < count; x += 32) list[x] = -1;
 }
 
+// Most lists need no more than 32 bits: fp32 scores are off by E at most, and where the last block taken and the first left lie further apart than 2 E, the
+// choice is that of 64 bits.  Where they do not, the scores from 2 E below the last one on are computed again in 64.
+// Two kernels, over slabs of queries whose scores stay in L2: a product of the queries' sums with the means, and a ranking by a warp per query, which needs many warps
+// to cover what it waits for and would not have them beside the product's tiles (in one kernel, with 16 warps an SM: 212 us at 16384 x 16384, 4 heads of keys,
+// d = 128; fp64 throughout, as below: 525).
+constexpr int kFastThreads = 256, kFastQueries = 64, kFastBlocks = 128, kFastPiece = 64, kFastPitch = kFastPiece + 4, kMembers = 256, kFastCount = 128;
+constexpr int kFastMost = 1024;   // blocks of a sequence
+__host__ __device__ constexpr int fast_pitch(int d) { return (d + 63) / 64 * 64 + 4; }
+constexpr int fast_bytes(int d) { return (kFastQueries * fast_pitch(d) + kFastBlocks * kFastPitch) * 4; }
+struct Slab {   // tiles of kFastQueries queries of a head of keys, from `first` on
+    int64_t first, tiles;
+    float *scores;   // [tiles][kFastQueries][blocks]
+    float *norms;    // [tiles][kFastQueries]: of the queries' sums
+};
+struct FastTile {
+    int b, h, i0, most;   // most: candidates of any query of the tile
+    int64_t bh;
+    __device__ __forceinline__ FastTile(const Shape &s, int64_t tile) {   // in 32 bits: every launch has fewer tiles
+        const uint32_t tiles = (s.queries + kFastQueries - 1) / kFastQueries, pair = (uint32_t)tile / tiles;
+        bh = pair;
+        i0 = (int)((uint32_t)tile - pair * tiles) * kFastQueries;
+        b = (int)(pair / (uint32_t)s.kv_heads);
+        h = (int)(pair - (uint32_t)b * s.kv_heads);
+        const int last = min(i0 + kFastQueries, s.rows(b)) - 1;
+        most = last < i0 ? 0 : s.causal ? s.position(last) / kBlock : (s.length(b) + kBlock - 1) / kBlock;
+    }
+};
+struct Members {   // of one warp: the query in 64 bits, the blocks to be ranked again, and which of all are taken
+    double q[kMaxD];
+    uint64_t keys[kMembers];
+    int16_t index[kMembers];
+    uint32_t taken[kMembers / 32];
+    uint32_t all[kFastMost / 32];
+};
+
+__device__ __forceinline__ uint32_t sortable32(float x) {
+    const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unsortable32(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
+
+// One query's `want` best of n candidates into `taken`, in 64 bits: those with fp32 scores from `from` on, or all.
+template <typename T> __device__ __forceinline__ void take_exactly(const Shape &s, const T *q, int64_t q_head, const double *means, const float *scores, float from, bool all, int n,
+                                                                   int want, uint32_t *taken, Members &m) {
+    const int lane = threadIdx.x & 31;
+    for (int x = lane; x < s.d; x += 32) {
+        double sum = 0;
+        for (int g = 0; g < s.group; ++g) sum += to_f32(q[g * q_head + x]);
+        m.q[x] = sum;
+    }
+    __syncwarp();
+    auto exact = [&](int j) {
+        double dot = 0;
+        const double *p = means + (int64_t)j * s.d;
+        for (int x = 0; x < s.d; ++x) dot = fma(m.q[x], p[x], dot);
+        return sortable(dot);
+    };
+    int count = 0;
+    for (int base = 0; base < n; base += 32) {
+        const bool mine = base + lane < n && (all || !(scores[base + lane] < from));
+        const uint32_t some = __ballot_sync(~0u, mine);
+        const int at = count + __popc(some & ((1u << lane) - 1));
+        if (mine && at < kMembers) m.index[at] = (int16_t)(base + lane);
+        count += __popc(some);
+    }
+    if (count <= kMembers) {
+        for (int x = lane; x < kMembers / 32; x += 32) m.taken[x] = 0;
+        __syncwarp();
+        for (int x = lane; x < count; x += 32) m.keys[x] = exact(m.index[x]);
+        __syncwarp();
+        take_best(m.keys, count, want, m.taken);
+        __syncwarp();
+        for (int x = lane; x < count; x += 32)
+            if (m.taken[x / 32] >> (x % 32) & 1u) atomicOr(taken + m.index[x] / 32, 1u << (m.index[x] % 32));
+    } else {   // scores that are all alike: one block after another
+        for (int x = 0; x < want; ++x) {
+            uint64_t best = 0;
+            int at = 0x7fffffff;
+            for (int j = lane; j < n; j += 32) {
+                if (taken[j / 32] >> (j % 32) & 1u) continue;
+                const uint64_t key = exact(j);
+                if (key > best) { best = key; at = j; }
+            }
+            const uint32_t hi = (uint32_t)(best >> 32), top = __reduce_max_sync(~0u, hi), lo = hi == top ? (uint32_t)best : 0u, low = __reduce_max_sync(~0u, lo);
+            if (!(top | low)) break;
+            const int winner = __reduce_min_sync(~0u, hi == top && lo == low ? at : 0x7fffffff);
+            if (lane == 0) taken[winner / 32] |= 1u << (winner % 32);
+            __syncwarp();
+        }
+    }
+    __syncwarp();
+}
+
+// Scores of a tile: 64 queries against all candidates of any of them, 128 blocks and 64 dimensions at a time, 4 x 8 to a thread.
+template <typename T> __global__ void __launch_bounds__(kFastThreads, 2) fast_score_kernel(const Shape s, const Operand q, const float *means32, const Slab slab) {
+    extern __shared__ __align__(16) float fsm[];
+    const int pitch = fast_pitch(s.d), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    float *sums = fsm, *piece = sums + kFastQueries * pitch;
+    pdl_launch_dependents();
+    const int64_t index = slab.tiles - 1 - blockIdx.x;   // the last queries have most candidates: they go first
+    const FastTile t(s, slab.first + index);
+    if (t.most == 0) {
+        pdl_wait();   // as every CTA: the kernels behind take the end of this one for the end of all before it
+        return;
+    }
+    const int rows = s.rows(t.b), chunks = fast_pitch(s.d) / 8;   // of 8 dimensions, zeros behind the last
+    const T *qp = static_cast<const T *>(q.at) + t.b * q.batch + t.h * s.group * q.head;
+    for (int x = tid; x < kFastQueries * chunks; x += kFastThreads) {
+        const int i = x / chunks, c = x % chunks * 8;
+        float sum[8] = {};
+        if (t.i0 + i < rows && c < s.d) {
+#pragma unroll 8
+            for (int g = 0; g < s.group; ++g) {
+                float f[8];
+                load8(qp + (t.i0 + i) * q.token + g * q.head + c, f);
+#pragma unroll
+                for (int y = 0; y < 8; ++y) sum[y] += f[y];
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < 8; y += 4) *reinterpret_cast<float4 *>(sums + i * pitch + c + y) = make_float4(sum[y], sum[y + 1], sum[y + 2], sum[y + 3]);
+    }
+    __syncthreads();
+    static_assert(kFastThreads == 4 * kFastQueries, "four threads to a query's norm");
+    {
+        const float *p = sums + tid / 4 * pitch;
+        float square = 0.f;
+        for (int x = tid % 4; x < s.d; x += 4) square = fmaf(p[x], p[x], square);
+#pragma unroll
+        for (int o = 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+        pdl_wait();   // the means are the kernel's before, and whoever reads the last slab is done
+        if (tid % 4 == 0) slab.norms[index * kFastQueries + tid / 4] = sqrtf(square) * 1.001f;
+    }
+    // queries 4 ty .. 4 ty + 3, blocks tx + 16 x
+    const int tx = lane % 16, ty = warp * 2 + lane / 16;
+    float *out = slab.scores + index * kFastQueries * s.blocks;
+    auto product = [&](auto blocks_each, int base) {
+        constexpr int kEach = decltype(blocks_each)::value;   // blocks of a thread
+        const int width = min(16 * kEach, t.most - base);
+        float2 acc[4][kEach];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) acc[r][x] = make_float2(0.f, 0.f);
+        for (int d0 = 0; d0 < s.d; d0 += kFastPiece) {
+            __syncthreads();
+            for (int x = tid; x < 16 * kEach * (kFastPiece / 4); x += kFastThreads) {
+                const int j = x / (kFastPiece / 4), y = x % (kFastPiece / 4) * 4;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (j < width && d0 + y < s.d) v = __ldcg(reinterpret_cast<const float4 *>(means32 + (t.bh * s.blocks + base + j) * s.d + d0 + y));
+                *reinterpret_cast<float4 *>(piece + j * kFastPitch + y) = v;
+            }
+            __syncthreads();
+#pragma unroll 2
+            for (int y = 0; y < kFastPiece; y += 4) {
+                float4 v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const float4 *>(sums + (ty * 4 + r) * pitch + d0 + y);
+#pragma unroll
+                for (int x = 0; x < kEach; ++x) {
+                    const float4 a = *reinterpret_cast<const float4 *>(piece + (tx + 16 * x) * kFastPitch + y);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        acc[r][x] = fma2(make_float2(v[r].x, v[r].y), make_float2(a.x, a.y), acc[r][x]);
+                        acc[r][x] = fma2(make_float2(v[r].z, v[r].w), make_float2(a.z, a.w), acc[r][x]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int x = 0; x < kEach; ++x)
+                if (tx + 16 * x < width) out[(int64_t)(ty * 4 + r) * s.blocks + base + tx + 16 * x] = acc[r][x].x + acc[r][x].y;
+    };
+    for (int base = 0; base < t.most;) {
+        const int left = t.most - base;
+        if (left > 64) product(std::integral_constant<int, 8>(), base), base += 128;
+        else if (left > 32) product(std::integral_constant<int, 4>(), base), base += 64;
+        else product(std::integral_constant<int, 2>(), base), base += 32;
+    }
+}
+
+// The list of one query from its n > want > 0 candidates' scores.  A lane holds kHeld of them in registers; more are read each time.
+template <typename T, int kHeld> __device__ __forceinline__ void rank_row(const Shape &s, const FastTile &t, const Operand &q, int i, int own, int n, int want, const float *row,
+                                                                          const float *query_norm, const double *means, const float *mean_norms, int32_t *list, Members &m) {
+    const int lane = threadIdx.x & 31;
+    float v[kHeld], top = -FLT_MAX, low = FLT_MAX, norm = 0.f;
+    bool number = true;
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) v[x] = lane + 32 * x < n ? __ldcg(row + lane + 32 * x) : -INFINITY;   // below every threshold
+    for (int j = lane; j < n; j += 32) {
+        const float m = __ldcg(mean_norms + t.bh * s.blocks + j);
+        norm = m <= FLT_MAX ? fmaxf(norm, m) : INFINITY;
+        number &= m <= FLT_MAX;
+    }
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x)
+        if (lane + 32 * x < n) {
+            number &= fabsf(v[x]) <= FLT_MAX;
+            top = fmaxf(top, v[x]);
+            low = fminf(low, v[x]);
+        }
+    for (int j = lane + 32 * kHeld; j < n; j += 32) {
+        const float f = __ldcg(row + j);
+        number &= fabsf(f) <= FLT_MAX;
+        top = fmaxf(top, f);
+        low = fminf(low, f);
+    }
+    float hi = unsortable32(__reduce_max_sync(~0u, sortable32(top))), lo = unsortable32(__reduce_min_sync(~0u, sortable32(low))), at = 0.5f * hi + 0.5f * lo;
+    // one rounding for each of the d terms of a sum, the group's, and those of the operands; what is denormal besides
+    const float off = (float)(s.d + s.group + 8) * 0x1p-24f * __ldcg(query_norm) * __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(norm))) * 1.01f + 0x1p-120f;
+    const bool usable = __all_sync(~0u, number) && off <= FLT_MAX;
+    bool found = false;
+    int reach_lo = n, reach_hi = 1;   // how many reach lo: more than `want`; and hi: fewer, or, at first, perhaps as many
+    for (int step = 1; usable && step < 32; ++step) {
+        if (!(at > lo && at < hi)) break;   // nothing between: scores that are alike
+        int count = 0;
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x) count += v[x] >= at;
+        for (int j = lane + 32 * kHeld; j < n; j += 32) count += __ldcg(row + j) >= at;
+        count = __reduce_add_sync(~0u, count);
+        if (count == want) {
+            found = true;
+            break;
+        }
+        if (count > want) lo = at, reach_lo = count;
+        else hi = at, reach_hi = count;
+        // as if the scores between lay evenly; every third step halves, whatever they do
+        const float part = step % 3 == 0 ? 0.5f : fminf(fmaxf(__fdividef(reach_lo - want - 0.5f, (float)max(1, reach_lo - reach_hi)), 0.05f), 0.95f);
+        at = lo + (hi - lo) * part;
+    }
+    bool near = !found;
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) near |= fabsf(v[x] - at) <= off;
+    for (int j = lane + 32 * kHeld; j < n; j += 32) near |= fabsf(__ldcg(row + j) - at) <= off;
+    if (__any_sync(~0u, near)) {
+        const int words = (s.blocks + 31) / 32;
+        for (int x = lane; x < words; x += 32) m.all[x] = own >= 0 && own / 32 == x ? 1u << (own & 31) : 0u;
+        __syncwarp();
+        take_exactly(s, static_cast<const T *>(q.at) + t.b * q.batch + t.h * s.group * q.head + i * q.token, q.head, means + t.bh * s.blocks * s.d, row,
+                     (found ? at : lo) - 2.f * off, !usable, n, want, m.all, m);
+        write_list(m.all, words, s.count, list);
+        return;
+    }
+    int before = 0;
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) {
+        const bool mine = v[x] >= at;
+        const uint32_t all = __ballot_sync(~0u, mine);
+        if (mine) list[before + __popc(all & ((1u << lane) - 1))] = lane + 32 * x;
+        before += __popc(all);
+    }
+    for (int base = 32 * kHeld; base < n; base += 32) {
+        const bool mine = base + lane < n && __ldcg(row + base + lane) >= at;
+        const uint32_t all = __ballot_sync(~0u, mine);
+        if (mine) list[before + __popc(all & ((1u << lane) - 1))] = base + lane;
+        before += __popc(all);
+    }
+    if (own >= 0 && lane == 0) list[s.count - 1] = own;
+}
+// The lists of a slab, a warp to a query: it narrows the interval between two scores until just as many reach a value as are wanted, a step being a comparison for each
+// score of a lane and one sum over the warp (taking the best one after another costs several times that for each).
+template <typename T> __global__ void __launch_bounds__(kFastThreads) fast_rank_kernel(const Shape s, const Operand q, const double *means, const float *mean_norms, const Slab slab,
+                                                                                      int32_t *lists) {
+    __shared__ Members members_all[kFastThreads / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    const int64_t row_index = slab.tiles * kFastQueries - 1 - ((int64_t)blockIdx.x * (kFastThreads / 32) + warp);   // as the scores were made
+    const FastTile t(s, slab.first + (row_index >> 6));
+    const int i = t.i0 + (int)(row_index & 63);
+    static_assert(kFastQueries == 64, "shifts");
+    pdl_wait();
+    if (i >= s.queries) return;
+    const int rows = s.rows(t.b), own = s.causal ? s.position(i) / kBlock : -1, n = i >= rows ? 0 : s.causal ? own : t.most, want = s.count - (own >= 0);
+    int32_t *list = lists + (t.bh * s.queries + i) * s.count;
+    if (n <= want || want == 0) {   // all candidates, or none
+        const int all = i >= rows ? 0 : want > 0 ? n + (own >= 0) : 0;   // the query's own block follows its candidates
+        for (int x = lane; x < s.count; x += 32) list[x] = x < all ? x : want == 0 && i < rows && x == 0 ? own : -1;
+        return;
+    }
+    const float *row = slab.scores + row_index * s.blocks, *query_norm = slab.norms + row_index;
+    if (n <= 64) rank_row<T, 2>(s, t, q, i, own, n, want, row, query_norm, means, mean_norms, list, members_all[warp]);
+    else if (n <= 128) rank_row<T, 4>(s, t, q, i, own, n, want, row, query_norm, means, mean_norms, list, members_all[warp]);
+    else rank_row<T, 8>(s, t, q, i, own, n, want, row, query_norm, means, mean_norms, list, members_all[warp]);
+}
+
+// 64 bits throughout, for lists and sequences that the kernel above has no room for.
 // One CTA scores QT queries of one head of keys against all their candidates, 64 blocks and 32 dimensions at a time, and each of its warps
 // then takes the best of one query after another.  Shared memory: the queries' sums, a piece of the means, the scores.
 constexpr int kScoreThreads = 256, kPiece = 32;

@@ -455,7 +455,7 @@ def select_blocks(q, k, blocks, workspace, causal=True, lengths=None):
 
 
 def select_blocks_workspace(q, k) -> int:
-    return _lib.lib().vs_select_blocks_workspace_bytes(k.shape[0], k.shape[1], k.shape[2], k.shape[3])
+    return _lib.lib().vs_select_blocks_workspace_bytes(q.shape[0], q.shape[1], *k.shape[1:])
 
 
 def selected_attention_workspace(q, k, backward=False) -> int:
