@@ -317,7 +317,7 @@ int vs_selected_attention_backward(int dtype, int batch, int queries, int keys, 
  * The same for single tokens, over a cache whose complete blocks are held in 8 bits.  No counterpart in the reference.
  *
  *   k_codes, v_codes    int8  [pages][kv_heads][64][d]    a block of a sequence is a page
- *   k_scales, v_scales  float [pages][kv_heads]           value = code * scale
+ *   k_scales, v_scales  float [pages][kv_heads]           value = code * scale; not negative
  *   k_sums              int16 [pages][kv_heads][d]        sum of the codes of a block of keys
  *   k_ring, v_ring      dtype [tails][kv_heads][128][d]   the newest tokens in 16 bits: token t of a sequence at t % 128, for the tokens
  *                                                         of its newest complete block and of the block behind it

@@ -43,10 +43,36 @@ struct Sequences {
     }
 };
 
+// Two 16-bit elements in a word.
+template <typename T> struct Two;
+template <> struct Two<__half> {
+    static __device__ __forceinline__ uint32_t most(uint32_t x, uint32_t y) {   // magnitudes; what is no number stays
+        const __half2 m = __hmax2_nan(__habs2(*reinterpret_cast<const __half2 *>(&x)), __habs2(*reinterpret_cast<const __half2 *>(&y)));
+        return *reinterpret_cast<const uint32_t *>(&m);
+    }
+    static __device__ __forceinline__ float2 floats(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+    static __device__ __forceinline__ float larger(uint32_t x) {
+        const float2 f = floats(x);
+        return __uint_as_float(max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    }
+};
+template <> struct Two<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t most(uint32_t x, uint32_t y) {
+        const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162 *>(&x)), __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&y)));
+        return *reinterpret_cast<const uint32_t *>(&m);
+    }
+    static __device__ __forceinline__ float2 floats(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
+    static __device__ __forceinline__ float larger(uint32_t x) {
+        const float2 f = floats(x);
+        return __uint_as_float(max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    }
+};
+
 // ---- appending ------------------------------------------------------------------------------------------------------
-// One CTA takes one block of one sequence and head, keys or values: a block that becomes complete is gathered from ring and new tokens, reduced
-// and rounded out of registers.  The CTA of a sequence's first block alone writes the ring, after it has read it.
-constexpr int kAppendThreads = 256;
+// One CTA takes one block of one sequence and head, keys or values: a block that becomes complete is gathered from ring and new tokens by asynchronous copies, reduced
+// and rounded out of shared memory.  A CTA is a chain of waits, so what counts is how many of them an SM holds: 12 with 16 KB each (with the block in
+// registers of 256 threads 5, and 40 us for 13 000 tokens of 8 heads, d = 128).  The CTA of a sequence's first block alone writes the ring, after it has read it.
+constexpr int kAppendThreads = 128;
 struct AppendArgs {
     Pages c;
     Sequences s;
@@ -55,71 +81,115 @@ struct AppendArgs {
     const void *at[2];        // new keys and values [count][tokens][kv heads][d]
     int64_t batch[2], token[2], head[2];
 };
-template <typename T> __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
-    __shared__ float most[kAppendThreads / 32];
-    __shared__ int part[kAppendThreads * 8];   // [groups of tokens][d]
+template <typename T> __global__ void __launch_bounds__(kAppendThreads, 12) append_kernel(const AppendArgs a) {
+    __shared__ uint32_t most[kAppendThreads / 32];
+    extern __shared__ __align__(16) uint4 tile[];   // [64][d / 8]
+    int16_t *part = reinterpret_cast<int16_t *>(tile);   // [groups of tokens][d], once the block has been rounded
     const int kv = blockIdx.y, tid = threadIdx.x;
-    const int64_t at = blockIdx.x;
-    const int x = (int)(at % a.touched), h = (int)(at / a.touched % a.c.kv_heads), r = (int)(at / a.touched / a.c.kv_heads);
-    const int before = max(a.s.lengths[r], 0), fresh = a.counts ? min(max(a.counts[r], 0), a.tokens) : a.tokens;
+    // neighbouring CTAs take the heads of one block, whose tokens lie side by side
+    const uint32_t block = blockIdx.x / (uint32_t)a.c.kv_heads;
+    const int h = (int)(blockIdx.x - block * a.c.kv_heads), r = (int)(block / (uint32_t)a.touched), x = (int)(block - (uint32_t)r * a.touched);
+    const int before = max(a.s.lengths[r], 0), fresh = a.counts ? min(max(a.counts[r], 0), a.tokens) : a.tokens, tail = a.s.tails[r];
     const int total = min(before, 0x7fffffff - fresh) + fresh, j = before / kBlock + x;
-    const int tail = a.s.tails[r], d = a.c.d;
+    const int d = a.c.d;
     if (tail < 0 || tail >= a.c.tails || fresh == 0) return;
     T *ring = static_cast<T *>(a.c.rings[kv]) + ((int64_t)tail * a.c.kv_heads + h) * kRing * d;
     const T *news = static_cast<const T *>(a.at[kv]) + r * a.batch[kv] + h * a.head[kv];
     const int chunks = d / 8, groups = kAppendThreads / chunks, c = tid % chunks, g = tid / chunks;   // 8 dimensions to a thread
-    const int page = total / kBlock > j ? a.s.page(r, j, a.c.pages) : -1;   // the same for all threads
-    if (page >= 0) {
-        constexpr int kPer = 4;   // tokens of a thread
-        static_assert(kBlock * (blocks::kMaxD / 8) <= kPer * kAppendThreads, "threads for a block");
-        float f[kPer][8];
-        float top = 0.f;
-#pragma unroll
-        for (int y = 0; y < kPer; ++y) {
-            const int o = g + y * groups, t = j * kBlock + o;
-            const bool here = g < groups && o < kBlock;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[y][e] = 0.f;
-            if (here) load8(t < before ? ring + (int64_t)(t % kRing) * d + c * 8 : news + (int64_t)(t - before) * a.token[kv] + c * 8, f[y]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float m = fabsf(f[y][e]);
-                if (m <= 3.402823466e38f) top = fmaxf(top, m);   // what is not finite does not set the scale
-            }
+    if (total / kBlock > j) {   // the same for all threads
+        const uint32_t tile_at = tc::smem_u32(tile);
+        for (int o = g; o < kBlock && g < groups; o += groups) {
+            const int t = j * kBlock + o;
+            tc::cp_async_16(tile_at + (o * chunks + c) * 16,
+                            t < before ? ring + (int64_t)(t % kRing) * d + c * 8 : news + (int64_t)(t - before) * a.token[kv] + c * 8, 16);
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        if (tid % 32 == 0) most[tid / 32] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kAppendThreads / 32; ++w) top = fmaxf(top, most[w]);
-        const float scale = top * (1.f / 127.f);
-        int8_t *codes = a.c.codes[kv] + ((int64_t)page * a.c.kv_heads + h) * kBlock * d;
-        int sum[8] = {};
-#pragma unroll
-        for (int y = 0; y < kPer; ++y) {
-            const int o = g + y * groups;
-            if (g >= groups || o >= kBlock) continue;
-            uint32_t word[2] = {};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float q = scale > 0.f ? rintf(__fdiv_rn(f[y][e], scale)) : 0.f;
-                const int code = q == q ? (int)fminf(fmaxf(q, -127.f), 127.f) : 0;
-                sum[e] += code;
-                word[e / 4] |= (uint32_t)(code & 255) << (e % 4 * 8);
-            }
-            *reinterpret_cast<uint2 *>(codes + (int64_t)o * d + c * 8) = make_uint2(word[0], word[1]);
-        }
-        if (tid == 0) a.c.scales[kv][(int64_t)page * a.c.kv_heads + h] = scale;
-        if (kv == 0) {
-            if (g < groups)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) part[g * d + c * 8 + e] = sum[e];
+        tc::cp_async_commit();
+        const int page = a.s.page(r, j, a.c.pages);
+        auto block_max = [&](float mine) {   // of magnitudes; what is no number counts as the largest
+            const uint32_t bits = __reduce_max_sync(~0u, __float_as_uint(mine) & 0x7fffffffu);
+            if (tid % 32 == 0) most[tid / 32] = bits;
             __syncthreads();
-            for (int e = tid; e < d; e += kAppendThreads) {
-                int all = 0;
-                for (int y = 0; y < groups; ++y) all += part[y * d + e];
-                a.c.sums[((int64_t)page * a.c.kv_heads + h) * d + e] = (int16_t)all;
+            uint32_t all = 0;
+#pragma unroll
+            for (int w = 0; w < kAppendThreads / 32; ++w) all = max(all, most[w]);
+            return all;
+        };
+        tc::cp_async_wait<0>();   // a thread reads what it has copied itself
+        uint32_t high = 0;
+        for (int o = g; o < kBlock && g < groups; o += groups) {
+            const uint4 v = tile[o * chunks + c];
+            high = Two<T>::most(high, Two<T>::most(Two<T>::most(v.x, v.y), Two<T>::most(v.z, v.w)));
+        }
+        uint32_t top = block_max(Two<T>::larger(high));
+        const bool odd = top >= 0x7f800000u;   // something is not finite: it does not set the scale
+        if (odd) {
+            float mine = 0.f;
+            for (int x4 = tid; x4 < kBlock * chunks * 4; x4 += kAppendThreads) {
+                const float2 f = Two<T>::floats(reinterpret_cast<const uint32_t *>(tile)[x4]);
+                if (fabsf(f.x) <= 3.402823466e38f) mine = fmaxf(mine, fabsf(f.x));
+                if (fabsf(f.y) <= 3.402823466e38f) mine = fmaxf(mine, fabsf(f.y));
+            }
+            __syncthreads();   // (copies of all threads have been here since the barrier in the first maximum)
+            top = block_max(mine);
+        }
+        if (page >= 0) {
+            const float scale = __uint_as_float(top) * (1.f / 127.f);
+            int8_t *codes = a.c.codes[kv] + ((int64_t)page * a.c.kv_heads + h) * kBlock * d;
+            // x / scale correctly rounded decides the code, but only next to a half does it matter: elsewhere x times the reciprocal rounds the same way.  Adding
+            // 1.5 * 2^23 rounds to a whole number whose low byte is the code.  Two elements to an instruction: this is what bounds a long prompt.
+            constexpr float kWhole = 12582912.f;
+            const bool exactly = odd || !(scale > 1e-30f);   // the reciprocal's own range
+            const float inverse = exactly ? 0.f : 1.f / scale;
+            uint32_t sum[8] = {};
+            int count = 0;
+#pragma unroll 2
+            for (int o = g; o < kBlock && g < groups; o += groups) {
+                const uint4 v = tile[o * chunks + c];
+                const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+                uint32_t code[8];
+                float off = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 q = blocks::fma2(Two<T>::floats(in[e]), make_float2(inverse, inverse), make_float2(0.f, 0.f));
+                    const float2 whole = blocks::fma2(q, make_float2(1.f, 1.f), make_float2(kWhole, kWhole));
+                    const float2 rest = blocks::fma2(blocks::fma2(whole, make_float2(1.f, 1.f), make_float2(-kWhole, -kWhole)), make_float2(-1.f, -1.f), q);
+                    off = fmaxf(off, fmaxf(fabsf(rest.x), fabsf(rest.y)));
+                    code[2 * e] = __float_as_uint(whole.x);
+                    code[2 * e + 1] = __float_as_uint(whole.y);
+                }
+                if (exactly || off >= 0.4999f)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = Two<T>::floats(in[e]);
+                        const float q[2] = {scale > 0.f ? rintf(__fdiv_rn(f.x, scale)) : 0.f, scale > 0.f ? rintf(__fdiv_rn(f.y, scale)) : 0.f};
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) code[2 * e + z] = __float_as_uint((q[z] == q[z] ? fminf(fmaxf(q[z], -127.f), 127.f) : 0.f) + kWhole);
+                    }
+                ++count;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += code[e];
+                uint32_t word[2];
+#pragma unroll
+                for (int e = 0; e < 8; e += 4)
+                    word[e / 4] = __byte_perm(__byte_perm(code[e], code[e + 1], 0x0040), __byte_perm(code[e + 2], code[e + 3], 0x0040), 0x5410);
+                *reinterpret_cast<uint2 *>(codes + (int64_t)o * d + c * 8) = make_uint2(word[0], word[1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] -= count * __float_as_uint(kWhole);
+            if (tid == 0) a.c.scales[kv][(int64_t)page * a.c.kv_heads + h] = scale;
+            if (kv == 0) {
+                __syncthreads();
+                if (g < groups) {
+                    // sums of a thread's codes, 16 bits each
+                    *reinterpret_cast<uint4 *>(part + g * d + c * 8) = make_uint4(__byte_perm(sum[0], sum[1], 0x5410), __byte_perm(sum[2], sum[3], 0x5410),
+                                                                                  __byte_perm(sum[4], sum[5], 0x5410), __byte_perm(sum[6], sum[7], 0x5410));
+                }
+                __syncthreads();
+                for (int e = tid; e < d; e += kAppendThreads) {
+                    int all = 0;
+                    for (int y = 0; y < groups; ++y) all += part[y * d + e];
+                    a.c.sums[((int64_t)page * a.c.kv_heads + h) * d + e] = (int16_t)all;
+                }
             }
         }
     }
@@ -198,10 +268,10 @@ template <typename T> __global__ void select_kernel(const SelectArgs a) {
 }
 
 // ---- attention of single tokens ------------------------------------------------------------------------------------------
-// A warp takes whole blocks: bulk copies bring a block's codes of one head (64 d bytes, contiguous) into its own ring in shared memory, two to three
+// A warp takes whole blocks: asynchronous copies bring a block's codes of one head (64 d bytes, contiguous) into its own ring in shared memory, two
 // pieces ahead, and mma.sync multiplies the group's query rows (up to 16) with them.  Few rows against a stream of keys: bound by the reading of
 // the cache, which tcgen05 tiles of 128 rows would not make quicker, while here codes go from bytes to fragments without another trip.
-// Codes are whole numbers up to 127, exact in fp16; the scale of a block of keys goes onto the scores, that of the values onto the block's
+// Codes are exact in fp16 (below); the scale of a block of keys goes onto the scores, that of the values onto the block's
 // product in fp32 before it joins the sums.  Probabilities are rounded to fp16 for the product (2^-11 relative; they are at most 1).  bf16 queries become
 // fp16 without a rounding that counts: a row is multiplied by the power of two that brings its largest element to 1 .. 2, so what falls below fp16's
 // normal range is off by less than 2^-24 of that element, fp32's own resolution.
@@ -211,7 +281,6 @@ template <typename T> __global__ void select_kernel(const SelectArgs a) {
 // its columns are free: lane g keeps four consecutive dimensions 32 u + 4 g of every 32 (and two of the last 16), one column of each
 // of the eight-wide tiles that they belong to.
 constexpr int kWarps = 4, kDecodeThreads = kWarps * 32, kSlots = 3;
-constexpr uint32_t kStatusTimeout = 4096u;   // bit raised in the status word when a bounded wait ran out
 
 struct AttentionArgs {
     Pages c;
@@ -224,20 +293,22 @@ struct AttentionArgs {
     float scale;
     void *out;                  // [count][heads][d]
     float *partial;             // [count * kv heads * parts][pieces][16][d + 2] when pieces > 1
-    uint32_t *status;
 };
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
-// bytes 0, 1 (2, 3) of a word of biased codes as two fp16: 0x6400 | x is 1024 + x
-__device__ __forceinline__ uint32_t codes_f16(uint32_t biased_pair) {
-    const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1024 + 128
-    const uint32_t w = biased_pair;
-    return half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&w), off));
-}
+// Codes as fp16 operands: code + 128 is a byte u, and the fp16 with the bits 0x00uu is u * 2^-24, exactly, so that spreading bytes is all the conversion there is.
+// Products are taken of u; what 128 makes of them is where their sums start.
+constexpr uint32_t kBias = 0x80808080u;
+constexpr float kUnit = 0x1p24f, kStart = -0x1p-17f;   // 1 / 2^-24; -128 * 2^-24
 __device__ __forceinline__ void key_codes(uint32_t word, uint32_t &lo, uint32_t &hi) {
-    word ^= 0x80808080u;
-    lo = codes_f16(__byte_perm(word, 0x64646464u, 0x4140));
-    hi = codes_f16(__byte_perm(word, 0x64646464u, 0x4342));
+    word ^= kBias;
+    lo = __byte_perm(word, 0u, 0x4140);
+    hi = __byte_perm(word, 0u, 0x4342);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 template <typename T> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -269,43 +340,77 @@ template <typename T, int NK> struct Rows {   // what a warp carries from block 
     float top[2], total[2];
 };
 
-// Scores of 64 keys (columns 8 n + 2 c, + 1 of rows g, g + 8) to probabilities, with the running maximum and sum; `n` keys are there.
+// Scores of 64 keys (columns 8 n + 2 c, + 1 of rows g, g + 8) to probabilities, with the running maximum and sum; `n` keys are there.  factor: not negative.
 template <typename T, int NK> __device__ __forceinline__ void softmax_step(Rows<T, NK> &r, float (&s)[8][4], const float (&factor)[2], int n) {
     const int c = threadIdx.x & 3;
+    if (n < kBlock) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x)
+        for (int x = 0; x < 8; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[x][e] = x * 8 + 2 * c + (e & 1) < n ? s[x][e] * factor[e >> 1] : -INFINITY;
+            for (int e = 0; e < 4; ++e)
+                if (x * 8 + 2 * c + (e & 1) >= n) s[x][e] = -INFINITY;
+    }
+    float shrink[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float m = r.top[i];
+        float m = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 8; ++x) m = fmaxf(m, fmaxf(s[x][2 * i], s[x][2 * i + 1]));
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
-        const float base = m == -INFINITY ? 0.f : m, shrink = exp2f(r.top[i] - base);
-        float sum = 0.f;
+        m = fmaxf(r.top[i], fmaxf(m, __shfl_xor_sync(~0u, m, 2)) * factor[i]);
+        const float base = m == -INFINITY ? 0.f : m;
+        shrink[i] = ex2(r.top[i] - base);
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < 8; ++x)
 #pragma unroll
             for (int e = 2 * i; e < 2 * i + 2; ++e) {
-                s[x][e] = exp2f(s[x][e] - base);
-                sum += s[x][e];
+                s[x][e] = ex2(fmaf(s[x][e], factor[i], -base));
+                sum[e & 1] += s[x][e];
             }
-        r.total[i] = r.total[i] * shrink + sum;   // this lane's part of the row: joined at the end
+        r.total[i] = r.total[i] * shrink[i] + (sum[0] + sum[1]);   // this lane's part of the row: joined at the end
         r.top[i] = m;
+    }
+    if (__any_sync(~0u, shrink[0] != 1.f || shrink[1] != 1.f)) {   // seldom, once the first blocks have gone by
 #pragma unroll
-        for (int t = 0; t < 2 * NK; ++t) {
-            r.acc[t][2 * i] *= shrink;
-            r.acc[t][2 * i + 1] *= shrink;
-        }
+        for (int t = 0; t < 2 * NK; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.acc[t][e] *= shrink[e >> 1];
     }
 }
 
+// d / 4 bytes of a key, as wide as they lie aligned
+template <int NK> __device__ __forceinline__ void key_words(const uint8_t *p, uint32_t (&w)[NK]) {
+    if constexpr (NK % 4 == 0) {
+#pragma unroll
+        for (int x = 0; x < NK; x += 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p + 4 * x);
+            w[x] = v.x; w[x + 1] = v.y; w[x + 2] = v.z; w[x + 3] = v.w;
+        }
+    } else if constexpr (NK % 2 == 0) {
+#pragma unroll
+        for (int x = 0; x < NK; x += 2) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(p + 4 * x);
+            w[x] = v.x; w[x + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < NK; ++x) w[x] = *reinterpret_cast<const uint32_t *>(p + 4 * x);
+    }
+}
+// A piece in shared memory: 64 rows of d bytes, 16 apart, so that the lanes of a fragment, which read eight rows (keys) or every second one (values), meet different
+// banks: bulk copies, which cannot leave a gap, made the reads the bound (8 and 4 lanes to a bank: 106 us for 23 900 blocks of two 8 KB pieces, now 75).
+template <int NK> constexpr int kPitch = NK * 16 + 16;
+template <int NK> constexpr int kPieceBytes = kBlock * kPitch<NK>;
+template <int NK> constexpr int decode_smem() {
+    constexpr int pieces = kWarps * kSlots * kPieceBytes<NK>, join = kWarps * 16 * (NK * 16 + 2) * 4;
+    return pieces > join ? pieces : join;
+}
+
 template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 2) decode_kernel(const AttentionArgs a) {
-    constexpr int D = NK * 16, kPiece = kBlock * D;   // bytes of a block's codes
+    constexpr int D = NK * 16, P = kPitch<NK>;
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ __align__(8) uint64_t bars[kWarps][kSlots];
+    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int piece = blockIdx.x % a.pieces, item = blockIdx.x / a.pieces;
     const int part = item % a.parts, h = item / a.parts % a.c.kv_heads, r = item / a.parts / a.c.kv_heads;
@@ -314,11 +419,8 @@ template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 
     const int32_t *list = a.lists ? a.lists + ((int64_t)r * a.c.kv_heads + h) * a.wanted : nullptr;
     const int units = list ? a.wanted : full;
     const int lo = (int)((int64_t)units * piece / a.pieces), hi = (int)((int64_t)units * (piece + 1) / a.pieces);
-    uint8_t *ring = raw + warp * kSlots * kPiece;
-    const uint32_t ring_at = tc::smem_u32(ring), bar = tc::smem_u32(&bars[warp][0]);
-    if (lane < kSlots) tc::mbar_init(bar + 8 * lane, 1);
-    tc::fence_mbar_init();
-    __syncwarp();
+    uint8_t *ring = raw + warp * kSlots * kPieceBytes<NK>;
+    const uint32_t ring_at = tc::smem_u32(ring);
 
     // Page of unit u, or -1: a list's entry counts where it names a complete block with a page and the list has not named it before.
     auto page_of = [&](int u) {
@@ -332,27 +434,40 @@ template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 
         }
         return a.s.page(r, j, a.c.pages);
     };
-    // the warp's next unit with a page, from u on
-    auto next = [&](int u, int &page) {
-        for (; u < hi; u += kWarps)
-            if ((page = page_of(u)) >= 0) return u;
-        return hi;
+    struct Unit {
+        int at, page;
+        float sk, sv;
     };
-    uint32_t sent = 0;   // pieces requested so far: keys and values of one block after another
-    auto request = [&](int kv, int page) {
-        const uint32_t slot = sent % kSlots;
-        if (lane == 0) {
-            tc::mbar_expect_tx(bar + 8 * slot, kPiece);
-            tc::bulk_copy_g2s(ring_at + slot * kPiece, a.c.codes[kv] + ((int64_t)page * a.c.kv_heads + h) * kPiece, kPiece, bar + 8 * slot);
+    // the warp's next unit with a page, from u on, and its scales
+    auto next = [&](int u) {
+        Unit x = {hi, -1, 0.f, 0.f};
+        for (; u < hi; u += kWarps)
+            if ((x.page = page_of(u)) >= 0) {
+                x.at = u;
+                x.sk = a.c.scales[0][(int64_t)x.page * a.c.kv_heads + h];
+                x.sv = a.c.scales[1][(int64_t)x.page * a.c.kv_heads + h];
+                break;
+            }
+        return x;
+    };
+    uint32_t sent = 0, used = 0;   // pieces requested and used so far: keys and values of one block after another
+    auto request = [&](int kv, const Unit &x) {   // one group of copies, an empty one where there is no unit
+        if (x.at < hi) {
+            const uint8_t *from = reinterpret_cast<const uint8_t *>(a.c.codes[kv]) + ((int64_t)x.page * a.c.kv_heads + h) * (kBlock * D);
+            const uint32_t to = ring_at + sent % kSlots * kPieceBytes<NK>;
+#pragma unroll
+            for (int y = 0; y < 2 * NK; ++y) {   // 64 rows of NK chunks
+                const int chunk = lane + 32 * y;
+                tc::cp_async_16(to + chunk / NK * P + chunk % NK * 16, from + chunk * 16, 16);
+            }
         }
+        tc::cp_async_commit();
         ++sent;
     };
-    bool ok = true;
-    uint32_t used = 0;
-    auto arrived = [&]() -> const uint8_t * {   // the oldest piece
-        const uint32_t slot = used % kSlots;
-        ok = ok && tc::mbar_wait(bar + 8 * slot, (used / kSlots) & 1);
-        return ring + slot * kPiece;
+    auto arrived = [&]() -> const uint8_t * {   // the oldest piece; two younger ones may be on their way
+        tc::cp_async_wait<2>();
+        __syncwarp();
+        return ring + used++ % kSlots * kPieceBytes<NK>;
     };
 
     // query rows: a[0] (row g, dimensions c D/4 + 4 s + 0, 1), a[1] row g + 8, a[2], a[3] dimensions + 2, + 3
@@ -397,6 +512,20 @@ template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 
             }
         }
     }
+    float start[2];   // of the rows' sums with codes + 128
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < 2 * NK; ++s) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&qf[s / 2][i + s % 2 * 2]));
+            sum += f.x + f.y;
+        }
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        start[i] = kStart * sum;
+        row_factor[i] *= kUnit;
+    }
     Rows<T, NK> rows;
 #pragma unroll
     for (int t = 0; t < 2 * NK; ++t)
@@ -406,36 +535,35 @@ template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 
     rows.total[0] = rows.total[1] = 0.f;
 
     // Pieces in the order K0 V0 K1 V1 ...; two are on their way ahead of the one in use.
-    int page = -1, page_next = -1, u = next(lo + warp, page);
-    if (u < hi) {
-        request(0, page);
-        request(1, page);
+    Unit now = next(lo + warp), then = {hi, -1, 0.f, 0.f};
+    if (now.at < hi) {
+        request(0, now);
+        request(1, now);
+        then = next(now.at + kWarps);
     }
-    while (u < hi && ok) {
-        const int un = next(u + kWarps, page_next);
-        const float sk = a.c.scales[0][(int64_t)page * a.c.kv_heads + h], sv = a.c.scales[1][(int64_t)page * a.c.kv_heads + h];
-        if (un < hi) request(0, page_next);   // into the third slot
+    while (now.at < hi) {
+        request(0, then);   // into the third slot
         const uint8_t *k = arrived();
-        if (!ok) break;
         float s[8][4];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
-            const uint8_t *kp = k + (x * 8 + g) * D + c * (D / 4);
+            s[x][0] = s[x][1] = start[0];
+            s[x][2] = s[x][3] = start[1];
+            uint32_t w[NK];
+            key_words<NK>(k + (x * 8 + g) * P + c * (D / 4), w);
 #pragma unroll
             for (int y = 0; y < NK; ++y) {
                 uint32_t b0, b1;
-                key_codes(*reinterpret_cast<const uint32_t *>(kp + 4 * y), b0, b1);
+                key_codes(w[y], b0, b1);
                 mma<__half>(s[x], qf[y], b0, b1);
             }
         }
-        ++used;
         __syncwarp();
-        if (un < hi) request(1, page_next);   // where the keys stood
-        const float factors[2] = {row_factor[0] * sk, row_factor[1] * sk};
+        request(1, then);   // where the keys stood
+        const Unit after = then.at < hi ? next(then.at + kWarps) : then;
+        const float factors[2] = {row_factor[0] * now.sk, row_factor[1] * now.sk}, sv = now.sv * kUnit;
         softmax_step<T, NK>(rows, s, factors, kBlock);
         const uint8_t *v = arrived();
-        if (!ok) break;
         uint32_t pf[4][4];
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
@@ -444,23 +572,31 @@ template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 
             pf[y][2] = pack<__half>(s[2 * y + 1][0], s[2 * y + 1][1]);
             pf[y][3] = pack<__half>(s[2 * y + 1][2], s[2 * y + 1][3]);
         }
+        float from[4] = {};   // what 128 makes of the values' sums: the probabilities, as they were rounded, times -128
+#pragma unroll
+        for (int y = 0; y < 4; ++y) mma<__half>(from, pf[y], 0x00800080u, 0x00800080u);
         auto values = [&](const int t0, const int tiles, const int dim, const bool half_word) {   // `tiles` tiles from t0 on: one word (half a word) per key
-            float o[4][4] = {};
+            float o[4][4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[x][e] = -from[e];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                uint32_t w[4];
+                uint32_t even[4], odd[4];   // bytes 0 and 2, 1 and 3 of four keys' words, a half each
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint8_t *vp = v + (16 * y + 2 * c + (e & 1) + 8 * (e >> 1)) * D + dim;
-                    w[e] = (half_word ? (uint32_t)*reinterpret_cast<const uint16_t *>(vp) : *reinterpret_cast<const uint32_t *>(vp)) ^ 0x80808080u;
+                    const uint8_t *vp = v + (16 * y + 2 * c + (e & 1) + 8 * (e >> 1)) * P + dim;
+                    const uint32_t w = (half_word ? (uint32_t)*reinterpret_cast<const uint16_t *>(vp) : *reinterpret_cast<const uint32_t *>(vp)) ^ kBias;
+                    even[e] = w & 0x00ff00ffu;
+                    odd[e] = __byte_perm(w, 0u, 0x4341);
                 }
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     if (x >= tiles) continue;
-                    // byte x of two keys side by side, each under the 0x64 that makes it 1024 + x
-                    const uint32_t sel = x | (4 + x) << 4;
-                    const uint32_t p0 = __byte_perm(w[0], w[1], sel), p1 = __byte_perm(w[2], w[3], sel);
-                    mma<__half>(o[x], pf[y], codes_f16(__byte_perm(p0, 0x64646464u, 0x4140)), codes_f16(__byte_perm(p1, 0x64646464u, 0x4140)));
+                    const uint32_t sel = x < 2 ? 0x5410 : 0x7632;   // halves of two keys side by side
+                    const uint32_t(&w)[4] = x % 2 ? odd : even;
+                    mma<__half>(o[x], pf[y], __byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel));
                 }
             }
 #pragma unroll
@@ -472,14 +608,11 @@ template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 
 #pragma unroll
         for (int y = 0; y < NK / 2; ++y) values(4 * y, 4, 32 * y + 4 * g, false);
         if constexpr (NK % 2 == 1) values(NK / 2 * 4, 2, NK / 2 * 32 + 2 * g, true);
-        ++used;
         __syncwarp();
-        u = un;
-        page = page_next;
+        now = then;
+        then = after;
     }
-    if (!ok && lane == 0) atomicOr(a.status, kStatusTimeout);
-    // copies in flight end before the block's shared memory is reused or given back (a bounded wait gave up above: again bounded)
-    for (; used < sent; ++used) (void)tc::mbar_wait(bar + 8 * (used % kSlots), (used / kSlots) & 1);
+    tc::cp_async_wait<0>();
 
     // the newest tokens, 16 bits, straight from the ring: one warp of the last piece
     if (rest > 0 && piece == a.pieces - 1 && warp == (hi - lo) % kWarps && tail >= 0 && tail < a.c.tails) {
@@ -569,7 +702,7 @@ template <typename T, int NK> __global__ void __launch_bounds__(kDecodeThreads, 
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float *p = joined + (w * 16 + row) * (D + 2);
-            const float f = exp2f(p[D] - base);
+            const float f = ex2(p[D] - base);
             sum = fmaf(f, p[dim], sum);
             total = fmaf(f, p[D + 1], total);
         }
@@ -601,7 +734,7 @@ template <typename T> __global__ void __launch_bounds__(128) join_kernel(const A
         const float base = top == -INFINITY ? 0.f : top;
         float sum = 0.f, total = 0.f;
         for (int y = 0; y < a.pieces; ++y) {
-            const float f = exp2f(__ldcg(p + y * step + D) - base);
+            const float f = ex2(__ldcg(p + y * step + D) - base);
             sum = fmaf(f, __ldcg(p + y * step + dim), sum);
             total = fmaf(f, __ldcg(p + y * step + D + 1), total);
         }
