@@ -240,7 +240,7 @@ template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint3
     uint32_t *redo_kv = redo + tiles;
     cudaError_t e = launch_behind(blocks::delta_kernel<T>, (unsigned)((rows + 15) / 16), 256, 0, st, a);
     if (e == cudaSuccess)
-        e = launch_behind(blocks::tcore::grad_q_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kForwardThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
+        e = launch_behind(blocks::tcore::grad_q_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kGradQThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
     if (e == cudaSuccess)
         e = launch_behind(blocks::tcore::grad_kv_kernel<T, DP>, (unsigned)blocks_all, blocks::tcore::kGradKVThreads, SmemKV::kBytes + 1024, st, a, q, g, k, v, redo_kv, status);
     if (e != cudaSuccess) return (int)e;

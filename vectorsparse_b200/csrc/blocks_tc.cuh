@@ -137,7 +137,8 @@ struct Scan {
 
 // Writes 32 rows of the warp, one to a lane, so that a row's bytes leave together: `value(g, v)` gives the lane's elements 32 g .. 32 g + 31 as
 // four 16-byte pieces.  They pass through `stage`, 32 rows of 128 bytes in each of DP / 64 slabs `slab` bytes apart, the pieces swizzled by the row.
-template <typename T, int DP, typename F> __device__ __forceinline__ void write_rows(uint8_t *stage, int slab, T *out, int64_t row_at, bool there, int d, F value) {
+// `first`: 0 or 1, the half of the slab that the first 32 elements take.
+template <typename T, int DP, typename F> __device__ __forceinline__ void write_rows(uint8_t *stage, int slab, T *out, int64_t row_at, bool there, int d, int first, F value) {
     const int lane = threadIdx.x & 31;
     __syncwarp();
 #pragma unroll
@@ -145,19 +146,22 @@ template <typename T, int DP, typename F> __device__ __forceinline__ void write_
         uint4 v[4];
         value(g, v);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(stage + g / 2 * slab + lane * 128 + ((((g % 2) * 4 + c) ^ (lane & 7)) << 4)) = v[c];
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4 *>(stage + (g + first) / 2 * slab + lane * 128 + ((((g + first) % 2 * 4 + c) ^ (lane & 7)) << 4)) = v[c];
     }
     __syncwarp();
     constexpr int kLanes = DP / 8;   // to a row
 #pragma unroll 4
     for (int r0 = 0; r0 < 32; r0 += 32 / kLanes) {
-        const int r = r0 + lane / kLanes, c = lane % kLanes;
+        const int r = r0 + lane / kLanes, c = lane % kLanes, at_slab = c + first * 4;
         const int64_t at = __shfl_sync(~0u, row_at, r);
         const bool live = __shfl_sync(~0u, (int)there, r);
         if (live && c * 8 < d)
-            *reinterpret_cast<uint4 *>(out + at + c * 8) = *reinterpret_cast<const uint4 *>(stage + c / 8 * slab + r * 128 + (((c % 8) ^ (r & 7)) << 4));
+            *reinterpret_cast<uint4 *>(out + at + c * 8) = *reinterpret_cast<const uint4 *>(stage + at_slab / 8 * slab + r * 128 + (((at_slab % 8) ^ (r & 7)) << 4));
     }
 }
+// The two warps of a quarter of the rows meet (64 threads, barriers 1 .. 4).
+__device__ __forceinline__ void bar_pair(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 template <typename T> __device__ __forceinline__ uint4 pack8(const float *f) {
     return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
@@ -398,7 +402,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 for (int y = 0; y < 32; ++y) f[y] = x > 0 && total != 0.f ? __uint_as_float(o[y]) * inv : 0.f;
             };
             uint8_t *stage = sm + M::kQ + warp * 32 * 128;
-            write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result), row, there, s.d, [&](int g, uint4 (&v)[4]) {
+            write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result), row, there, s.d, 0, [&](int g, uint4 (&v)[4]) {
                 float f[32];
                 result(g, f);
 #pragma unroll
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
             });
             if (a.result_low)
-                write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result_low), row, there, s.d, [&](int g, uint4 (&v)[4]) {
+                write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result_low), row, there, s.d, 0, [&](int g, uint4 (&v)[4]) {
                     float f[32];
                     result(g, f);
 #pragma unroll
@@ -456,8 +460,9 @@ template <int DP> struct GradQSmem {
     static_assert(kHolder + 4 <= 1024, "head");
     static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs an SM");
 };
+constexpr int kGradQThreads = 320;
 template <typename T, int DP>
-__global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
+__global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
                                                                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, uint32_t *redo,
                                                                     uint32_t *status) {
     using M = GradQSmem<DP>;
@@ -477,12 +482,12 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
 
     if (threadIdx.x == 0) {
         for (int bar : {M::kBarQ, M::kKFull, M::kKFull + 8, M::kKEmpty, M::kKEmpty + 8, M::kVFull, M::kVEmpty, M::kSP, M::kDq, M::kDrain}) tc::mbar_init(base + bar, 1);
-        tc::mbar_init(base + M::kDs, 4);
+        tc::mbar_init(base + M::kDs, 8);
         for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
         *abort_flag = 0;
         tc::fence_mbar_init();
     }
-    if (warp == 5) {
+    if (warp == 9) {
         tc::tmem_alloc(base + M::kHolder, 256);
         tc::tmem_relinquish();
     }
@@ -492,7 +497,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder);
     bool bad = false;
 
-    if (warp == 4) {
+    if (warp == 8) {
         pdl_wait();
         const uint32_t q_bytes = (uint32_t)(a.tile * s.group * 128 * (DP / 64));
         if (lane == 0) {
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
                 }
             }
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         if (lane == 0) {
             constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescQ = idesc<T>(DP, 0, 1);
             const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
@@ -581,10 +586,11 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
         }
     } else {
-        const int r = threadIdx.x, qx = r / s.group, i = t.i0 + qx;
+        const int quarter = warp & 3, half = warp >> 2;   // two warps to a quarter of the rows, 32 keys each
+        const int r = quarter * 32 + lane, qx = r / s.group, i = t.i0 + qx;
         const bool there = r < a.tile * s.group && i < s.queries;
         const int h = t.kvh * s.group + r % s.group, end = there ? s.end(i, len) : 0;
-        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
         const float c = a.scale * kLog2e;
         float lse = INFINITY, lift = 1.f, minus_delta = 0.f;
         uint32_t x = 0;
@@ -610,28 +616,26 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
             tc::tc_fence_after_sync();
             const bool whole = __all_sync(~0u, n <= 0 || n == kBlock);
             const float off = n > 0 ? -lse : -INFINITY;   // a row that has not listed the block has no weight there
-            uint32_t ds[32];
+            uint32_t u[32], d[32], ds[16];
+            tc::tmem_ld_x32_issue(mine + 32 * half, u);
+            tc::tmem_ld_x32_issue(mine + 64 + 32 * half, d);
+            tc::tmem_ld_x32_wait(u);
+            tc::tmem_ld_x32_wait(d);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t u[32], d[32];
-                tc::tmem_ld_x32_issue(mine + 32 * half, u);
-                tc::tmem_ld_x32_issue(mine + 64 + 32 * half, d);
-                tc::tmem_ld_x32_wait(u);
-                tc::tmem_ld_x32_wait(d);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    float2 w = fma2(pair(u[2 * k], u[2 * k + 1]), make_float2(c, c), make_float2(off, off));
-                    w.x = ex2(w.x);
-                    w.y = ex2(w.y);
-                    float2 f = mul2(w, fma2(pair(d[2 * k], d[2 * k + 1]), make_float2(lift, lift), make_float2(minus_delta, minus_delta)));
-                    if (!whole) {
-                        if (32 * half + 2 * k >= n) f.x = 0.f;
-                        if (32 * half + 2 * k + 1 >= n) f.y = 0.f;
-                    }
-                    ds[16 * half + k] = pack2<T>(f.x, f.y);
+            for (int k = 0; k < 16; ++k) {
+                float2 w = fma2(pair(u[2 * k], u[2 * k + 1]), make_float2(c, c), make_float2(off, off));
+                w.x = ex2(w.x);
+                w.y = ex2(w.y);
+                float2 f = mul2(w, fma2(pair(d[2 * k], d[2 * k + 1]), make_float2(lift, lift), make_float2(minus_delta, minus_delta)));
+                if (!whole) {
+                    if (32 * half + 2 * k >= n) f.x = 0.f;
+                    if (32 * half + 2 * k + 1 >= n) f.y = 0.f;
                 }
+                ds[k] = pack2<T>(f.x, f.y);
             }
-            tc::tmem_st_x32(mine, ds);
+            // dS goes where the first half's scores stood, which that half's other warp has read before it comes here
+            bar_pair(1 + quarter);
+            tc::tmem_st_x16(mine + 16 * half, ds);
             tc::tmem_st_wait();
             tc::tc_fence_before_sync();
             __syncwarp();
@@ -642,10 +646,12 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
             tc::tc_fence_after_sync();
             const int64_t row = (((int64_t)t.b * s.queries + i) * s.heads + h) * s.d;
             const float back = a.scale / lift;
-            write_rows<T, DP>(sm + M::kQ + warp * 32 * 128, kRows * 128, static_cast<T *>(a.result), row, there, s.d, [&](int g, uint4 (&v)[4]) {
+            // the two warps of a quarter take a half of the dimensions each
+            write_rows<T, DP / 2>(sm + M::kQ + quarter * 32 * 128 + (DP == 128 ? half * kRows * 128 : 0), kRows * 128, static_cast<T *>(a.result) + half * (DP / 2), row, there,
+                                  s.d - half * (DP / 2), half * (DP == 64), [&](int g, uint4 (&v)[4]) {
                 uint32_t o[32];
                 float f[32];
-                if (x > 0) tc::tmem_ld_x32(mine + 128 + 32 * g, o);
+                if (x > 0) tc::tmem_ld_x32(mine + 128 + half * (DP / 2) + 32 * g, o);
 #pragma unroll
                 for (int y = 0; y < 32; ++y) {
                     f[y] = x > 0 ? __uint_as_float(o[y]) * back : 0.f;
@@ -662,7 +668,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) grad_q_kernel(const Args a
         redo[t.index] = again;
         if (*abort_flag) atomicOr(status, kStatusGradQ);
     }
-    if (warp == 5) {
+    if (warp == 9) {
         tc::tc_fence_after_sync();
         tc::tmem_dealloc(tmem, 256);
     }
