@@ -94,18 +94,25 @@ __device__ __forceinline__ Tile tile_of(const Shape &s, int tile, int64_t index)
     return t;
 }
 
+// A load that stays where it is written: left to itself the compiler moves it to each use of its word, into the loop over a word's bits, and every step of
+// the loader waits for L2.
+__device__ __forceinline__ uint32_t load_here(const uint32_t *p) {
+    uint32_t v;
+    asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
 // The blocks that a tile of queries has listed, in ascending order, found by a warp 32 at a time.
 struct Scan {
     const uint32_t *bits;
     int blocks, end, words, shift;
     uint32_t mask;
     int base = 0;
-    uint32_t now[4], then[4];
+    uint32_t then[4];
 
     __device__ __forceinline__ void fetch(int from, uint32_t (&to)[4]) const {
         const int j = from + (threadIdx.x & 31);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) to[k] = k < words && j < end ? (__ldg(bits + (int64_t)k * blocks + j) >> shift) & mask : 0u;
+        for (int k = 0; k < 4; ++k) to[k] = k < words && j < end ? (load_here(bits + (int64_t)k * blocks + j) >> shift) & mask : 0u;
     }
     __device__ __forceinline__ Scan(const Shape &s, const uint32_t *all, const Tile &t, int tile) {
         blocks = s.blocks;
@@ -118,20 +125,19 @@ struct Scan {
         end = min(s.blocks, (s.end(last, len) + kBlock - 1) / kBlock);
         fetch(0, then);
     }
-    // the lanes' next 32 blocks: false where there are no more
-    __device__ __forceinline__ bool next(uint32_t &some) {
+    // The next 32 blocks' words go to `to` (a row of 32 for each of four words); false where there are no more.  One lane then goes through the chunk on its own:
+    // shuffles for each of its entries, between waits of that lane, cost the warp a thousand cycles an entry.
+    __device__ __forceinline__ bool next(uint32_t (*to)[32], uint32_t &some) {
         if (base >= end) return false;
+        const int lane = threadIdx.x & 31;
+        __syncwarp();   // the chunk before has been gone through
 #pragma unroll
-        for (int k = 0; k < 4; ++k) now[k] = then[k];
+        for (int k = 0; k < 4; ++k) to[k][lane] = then[k];
+        some = __ballot_sync(~0u, (then[0] | then[1] | then[2] | then[3]) != 0);
         fetch(base + 32, then);
-        some = __ballot_sync(~0u, (now[0] | now[1] | now[2] | now[3]) != 0);
         base += 32;
+        __syncwarp();
         return true;
-    }
-    __device__ __forceinline__ void entry(int lane, Entry &e) const {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) e.rows[k] = __shfl_sync(~0u, now[k], lane);
-        e.block = base - 32 + lane;
     }
 };
 
@@ -177,11 +183,12 @@ constexpr float kSlack = 8.f;
 template <int DP> struct ForwardSmem {
     static constexpr int kSlots = DP == 128 ? 4 : 6;
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
-    static constexpr int kQ = 1024, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // the first 1024 bytes: entries, barriers
+    static constexpr int kQ = 1024, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // the first 1024 bytes: entries, barriers, a chunk of the scan
     static constexpr int kEntriesAt = 0, kBars = kEntries * sizeof(Entry);
     static constexpr int kBarQ = kBars, kFull = kBarQ + 8, kEmpty = kFull + 8 * kSlots, kS = kEmpty + 8 * kSlots, kP = kS + 16, kPv = kP + 16, kE = kPv + 16, kDrain = kE + 8 * kEntries, kAbort = kDrain + 8,
                          kHolder = kAbort + 4;
-    static_assert(kHolder + 4 <= 1024, "head");
+    static constexpr int kChunk = 512;
+    static_assert(kHolder + 4 <= kChunk, "head");
 };
 constexpr int kForwardThreads = 192;
 
@@ -246,26 +253,22 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             ++at;
         };
         Scan scan(s, a.bits, t, a.tile);
+        uint32_t(*chunk)[32] = reinterpret_cast<uint32_t(*)[32]>(sm + M::kChunk);
         uint32_t some;
-        while (ok && scan.next(some)) {
-            for (; some && ok; some &= some - 1) {
-                Entry e;
-                scan.entry(__ffs(some) - 1, e);
-                if (lane == 0) {
+        while (scan.next(chunk, some))
+            if (lane == 0)
+                for (; some && ok; some &= some - 1) {
+                    const int x = __ffs(some) - 1, block = scan.base - 32 + x;
                     ok = slot_free();
-                    if (ok) {
-                        Entry *to = reinterpret_cast<Entry *>(sm + M::kEntriesAt) + (at / 2) % kEntries;
-                        *reinterpret_cast<uint4 *>(to->rows) = make_uint4(e.rows[0], e.rows[1], e.rows[2], e.rows[3]);
-                        to->block = e.block;
-                        tc::mbar_arrive(base + M::kE + 8 * ((at / 2) % kEntries));
-                        load(&map_k, e.block);
-                        ok = slot_free();
-                        if (ok) load(&map_v, e.block);
-                    }
+                    if (!ok) break;
+                    Entry *to = reinterpret_cast<Entry *>(sm + M::kEntriesAt) + (at / 2) % kEntries;
+                    *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][x], chunk[1][x], chunk[2][x], chunk[3][x]);
+                    to->block = block;
+                    tc::mbar_arrive(base + M::kE + 8 * ((at / 2) % kEntries));
+                    load(&map_k, block);
+                    ok = slot_free();
+                    if (ok) load(&map_v, block);
                 }
-                ok = __shfl_sync(~0u, (int)ok, 0);
-            }
-        }
         if (lane == 0) {
             if (ok && slot_free()) {
                 reinterpret_cast<Entry *>(sm + M::kEntriesAt)[(at / 2) % kEntries].block = -1;
@@ -457,7 +460,8 @@ template <int DP> struct GradQSmem {
     static constexpr int kBars = kEntries * sizeof(Entry);
     static constexpr int kBarQ = kBars, kKFull = kBarQ + 8, kKEmpty = kKFull + 16, kVFull = kKEmpty + 16, kVEmpty = kVFull + 8, kSP = kVEmpty + 8, kDs = kSP + 8, kDq = kDs + 8,
                          kE = kDq + 8, kDrain = kE + 8 * kEntries, kAbort = kDrain + 8, kHolder = kAbort + 4;
-    static_assert(kHolder + 4 <= 1024, "head");
+    static constexpr int kChunk = 512;
+    static_assert(kHolder + 4 <= kChunk, "head");
     static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 constexpr int kGradQThreads = 320;
@@ -514,27 +518,22 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
             for (int y = 0; y < DP / 64; ++y) tc::tma_load_4d(to + y * kBlock * 128, map, bar, y * 64, t.kvh, j * kBlock, t.b);
         };
         Scan scan(s, a.bits, t, a.tile);
+        uint32_t(*chunk)[32] = reinterpret_cast<uint32_t(*)[32]>(sm + M::kChunk);
         uint32_t some;
-        while (ok && scan.next(some)) {
-            for (; some && ok; some &= some - 1) {
-                Entry e;
-                scan.entry(__ffs(some) - 1, e);
-                if (lane == 0) {
+        while (scan.next(chunk, some))
+            if (lane == 0)
+                for (; some && ok; some &= some - 1, ++x) {
+                    const int y = __ffs(some) - 1, block = scan.base - 32 + y;
                     ok = x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
-                    if (ok) {
-                        Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
-                        *reinterpret_cast<uint4 *>(to->rows) = make_uint4(e.rows[0], e.rows[1], e.rows[2], e.rows[3]);
-                        to->block = e.block;
-                        tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                        load(&map_k, base + M::kK + (x & 1) * M::kSlotBytes, base + M::kKFull + 8 * (x & 1), e.block);
-                        ok = x < 1 || wait(base + M::kVEmpty, (x - 1) & 1, abort_flag);
-                        if (ok) load(&map_v, base + M::kV, base + M::kVFull, e.block);
-                    }
+                    if (!ok) break;
+                    Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
+                    *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][y], chunk[1][y], chunk[2][y], chunk[3][y]);
+                    to->block = block;
+                    tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
+                    load(&map_k, base + M::kK + (x & 1) * M::kSlotBytes, base + M::kKFull + 8 * (x & 1), block);
+                    ok = x < 1 || wait(base + M::kVEmpty, (x - 1) & 1, abort_flag);
+                    if (ok) load(&map_v, base + M::kV, base + M::kVFull, block);
                 }
-                ok = __shfl_sync(~0u, (int)ok, 0);
-                ++x;
-            }
-        }
         if (lane == 0) {
             if (ok && (x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
                 reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
@@ -685,7 +684,8 @@ template <int DP> struct GradKVSmem {
     static constexpr int kBars = kEntries * sizeof(Entry);
     static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 16, kSP = kEmpty + 16, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
                          kAbort = kDrain + 8, kHolder = kAbort + 4;
-    static_assert(kHolder + 4 <= 1024 && kBytes + 1024 <= 227 * 1024, "shared memory");
+    static constexpr int kChunk = 512;
+    static_assert(kHolder + 4 <= kChunk && kBytes + 1024 <= 227 * 1024, "shared memory");
 };
 constexpr int kGradKVThreads = 320;
 template <typename T, int DP>
@@ -739,46 +739,43 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
         const int shown = j * kBlock >= len ? tiles : s.causal ? max(0, j * kBlock - (s.keys - s.queries)) / a.tile : 0;   // no tile before can have the block
         const uint32_t mask = a.tile >= 32 ? ~0u : (1u << a.tile) - 1;
         const uint32_t *bits = a.bits + bh * s.words * s.blocks + j;
-        uint32_t then[4], now[4];
+        uint32_t then[4];
         auto fetch = [&](int from) {
             const int i0 = (from + lane) * a.tile;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 then[k] = from + lane < tiles && (k == 0 || 32 * k < a.tile) && (i0 >> 5) + k < s.words
-                              ? (__ldcg(bits + (int64_t)((i0 >> 5) + k) * s.blocks) >> (i0 & 31)) & mask
+                              ? (load_here(bits + (int64_t)((i0 >> 5) + k) * s.blocks) >> (i0 & 31)) & mask
                               : 0u;
         };
+        uint32_t(*chunk)[32] = reinterpret_cast<uint32_t(*)[32]>(sm + M::kChunk);
         uint32_t x = 0;
         bool ok = true;
         fetch(shown);
-        for (int from = shown; ok && from < tiles; from += 32) {
+        for (int from = shown; from < tiles; from += 32) {   // as Scan::next
+            __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) now[k] = then[k];
+            for (int k = 0; k < 4; ++k) chunk[k][lane] = then[k];
+            uint32_t some = __ballot_sync(~0u, (then[0] | then[1] | then[2] | then[3]) != 0);
             fetch(from + 32);
-            for (uint32_t some = __ballot_sync(~0u, (now[0] | now[1] | now[2] | now[3]) != 0); some && ok; some &= some - 1) {
-                const int src = __ffs(some) - 1;
-                uint32_t rows[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(~0u, now[k], src);
-                if (lane == 0) {
+            __syncwarp();
+            if (lane == 0)
+                for (; some && ok; some &= some - 1, ++x) {
+                    const int src = __ffs(some) - 1;
                     ok = x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
-                    if (ok) {
-                        const int i0 = (from + src) * a.tile;
-                        Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
-                        *reinterpret_cast<uint4 *>(to->rows) = make_uint4(rows[0], rows[1], rows[2], rows[3]);
-                        to->block = i0;
-                        tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                        const uint32_t bar = base + M::kFull + 8 * (x & 1), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
-                        tc::mbar_expect_tx(bar, 2 * q_bytes);
-                        for (int y = 0; y < DP / 64; ++y) {
-                            tc::tma_load_4d(at + y * kRows * 128, &map_q, bar, y * 64, kvh * s.group, i0, b);
-                            tc::tma_load_4d(at + M::kQBytes + y * kRows * 128, &map_g, bar, y * 64, kvh * s.group, i0, b);
-                        }
+                    if (!ok) break;
+                    const int i0 = (from + src) * a.tile;
+                    Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
+                    *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][src], chunk[1][src], chunk[2][src], chunk[3][src]);
+                    to->block = i0;
+                    tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
+                    const uint32_t bar = base + M::kFull + 8 * (x & 1), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
+                    tc::mbar_expect_tx(bar, 2 * q_bytes);
+                    for (int y = 0; y < DP / 64; ++y) {
+                        tc::tma_load_4d(at + y * kRows * 128, &map_q, bar, y * 64, kvh * s.group, i0, b);
+                        tc::tma_load_4d(at + M::kQBytes + y * kRows * 128, &map_g, bar, y * 64, kvh * s.group, i0, b);
                     }
                 }
-                ok = __shfl_sync(~0u, (int)ok, 0);
-                ++x;
-            }
         }
         if (lane == 0) {
             if (ok && (x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
