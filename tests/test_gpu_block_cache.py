@@ -325,3 +325,28 @@ def test_a_dispatch_mode_sees_the_operators():
     m.check()
     assert mode.seen == ["cache_select", "cache_attention", "cache_append", "select_blocks", "selected_attention", "selected_attention_backward", "selected_attention"]
     assert torch.isfinite(leaf.grad).all()
+
+
+@pytest.mark.parametrize("blocks", [40, 300, 1300])
+def test_selection_of_equal_scores_and_missing_pages(blocks):
+    """Scores that are all alike, or alike in groups: the lowest blocks; blocks without a page cannot be had."""
+    m = Model(2, blocks, 1, 16, torch.float16)
+    length = torch.tensor([blocks * 64 + 3, blocks * 64], dtype=torch.int32, device=DEV)
+    c, q = m.cache, torch.ones((2, 2, 16), dtype=torch.float16, device=DEV)
+    c.k_sums.fill_(3)
+    c.k_scales.fill_(0.5)
+    table = m.dev[0].clone()
+    for count in (1, 2, 7, 33, blocks, blocks + 4):
+        got = torch_ops.cache_select(q, c, table, length, count).cpu().numpy()
+        want = sorted({blocks - 1, *range(min(count, blocks) - 1)})
+        assert (got[:, 0, :len(want)] == np.array(want)).all() and (got[:, 0, len(want):] == -1).all()
+    c.k_sums[table[0, 5::9].long()] = 4             # a group above the rest
+    c.k_sums[table[1, 11].long()] = 5
+    table[0, 14], table[1, 3] = -1, c.pages
+    for count in (2, 5, 20):
+        got = torch_ops.cache_select(q, c, table, length, count).cpu().numpy()
+        best = [[j for j in range(5, blocks, 9) if j != 14], [11]]
+        for r, gone in ((0, 14), (1, 3)):
+            order = [j for j in best[r] if j != blocks - 1] + [j for j in range(blocks - 1) if j not in best[r] and j != gone]
+            want = sorted(order[:count - 1] + [blocks - 1])
+            assert got[r, 0, :len(want)].tolist() == want and (got[r, 0, len(want):] == -1).all(), (count, r)
