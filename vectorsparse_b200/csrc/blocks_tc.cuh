@@ -174,7 +174,7 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const float *f) {
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // A barrier tells a phase from the next but not from the one after that, so what may be two products ahead or behind has two barriers, one for either buffer of S.
-// Per block: S[128 x 64] = Q K^T (operands in shared memory), the softmax's step by one thread per row out of tensor memory, P (16 bits) back into S's place,
+// Per block: S[128 x 64] = Q K^T (operands in shared memory), the softmax's step by two threads per row, 32 keys each, out of tensor memory, P (16 bits) back into S's place,
 // O[128 x d] += P V with P as the operand in tensor memory.  S is double buffered; 256 columns of tensor memory and ~100 KB of shared memory, so that
 // two CTAs share an SM and one's products run under the other's exponentials.
 // The maximum that weights are taken relative to follows the true one only when that has grown by 2^8: weights then stay below 256, exact enough in
@@ -183,14 +183,15 @@ constexpr float kSlack = 8.f;
 template <int DP> struct ForwardSmem {
     static constexpr int kSlots = DP == 128 ? 4 : 6;
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
-    static constexpr int kQ = 1024, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // the first 1024 bytes: entries, barriers, a chunk of the scan
+    static constexpr int kQ = 3072, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // ahead: entries, barriers, a chunk of the scan, 2 KB for the rows' threads
     static constexpr int kEntriesAt = 0, kBars = kEntries * sizeof(Entry);
     static constexpr int kBarQ = kBars, kFull = kBarQ + 8, kEmpty = kFull + 8 * kSlots, kS = kEmpty + 8 * kSlots, kP = kS + 16, kPv = kP + 16, kE = kPv + 16, kDrain = kE + 8 * kEntries, kAbort = kDrain + 8,
                          kHolder = kAbort + 4;
-    static constexpr int kChunk = 512;
-    static_assert(kHolder + 4 <= kChunk, "head");
+    static constexpr int kChunk = 512, kMeet = 1024;
+    static_assert(kHolder + 4 <= kChunk && kMeet + 4 * kRows * 4 <= kQ, "head");
+    static_assert(2 * (kBytes + 2048) <= 228 * 1024, "two CTAs an SM");
 };
-constexpr int kForwardThreads = 192;
+constexpr int kForwardThreads = 320;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(base + M::kS + 8 * i, 1);
-            tc::mbar_init(base + M::kP + 8 * i, 4);
+            tc::mbar_init(base + M::kP + 8 * i, 8);
             tc::mbar_init(base + M::kPv + 8 * i, 1);
         }
         tc::mbar_init(base + M::kDrain, 1);
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         *abort_flag = 0;
         tc::fence_mbar_init();
     }
-    if (warp == 5) {
+    if (warp == 9) {
         tc::tmem_alloc(base + M::kHolder, 256);
         tc::tmem_relinquish();
     }
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
     bool bad = false;
     pdl_launch_dependents();
 
-    if (warp == 4) {
+    if (warp == 8) {
         // loader: position 2 x holds the keys, 2 x + 1 the values of the x-th block
         pdl_wait();   // the bits are the kernel's before
         const uint32_t q_bytes = (uint32_t)(a.tile * s.group * 128 * (DP / 64));
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                     for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (x % M::kSlots), (x / M::kSlots) & 1); ++y) {}
             }
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         if (lane == 0) {
             constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescO = idesc<T>(DP, 0, 1);
             const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
@@ -320,12 +321,13 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
         }
     } else {
-        const int r = threadIdx.x, qx = r / s.group, i = t.i0 + qx;
+        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane, qx = r / s.group, i = t.i0 + qx;
+        float *meet = reinterpret_cast<float *>(sm + M::kMeet);   // [2][2][128]: what the two threads of a row tell each other
         const bool there = r < a.tile * s.group && i < s.queries;
         const int h = t.kvh * s.group + r % s.group, end = there ? s.end(i, len) : 0;
-        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
         const float c = a.scale * kLog2e;
-        float top = -INFINITY, total = 0.f;   // what the weights are relative to, and their sum
+        float top = -INFINITY, total = 0.f;   // what the weights are relative to, and the sum of this thread's
         uint32_t x = 0;
         bool ok = true;
         for (;; ++x) {
@@ -339,21 +341,21 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             ok = __all_sync(~0u, wait(base + M::kS + 8 * (x & 1), (x >> 1) & 1, abort_flag));
             if (!ok) break;
             tc::tc_fence_after_sync();
-            uint32_t u[64];
-            uint32_t (&lo)[32] = *reinterpret_cast<uint32_t (*)[32]>(u), (&hi)[32] = *reinterpret_cast<uint32_t (*)[32]>(u + 32);
-            tc::tmem_ld_x32_issue(mine + (x & 1) * 64, lo);
-            tc::tmem_ld_x32_issue(mine + (x & 1) * 64 + 32, hi);
-            tc::tmem_ld_x32_wait(lo);
-            tc::tmem_ld_x32_wait(hi);
+            uint32_t u[32];
+            tc::tmem_ld_x32(mine + (x & 1) * 64 + 32 * half, u);
             if (__any_sync(~0u, n > 0 && n < kBlock)) {   // a block that ends inside: the queries' own, mostly
 #pragma unroll
-                for (int k = 0; k < kBlock; ++k)
-                    if (k >= n) u[k] = __float_as_uint(-INFINITY);
+                for (int k = 0; k < 32; ++k)
+                    if (32 * half + k >= n) u[k] = __float_as_uint(-INFINITY);
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 0; k < kBlock; k += 2) m[k / 2 % 4] = max3(m[k / 2 % 4], __uint_as_float(u[k]), __uint_as_float(u[k + 1]));
-            const float high = n > 0 ? fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c : -INFINITY;
+            for (int k = 0; k < 32; k += 2) m[k / 2 % 4] = max3(m[k / 2 % 4], __uint_as_float(u[k]), __uint_as_float(u[k + 1]));
+            m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            float *here = meet + (x & 1) * 2 * kRows + r;
+            here[half * kRows] = m[0];
+            bar_pair(1 + quarter);   // also: both have read their scores, P may go where the first half's stood
+            const float high = n > 0 ? fmaxf(m[0], here[(half ^ 1) * kRows]) * c : -INFINITY;
             if (__any_sync(~0u, high > top + kSlack)) {
                 const float to = fmaxf(top, high), shrink = to == -INFINITY ? 1.f : ex2(top - to);
                 top = to;
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                     if (!ok) break;
                     tc::tc_fence_after_sync();
 #pragma unroll 1
-                    for (int k = 0; k < DP; k += 32) {
+                    for (int k = half * (DP / 2); k < (half + 1) * (DP / 2); k += 32) {
                         uint32_t o[32];
                         tc::tmem_ld_x32(mine + 128 + k, o);
 #pragma unroll
@@ -375,9 +377,9 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             // a row that has not listed the block has no weight there: its scores, finite ones, all end at -inf
             const float off = n <= 0 ? -INFINITY : top == -INFINITY ? 0.f : -top;
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            uint32_t p[32];
+            uint32_t p[16];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
+            for (int k = 0; k < 16; ++k) {
                 float2 y = fma2(pair(u[2 * k], u[2 * k + 1]), make_float2(c, c), make_float2(off, off));
                 y.x = ex2(y.x);
                 y.y = ex2(y.y);
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             }
             sum[0] = add2(sum[0], sum[1]);
             total += sum[0].x + sum[0].y;
-            tc::tmem_st_x32(mine + (x & 1) * 64, p);
+            tc::tmem_st_x16(mine + (x & 1) * 64 + 16 * half, p);
             tc::tmem_st_wait();
             tc::tc_fence_before_sync();
             __syncwarp();
@@ -397,15 +399,21 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         if (ok) {
             tc::tc_fence_after_sync();
             const int64_t row = (((int64_t)t.b * s.queries + i) * s.heads + h) * s.d;
+            float *here = meet + (x & 1) * 2 * kRows + r;
+            here[half * kRows] = total;
+            bar_pair(1 + quarter);
+            total = meet[(x & 1) * 2 * kRows + r] + meet[((x & 1) * 2 + 1) * kRows + r];   // in the same order in both
             const float inv = total == 0.f ? 0.f : 1.f / total;
             auto result = [&](int g, float (&f)[32]) {
                 uint32_t o[32];
-                if (x > 0) tc::tmem_ld_x32(mine + 128 + 32 * g, o);
+                if (x > 0) tc::tmem_ld_x32(mine + 128 + half * (DP / 2) + 32 * g, o);
 #pragma unroll
                 for (int y = 0; y < 32; ++y) f[y] = x > 0 && total != 0.f ? __uint_as_float(o[y]) * inv : 0.f;
             };
-            uint8_t *stage = sm + M::kQ + warp * 32 * 128;
-            write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result), row, there, s.d, 0, [&](int g, uint4 (&v)[4]) {
+            // the two warps of a quarter take a half of the dimensions each
+            uint8_t *stage = sm + M::kQ + quarter * 32 * 128 + (DP == 128 ? half * kRows * 128 : 0);
+            const int first = half * (DP / 2);
+            write_rows<T, DP / 2>(stage, kRows * 128, static_cast<T *>(a.result) + first, row, there, s.d - first, half * (DP == 64), [&](int g, uint4 (&v)[4]) {
                 float f[32];
                 result(g, f);
 #pragma unroll
@@ -414,7 +422,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
             });
             if (a.result_low)
-                write_rows<T, DP>(stage, kRows * 128, static_cast<T *>(a.result_low), row, there, s.d, 0, [&](int g, uint4 (&v)[4]) {
+                write_rows<T, DP / 2>(stage, kRows * 128, static_cast<T *>(a.result_low) + first, row, there, s.d - first, half * (DP == 64), [&](int g, uint4 (&v)[4]) {
                     float f[32];
                     result(g, f);
 #pragma unroll
@@ -423,7 +431,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                     for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
                 });
             bad |= there && total != total;
-            if (there) a.lse[((int64_t)t.b * s.heads + h) * s.queries + i] = total == 0.f ? INFINITY : top + log2f(total);
+            if (there && half == 0) a.lse[((int64_t)t.b * s.heads + h) * s.queries + i] = total == 0.f ? INFINITY : top + log2f(total);
         }
     }
     tc::tc_fence_before_sync();
@@ -432,7 +440,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         redo[t.index] = again;
         if (*abort_flag) atomicOr(status, kStatusForward);
     }
-    if (warp == 5) {
+    if (warp == 9) {
         tc::tc_fence_after_sync();
         tc::tmem_dealloc(tmem, 256);
     }
