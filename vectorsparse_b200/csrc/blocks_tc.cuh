@@ -25,10 +25,25 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc(int n, int a_
     return tc::make_idesc_f16(kRows, n, a_mn, b_mn) | (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? kBf16Operands : 0u);
 }
 
-// Waits for a phase, or until another role of the CTA has given up; gives up itself after as many polls as the other tensor kernels.
+// Waits for a phase, or until another role of the CTA has given up; gives up itself after some seconds.  Polls without a time to be suspended for: those are quicker
+// by a third where the phase is there already, as it mostly is, and that is 5 % of the forward kernel.
+constexpr uint32_t kMaxPolls = 1u << 22;
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
-    for (uint32_t i = 0; i < tc::kMaxPolls; ++i) {
-        if (tc::mbar_try_wait(bar, parity)) return true;
+    for (uint32_t i = 0; i < kMaxPolls; ++i) {
+        if (try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
     }
     *abort_flag = 1;
@@ -185,7 +200,7 @@ template <int DP> struct ForwardSmem {
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
     static constexpr int kQ = 3072, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // ahead: entries, barriers, a chunk of the scan, 2 KB for the rows' threads
     static constexpr int kEntriesAt = 0, kBars = kEntries * sizeof(Entry);
-    static constexpr int kBarQ = kBars, kFull = kBarQ + 8, kEmpty = kFull + 8 * kSlots, kS = kEmpty + 8 * kSlots, kP = kS + 16, kPv = kP + 16, kE = kPv + 16, kDrain = kE + 8 * kEntries, kAbort = kDrain + 8,
+    static constexpr int kBarQ = kBars, kFull = kBarQ + 8, kEmpty = kFull + 8 * kSlots, kS = kEmpty + 8 * kSlots, kP = kS + 16, kPv = kP + 16, kDrain = kPv + 16, kAbort = kDrain + 8,
                          kHolder = kAbort + 4;
     static constexpr int kChunk = 512, kMeet = 1024;
     static_assert(kHolder + 4 <= kChunk && kMeet + 4 * kRows * 4 <= kQ, "head");
@@ -213,12 +228,11 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             tc::mbar_init(base + M::kEmpty + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(base + M::kS + 8 * i, 1);
+            tc::mbar_init(base + M::kS + 8 * i, 2);   // the product, and the word of the thread that issued it on the entry
             tc::mbar_init(base + M::kP + 8 * i, 8);
             tc::mbar_init(base + M::kPv + 8 * i, 1);
         }
         tc::mbar_init(base + M::kDrain, 1);
-        for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
         *abort_flag = 0;
         tc::fence_mbar_init();
     }
@@ -265,7 +279,6 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                     Entry *to = reinterpret_cast<Entry *>(sm + M::kEntriesAt) + (at / 2) % kEntries;
                     *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][x], chunk[1][x], chunk[2][x], chunk[3][x]);
                     to->block = block;
-                    tc::mbar_arrive(base + M::kE + 8 * ((at / 2) % kEntries));
                     load(&map_k, block);
                     ok = slot_free();
                     if (ok) load(&map_v, block);
@@ -273,7 +286,6 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         if (lane == 0) {
             if (ok && slot_free()) {
                 reinterpret_cast<Entry *>(sm + M::kEntriesAt)[(at / 2) % kEntries].block = -1;
-                tc::mbar_arrive(base + M::kE + 8 * ((at / 2) % kEntries));
                 tc::mbar_arrive(base + M::kFull + 8 * (at % M::kSlots));
             }
             if (*abort_flag) {   // copies in flight end before the shared memory is given back
@@ -303,7 +315,12 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             for (; ok; ++x) {
                 const uint32_t at = 2 * x, slot = at % M::kSlots;
                 ok = wait(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag);
-                if (!ok || reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries].block < 0) break;
+                if (!ok) break;
+                if (reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries].block < 0) {
+                    tc::mbar_arrive(base + M::kS + 8 * (x & 1));
+                    tc::mbar_arrive(base + M::kS + 8 * (x & 1));
+                    break;
+                }
                 // S goes where the P of two blocks ago stood: its product has ended
                 if (x >= 2 && !(ok = wait(base + M::kPv + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) break;
                 tc::tc_fence_after_sync();
@@ -312,6 +329,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                     tc::mma_f16_ss(tmem + (x & 1) * 64, tc::desc64(q_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
                                    tc::desc64(k_lo + slot * (M::kSlotBytes >> 4) + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
                 tc::mma_commit(base + M::kS + 8 * (x & 1));
+                tc::mbar_arrive(base + M::kS + 8 * (x & 1));
                 tc::mma_commit(base + M::kEmpty + 8 * slot);
                 if (x > 0) values(x - 1);
             }
@@ -331,15 +349,13 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         uint32_t x = 0;
         bool ok = true;
         for (;; ++x) {
-            ok = __all_sync(~0u, wait(base + M::kE + 8 * (x % kEntries), (x / kEntries) & 1, abort_flag));
+            ok = __all_sync(~0u, wait(base + M::kS + 8 * (x & 1), (x >> 1) & 1, abort_flag));
             if (!ok) break;
             const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries];
             const int block = e.block;
             if (block < 0) break;
             const bool listed = there && (e.rows[qx >> 5] >> (qx & 31) & 1u);
             const int n = listed ? min(kBlock, end - block * kBlock) : 0;   // keys of the row
-            ok = __all_sync(~0u, wait(base + M::kS + 8 * (x & 1), (x >> 1) & 1, abort_flag));
-            if (!ok) break;
             tc::tc_fence_after_sync();
             uint32_t u[32];
             tc::tmem_ld_x32(mine + (x & 1) * 64 + 32 * half, u);
@@ -684,13 +700,14 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 // dK, dV: a block of 64 keys of one head through the tiles of queries in which any has listed it.  Per tile S = Q K^T and dP = dO V^T as above, rows in lanes;
 // P and dS go to shared memory, where they are the operands of dV^T[d x 64] += dO^T P and dK^T += Q^T dS: contracted over the rows, all heads of the group
 // summed on the way, in the order of the tiles.  d <= 64: both at once, [dO Q]^T [P dS], whose other two quarters are not used.
-// Q and dO are double buffered (192 KB of shared memory, one CTA an SM), and so are S and dP in tensor memory: the products of the next tile run under this
-// one's exponentials.  The softmax has eight warps, two to a quarter of the rows, 32 keys each.
+// Q and dO are double buffered (192 KB of shared memory, one CTA an SM; d <= 64: four times), and so are S and dP in tensor memory: the products of the next tile
+// run under this one's exponentials.  The softmax has eight warps, two to a quarter of the rows, 32 keys each.
 template <int DP> struct GradKVSmem {
+    static constexpr int kStages = DP == 64 ? 4 : 2;
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2, kPBytes = kRows * kBlock * 2;
-    static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes, kBytes = kStage + 4 * kQBytes;   // P, dS; twice Q, dO
+    static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes, kBytes = kStage + 2 * kStages * kQBytes;   // P, dS; Q and dO of a tile kStages times
     static constexpr int kBars = kEntries * sizeof(Entry);
-    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 16, kSP = kEmpty + 16, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
+    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 8 * kStages, kSP = kEmpty + 8 * kStages, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
                          kAbort = kDrain + 8, kHolder = kAbort + 4;
     static constexpr int kChunk = 512;
     static_assert(kHolder + 4 <= kChunk && kBytes + 1024 <= 227 * 1024, "shared memory");
@@ -713,7 +730,8 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
     pdl_launch_dependents();
 
     if (threadIdx.x == 0) {
-        for (int bar : {M::kKV, M::kFull, M::kFull + 8, M::kEmpty, M::kEmpty + 8, M::kSP, M::kSP + 8, M::kDone, M::kDrain}) tc::mbar_init(base + bar, 1);
+        for (int bar : {M::kKV, M::kSP, M::kSP + 8, M::kDone, M::kDrain}) tc::mbar_init(base + bar, 1);
+        for (int i = 0; i < 2 * M::kStages; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
         tc::mbar_init(base + M::kPds, 8);
         for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
         *abort_flag = 0;
@@ -724,7 +742,7 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
         tc::tmem_relinquish();
     }
     // rows of the last places, which no copy fills, are contracted over too: zeros
-    for (int x = threadIdx.x; x < (kRows - live) * 8 * 4 * (DP / 64); x += kGradKVThreads)
+    for (int x = threadIdx.x; x < (kRows - live) * 8 * 2 * M::kStages * (DP / 64); x += kGradKVThreads)
         *reinterpret_cast<uint4 *>(sm + M::kStage + x / ((kRows - live) * 8) * (kRows * 128) + live * 128 + x % ((kRows - live) * 8) * 16) = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
     tc::tc_fence_before_sync();
@@ -770,14 +788,14 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
             if (lane == 0)
                 for (; some && ok; some &= some - 1, ++x) {
                     const int src = __ffs(some) - 1;
-                    ok = x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
+                    ok = x < (uint32_t)M::kStages || wait(base + M::kEmpty + 8 * (x % M::kStages), (x / M::kStages - 1) & 1, abort_flag);
                     if (!ok) break;
                     const int i0 = (from + src) * a.tile;
                     Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
                     *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][src], chunk[1][src], chunk[2][src], chunk[3][src]);
                     to->block = i0;
                     tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                    const uint32_t bar = base + M::kFull + 8 * (x & 1), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
+                    const uint32_t bar = base + M::kFull + 8 * (x % M::kStages), at = base + M::kStage + x % M::kStages * 2 * M::kQBytes;
                     tc::mbar_expect_tx(bar, 2 * q_bytes);
                     for (int y = 0; y < DP / 64; ++y) {
                         tc::tma_load_4d(at + y * kRows * 128, &map_q, bar, y * 64, kvh * s.group, i0, b);
@@ -786,14 +804,14 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
                 }
         }
         if (lane == 0) {
-            if (ok && (x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
+            if (ok && (x < (uint32_t)M::kStages || wait(base + M::kEmpty + 8 * (x % M::kStages), (x / M::kStages - 1) & 1, abort_flag))) {
                 reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
                 tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                tc::mbar_arrive(base + M::kFull + 8 * (x & 1));
+                tc::mbar_arrive(base + M::kFull + 8 * (x % M::kStages));
             }
             if (*abort_flag)   // copies in flight end before the shared memory is given back
-                for (uint32_t z = x > 2 ? x - 2 : 0; z < x; ++z)
-                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (z & 1), (z >> 1) & 1); ++y) {}
+                for (uint32_t z = x > (uint32_t)M::kStages ? x - M::kStages : 0; z < x; ++z)
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (z % M::kStages), (z / M::kStages) & 1); ++y) {}
             for (uint32_t y = 0; y < tc::kMaxPolls && !tc::mbar_try_wait(base + M::kKV, 0); ++y) {}   // nobody else waits for these where no tile has the block
         }
     } else if (warp == 9) {
@@ -808,7 +826,7 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
             bool ok = wait(base + M::kKV, 0, abort_flag);
             uint32_t x = 0;
             auto grads = [&](uint32_t y) {
-                const uint32_t at = (y & 1) * (2 * M::kQBytes >> 4);
+                const uint32_t at = y % M::kStages * (2 * M::kQBytes >> 4);
                 if (!(ok = ok && wait(base + M::kPds, y & 1, abort_flag))) return;
                 tc::tc_fence_after_sync();
 #pragma unroll
@@ -821,11 +839,11 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
                     }
                 }
                 tc::mma_commit(base + M::kDone);
-                tc::mma_commit(base + M::kEmpty + 8 * (y & 1));
+                tc::mma_commit(base + M::kEmpty + 8 * (y % M::kStages));
             };
             for (; ok; ++x) {
-                const uint32_t at = (x & 1) * (2 * M::kQBytes >> 4), to = tmem + (x & 1) * 128;
-                ok = wait(base + M::kFull + 8 * (x & 1), (x >> 1) & 1, abort_flag);
+                const uint32_t at = x % M::kStages * (2 * M::kQBytes >> 4), to = tmem + (x & 1) * 128;
+                ok = wait(base + M::kFull + 8 * (x % M::kStages), (x / M::kStages) & 1, abort_flag);
                 if (!ok || reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0) break;
                 tc::tc_fence_after_sync();   // S and dP go where those of two tiles ago stood: read before P and dS were said to be there
 #pragma unroll
