@@ -234,7 +234,7 @@ template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint3
     if (rc == VS_OK) rc = make_map<T>(&k, a.k, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
     if (rc == VS_OK) rc = make_map<T>(&v, a.v, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
     if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_q_kernel<T, DP>>(SmemQ::kBytes);
-    if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_kv_kernel<T, DP>>(SmemKV::kBytes + 1024);
+    if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_kv_kernel<T, DP>>(SmemKV::kBytes);
     if (rc != VS_OK) return rc;
     const int64_t rows = (int64_t)s.batch * s.queries * s.heads, tiles = query_tiles(s), blocks_all = (int64_t)s.batch * s.kv_heads * s.blocks;
     uint32_t *redo_kv = redo + tiles;
@@ -242,7 +242,7 @@ template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint3
     if (e == cudaSuccess)
         e = launch_behind(blocks::tcore::grad_q_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kGradQThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
     if (e == cudaSuccess)
-        e = launch_behind(blocks::tcore::grad_kv_kernel<T, DP>, (unsigned)blocks_all, blocks::tcore::kGradKVThreads, SmemKV::kBytes + 1024, st, a, q, g, k, v, redo_kv, status);
+        e = launch_behind(blocks::tcore::grad_kv_kernel<T, DP>, (unsigned)blocks_all, blocks::tcore::kGradKVThreads, SmemKV::kBytes, st, a, q, g, k, v, redo_kv, status);
     if (e != cudaSuccess) return (int)e;
     a.redo = redo;
     e = launch_behind(blocks::rows_kernel<T, true>, again_grid(tiles), blocks::kRowThreads, 0, st, a);

@@ -49,6 +49,21 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uin
     *abort_flag = 1;
     return false;
 }
+// The same by a whole warp, which stays together.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) { return __all_sync(~0u, wait(bar, parity, abort_flag)); }
+// One lane of a warp that is together.  The warp that issues products goes through its loop as a whole, and this lane issues: descriptors then come out of uniform
+// registers; in a loop of one lane each of their halves is moved there first, and the products wait for that.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t chosen;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(chosen));
+    return chosen != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -295,35 +310,42 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             }
         }
     } else if (warp == 9) {
-        if (lane == 0) {
-            constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescO = idesc<T>(DP, 0, 1);
-            const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
-            const uint32_t q_lo = tc::smem_desc_lo(base + M::kQ, 16), k_lo = tc::smem_desc_lo(base + M::kRing, 16);
-            const uint32_t v_lo = tc::smem_desc_lo(base + M::kRing, kBlock * 128);   // 64-dimension slabs
-            bool ok = wait(base + M::kBarQ, 0, abort_flag);
-            uint32_t x = 0;
-            auto values = [&](uint32_t y) {   // O += P V of the y-th block
-                const uint32_t at = 2 * y + 1, slot = at % M::kSlots;
-                if (!(ok = ok && wait(base + M::kP + 8 * (y & 1), (y >> 1) & 1, abort_flag) && wait(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag))) return;
-                tc::tc_fence_after_sync();
+        constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescO = idesc<T>(DP, 0, 1);
+        const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
+        const uint32_t q_lo = tc::smem_desc_lo(base + M::kQ, 16), k_lo = tc::smem_desc_lo(base + M::kRing, 16);
+        const uint32_t v_lo = tc::smem_desc_lo(base + M::kRing, kBlock * 128);   // 64-dimension slabs
+        const bool leader = elect_one();
+        bool ok = wait_all(base + M::kBarQ, 0, abort_flag);
+        uint32_t x = 0;
+        auto values = [&](uint32_t y) {   // O += P V of the y-th block
+            const uint32_t at = 2 * y + 1, slot = at % M::kSlots;
+            ok = ok && wait_all(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag) && wait_all(base + M::kP + 8 * (y & 1), (y >> 1) & 1, abort_flag);
+            if (!ok) return;
+            tc::tc_fence_after_sync();
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < kBlock / 16; ++k)
                     tc::mma_f16_ts(tmem_o, tmem + (y & 1) * 64 + 8 * k, tc::desc64(v_lo + slot * (M::kSlotBytes >> 4) + 128 * k, hi), kIdescO, y > 0 || k > 0);
                 tc::mma_commit(base + M::kPv + 8 * (y & 1));
                 tc::mma_commit(base + M::kEmpty + 8 * slot);
-            };
-            for (; ok; ++x) {
-                const uint32_t at = 2 * x, slot = at % M::kSlots;
-                ok = wait(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag);
-                if (!ok) break;
-                if (reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries].block < 0) {
+            }
+            __syncwarp();
+        };
+        for (; ok; ++x) {
+            const uint32_t at = 2 * x, slot = at % M::kSlots;
+            ok = wait_all(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag);
+            if (!ok) break;
+            if (__any_sync(~0u, reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries].block < 0)) {
+                if (leader) {
                     tc::mbar_arrive(base + M::kS + 8 * (x & 1));
                     tc::mbar_arrive(base + M::kS + 8 * (x & 1));
-                    break;
                 }
-                // S goes where the P of two blocks ago stood: its product has ended
-                if (x >= 2 && !(ok = wait(base + M::kPv + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) break;
-                tc::tc_fence_after_sync();
+                break;
+            }
+            // S goes where the P of two blocks ago stood: its product has ended
+            if (x >= 2 && !(ok = wait_all(base + M::kPv + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) break;
+            tc::tc_fence_after_sync();
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     tc::mma_f16_ss(tmem + (x & 1) * 64, tc::desc64(q_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
@@ -331,13 +353,17 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 tc::mma_commit(base + M::kS + 8 * (x & 1));
                 tc::mbar_arrive(base + M::kS + 8 * (x & 1));
                 tc::mma_commit(base + M::kEmpty + 8 * slot);
-                if (x > 0) values(x - 1);
             }
-            if (ok && x > 0) values(x - 1);
-            // what was issued ends before tensor memory is given back; normally the softmax has waited for it already
+            __syncwarp();
+            if (x > 0) values(x - 1);
+        }
+        if (ok && x > 0) values(x - 1);
+        // what was issued ends before tensor memory is given back; normally the softmax has waited for it already
+        if (leader) {
             tc::mma_commit(base + M::kDrain);
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
         }
+        __syncwarp();
     } else {
         const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane, qx = r / s.group, i = t.i0 + qx;
         float *meet = reinterpret_cast<float *>(sm + M::kMeet);   // [2][2][128]: what the two threads of a row tell each other
@@ -573,41 +599,51 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
             }
         }
     } else if (warp == 9) {
-        if (lane == 0) {
-            constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescQ = idesc<T>(DP, 0, 1);
-            const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
-            const uint32_t q_lo = tc::smem_desc_lo(base + M::kQ, 16), g_lo = tc::smem_desc_lo(base + M::kG, 16), k_lo = tc::smem_desc_lo(base + M::kK, 16);
-            const uint32_t v_lo = tc::smem_desc_lo(base + M::kV, 16), kt_lo = tc::smem_desc_lo(base + M::kK, kBlock * 128);
-            bool ok = wait(base + M::kBarQ, 0, abort_flag);
-            for (uint32_t x = 0; ok; ++x) {
-                const uint32_t slot = x & 1, at = slot * (M::kSlotBytes >> 4);
-                ok = wait(base + M::kKFull + 8 * slot, (x >> 1) & 1, abort_flag);
-                if (!ok || reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0) break;
-                if (x > 0 && !(ok = wait(base + M::kDq, (x - 1) & 1, abort_flag))) break;   // S goes where dS stood
-                tc::tc_fence_after_sync();
+        constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescQ = idesc<T>(DP, 0, 1);
+        const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
+        const uint32_t q_lo = tc::smem_desc_lo(base + M::kQ, 16), g_lo = tc::smem_desc_lo(base + M::kG, 16), k_lo = tc::smem_desc_lo(base + M::kK, 16);
+        const uint32_t v_lo = tc::smem_desc_lo(base + M::kV, 16), kt_lo = tc::smem_desc_lo(base + M::kK, kBlock * 128);
+        const bool leader = elect_one();
+        bool ok = wait_all(base + M::kBarQ, 0, abort_flag);
+        for (uint32_t x = 0; ok; ++x) {
+            const uint32_t slot = x & 1, at = slot * (M::kSlotBytes >> 4);
+            ok = wait_all(base + M::kKFull + 8 * slot, (x >> 1) & 1, abort_flag);
+            if (!ok || __any_sync(~0u, reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0)) break;
+            if (x > 0 && !(ok = wait_all(base + M::kDq, (x - 1) & 1, abort_flag))) break;   // S goes where dS stood
+            tc::tc_fence_after_sync();
+            if (leader)
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     tc::mma_f16_ss(tmem, tc::desc64(q_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
                                    tc::desc64(k_lo + at + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
-                if (!(ok = wait(base + M::kVFull, x & 1, abort_flag))) break;
-                tc::tc_fence_after_sync();
+            __syncwarp();
+            if (!(ok = wait_all(base + M::kVFull, x & 1, abort_flag))) break;
+            tc::tc_fence_after_sync();
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     tc::mma_f16_ss(tmem + 64, tc::desc64(g_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
                                    tc::desc64(v_lo + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
                 tc::mma_commit(base + M::kSP);
                 tc::mma_commit(base + M::kVEmpty);
-                if (!(ok = wait(base + M::kDs, x & 1, abort_flag))) break;
-                tc::tc_fence_after_sync();
+            }
+            __syncwarp();
+            if (!(ok = wait_all(base + M::kDs, x & 1, abort_flag))) break;
+            tc::tc_fence_after_sync();
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < kBlock / 16; ++k)
                     tc::mma_f16_ts(tmem + 128, tmem + 8 * k, tc::desc64(kt_lo + at + 128 * k, hi), kIdescQ, x > 0 || k > 0);
                 tc::mma_commit(base + M::kDq);
                 tc::mma_commit(base + M::kKEmpty + 8 * slot);
             }
+            __syncwarp();
+        }
+        if (leader) {
             tc::mma_commit(base + M::kDrain);
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
         }
+        __syncwarp();
     } else {
         const int quarter = warp & 3, half = warp >> 2;   // two warps to a quarter of the rows, 32 keys each
         const int r = quarter * 32 + lane, qx = r / s.group, i = t.i0 + qx;
@@ -700,27 +736,29 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 // dK, dV: a block of 64 keys of one head through the tiles of queries in which any has listed it.  Per tile S = Q K^T and dP = dO V^T as above, rows in lanes;
 // P and dS go to shared memory, where they are the operands of dV^T[d x 64] += dO^T P and dK^T += Q^T dS: contracted over the rows, all heads of the group
 // summed on the way, in the order of the tiles.  d <= 64: both at once, [dO Q]^T [P dS], whose other two quarters are not used.
-// Q and dO are double buffered (192 KB of shared memory, one CTA an SM; d <= 64: four times), and so are S and dP in tensor memory: the products of the next tile
-// run under this one's exponentials.  The softmax has eight warps, two to a quarter of the rows, 32 keys each.
+// Q and dO are double buffered.  d > 64: 192 KB of shared memory, one CTA an SM, S and dP double buffered in tensor memory: the products of the next tile
+// run under this one's exponentials.  d <= 64: two CTAs an SM with one buffer each, so that one begins and ends under the other's work; few tiles have listed a
+// block where a tile is 128 queries.  The softmax has eight warps, two to a quarter of the rows, 32 keys each.
 template <int DP> struct GradKVSmem {
-    static constexpr int kStages = DP == 64 ? 4 : 2;
+    static constexpr int kBuffers = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;   // of S and dP; CTAs an SM
+    static constexpr uint32_t kColumns = kBuffers * 128 + 128;   // of tensor memory: S and dP, the gradients
+    static constexpr uint32_t kAlloc = kColumns > 256 ? 512 : 256;
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2, kPBytes = kRows * kBlock * 2;
-    static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes, kBytes = kStage + 2 * kStages * kQBytes;   // P, dS; Q and dO of a tile kStages times
+    static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes, kBytes = kStage + 4 * kQBytes;   // P, dS; twice Q, dO
     static constexpr int kBars = kEntries * sizeof(Entry);
-    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 8 * kStages, kSP = kEmpty + 8 * kStages, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
+    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 16, kSP = kEmpty + 16, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
                          kAbort = kDrain + 8, kHolder = kAbort + 4;
     static constexpr int kChunk = 512;
-    static_assert(kHolder + 4 <= kChunk && kBytes + 1024 <= 227 * 1024, "shared memory");
+    static_assert(kHolder + 4 <= kChunk && kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
 };
 constexpr int kGradKVThreads = 320;
 template <typename T, int DP>
-__global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
+__global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
                                                                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, uint32_t *redo,
                                                                     uint32_t *status) {
     using M = GradKVSmem<DP>;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    const uint32_t raw = tc::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    uint8_t *sm = smem_raw + (base - raw);
+    extern __shared__ __align__(1024) uint8_t sm[];
+    const uint32_t base = tc::smem_u32(sm);
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(sm + M::kAbort);
     const Shape &s = a.s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -728,27 +766,32 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
     const int j = (int)(blockIdx.x / ((int64_t)s.batch * s.kv_heads)), kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
     const int len = s.length(b), live = a.tile * s.group;
     pdl_launch_dependents();
+    if (base & 1023u) {   // as in the kernel above
+        pdl_wait();
+        if (threadIdx.x == 0) redo[bh * s.blocks + j] = 1;
+        return;
+    }
 
     if (threadIdx.x == 0) {
         for (int bar : {M::kKV, M::kSP, M::kSP + 8, M::kDone, M::kDrain}) tc::mbar_init(base + bar, 1);
-        for (int i = 0; i < 2 * M::kStages; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
+        for (int i = 0; i < 2 * 2; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
         tc::mbar_init(base + M::kPds, 8);
         for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
         *abort_flag = 0;
         tc::fence_mbar_init();
     }
     if (warp == 9) {
-        tc::tmem_alloc(base + M::kHolder, 512);
+        tc::tmem_alloc(base + M::kHolder, M::kAlloc);
         tc::tmem_relinquish();
     }
     // rows of the last places, which no copy fills, are contracted over too: zeros
-    for (int x = threadIdx.x; x < (kRows - live) * 8 * 2 * M::kStages * (DP / 64); x += kGradKVThreads)
+    for (int x = threadIdx.x; x < (kRows - live) * 8 * 2 * 2 * (DP / 64); x += kGradKVThreads)
         *reinterpret_cast<uint4 *>(sm + M::kStage + x / ((kRows - live) * 8) * (kRows * 128) + live * 128 + x % ((kRows - live) * 8) * 16) = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
     tc::tc_fence_before_sync();
     __syncthreads();
     tc::tc_fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder), tmem_acc = tmem + 256;
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder), tmem_acc = tmem + M::kBuffers * 128;
     bool bad = false;
 
     if (warp == 8) {
@@ -788,14 +831,14 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
             if (lane == 0)
                 for (; some && ok; some &= some - 1, ++x) {
                     const int src = __ffs(some) - 1;
-                    ok = x < (uint32_t)M::kStages || wait(base + M::kEmpty + 8 * (x % M::kStages), (x / M::kStages - 1) & 1, abort_flag);
+                    ok = x < 2 || wait(base + M::kEmpty + 8 * ((x & 1)), ((x - 2) >> 1) & 1, abort_flag);
                     if (!ok) break;
                     const int i0 = (from + src) * a.tile;
                     Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
                     *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][src], chunk[1][src], chunk[2][src], chunk[3][src]);
                     to->block = i0;
                     tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                    const uint32_t bar = base + M::kFull + 8 * (x % M::kStages), at = base + M::kStage + x % M::kStages * 2 * M::kQBytes;
+                    const uint32_t bar = base + M::kFull + 8 * ((x & 1)), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
                     tc::mbar_expect_tx(bar, 2 * q_bytes);
                     for (int y = 0; y < DP / 64; ++y) {
                         tc::tma_load_4d(at + y * kRows * 128, &map_q, bar, y * 64, kvh * s.group, i0, b);
@@ -804,31 +847,32 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
                 }
         }
         if (lane == 0) {
-            if (ok && (x < (uint32_t)M::kStages || wait(base + M::kEmpty + 8 * (x % M::kStages), (x / M::kStages - 1) & 1, abort_flag))) {
+            if (ok && (x < 2 || wait(base + M::kEmpty + 8 * ((x & 1)), ((x - 2) >> 1) & 1, abort_flag))) {
                 reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
                 tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                tc::mbar_arrive(base + M::kFull + 8 * (x % M::kStages));
+                tc::mbar_arrive(base + M::kFull + 8 * ((x & 1)));
             }
             if (*abort_flag)   // copies in flight end before the shared memory is given back
-                for (uint32_t z = x > (uint32_t)M::kStages ? x - M::kStages : 0; z < x; ++z)
-                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (z % M::kStages), (z / M::kStages) & 1); ++y) {}
+                for (uint32_t z = x > 2 ? x - 2 : 0; z < x; ++z)
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * ((z & 1)), (z >> 1) & 1); ++y) {}
             for (uint32_t y = 0; y < tc::kMaxPolls && !tc::mbar_try_wait(base + M::kKV, 0); ++y) {}   // nobody else waits for these where no tile has the block
         }
     } else if (warp == 9) {
-        if (lane == 0) {
-            constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescG = idesc<T>(DP == 64 ? 2 * kBlock : kBlock, 1, 1);
-            const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
-            const uint32_t k_lo = tc::smem_desc_lo(base + M::kK, 16), v_lo = tc::smem_desc_lo(base + M::kV, 16);
-            const uint32_t q_lo = tc::smem_desc_lo(base + M::kStage, 16), g_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, 16);
-            // contracted over the rows: 64-dimension slabs; at d <= 64 Q's slab and dO's are the two halves of one operand, P and dS of the other
-            const uint32_t qt_lo = tc::smem_desc_lo(base + M::kStage, kRows * 128), gt_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, kRows * 128);
-            const uint32_t p_lo = tc::smem_desc_lo(base + M::kP, M::kPBytes), ds_lo = tc::smem_desc_lo(base + M::kP + M::kPBytes, M::kPBytes);
-            bool ok = wait(base + M::kKV, 0, abort_flag);
-            uint32_t x = 0;
-            auto grads = [&](uint32_t y) {
-                const uint32_t at = y % M::kStages * (2 * M::kQBytes >> 4);
-                if (!(ok = ok && wait(base + M::kPds, y & 1, abort_flag))) return;
-                tc::tc_fence_after_sync();
+        constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescG = idesc<T>(DP == 64 ? 2 * kBlock : kBlock, 1, 1);
+        const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
+        const uint32_t k_lo = tc::smem_desc_lo(base + M::kK, 16), v_lo = tc::smem_desc_lo(base + M::kV, 16);
+        const uint32_t q_lo = tc::smem_desc_lo(base + M::kStage, 16), g_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, 16);
+        // contracted over the rows: 64-dimension slabs; at d <= 64 Q's slab and dO's are the two halves of one operand, P and dS of the other
+        const uint32_t qt_lo = tc::smem_desc_lo(base + M::kStage, kRows * 128), gt_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, kRows * 128);
+        const uint32_t p_lo = tc::smem_desc_lo(base + M::kP, M::kPBytes), ds_lo = tc::smem_desc_lo(base + M::kP + M::kPBytes, M::kPBytes);
+        const bool leader = elect_one();
+        bool ok = wait_all(base + M::kKV, 0, abort_flag);
+        uint32_t x = 0;
+        auto grads = [&](uint32_t y) {
+            const uint32_t at = (y & 1) * (2 * M::kQBytes >> 4);
+            if (!(ok = ok && wait_all(base + M::kPds, y & 1, abort_flag))) return;
+            tc::tc_fence_after_sync();
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < kRows / 16; ++k) {
                     if constexpr (DP == 64) {   // rows of the result: Q's dimensions, then dO's; columns: with P, then with dS
@@ -839,13 +883,16 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
                     }
                 }
                 tc::mma_commit(base + M::kDone);
-                tc::mma_commit(base + M::kEmpty + 8 * (y % M::kStages));
-            };
-            for (; ok; ++x) {
-                const uint32_t at = x % M::kStages * (2 * M::kQBytes >> 4), to = tmem + (x & 1) * 128;
-                ok = wait(base + M::kFull + 8 * (x % M::kStages), (x / M::kStages) & 1, abort_flag);
-                if (!ok || reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0) break;
-                tc::tc_fence_after_sync();   // S and dP go where those of two tiles ago stood: read before P and dS were said to be there
+                tc::mma_commit(base + M::kEmpty + 8 * (y & 1));
+            }
+            __syncwarp();
+        };
+        for (; ok; ++x) {
+            const uint32_t at = (x & 1) * (2 * M::kQBytes >> 4), to = tmem + x % M::kBuffers * 128;
+            ok = wait_all(base + M::kFull + 8 * (x & 1), (x >> 1) & 1, abort_flag);
+            if (!ok || __any_sync(~0u, reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0)) break;
+            tc::tc_fence_after_sync();   // S and dP go where those of kBuffers tiles ago stood: read before P and dS were said to be there
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     tc::mma_f16_ss(to, tc::desc64(q_lo + at + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
@@ -854,13 +901,18 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
                 for (int k = 0; k < DP / 16; ++k)
                     tc::mma_f16_ss(to + 64, tc::desc64(g_lo + at + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
                                    tc::desc64(v_lo + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
-                tc::mma_commit(base + M::kSP + 8 * (x & 1));
-                if (x > 0) grads(x - 1);
+                tc::mma_commit(base + M::kSP + 8 * (x % M::kBuffers));
             }
-            if (ok && x > 0) grads(x - 1);
+            __syncwarp();
+            if (M::kBuffers == 1) grads(x);
+            else if (x > 0) grads(x - 1);
+        }
+        if (M::kBuffers == 2 && ok && x > 0) grads(x - 1);
+        if (leader) {
             tc::mma_commit(base + M::kDrain);
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
         }
+        __syncwarp();
     } else {
         const int quarter = warp & 3, half = warp >> 2;
         const int r = quarter * 32 + lane, qx = r / s.group, g = r % s.group, h = kvh * s.group + g;
@@ -884,13 +936,13 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
                 base2 = __ldcg(a.lse + row) - Lift<T>::kWeight;
                 minus_delta = -__ldcg(a.delta + row) * lift;
             }
-            ok = __all_sync(~0u, wait(base + M::kSP + 8 * (x & 1), (x >> 1) & 1, abort_flag));
+            ok = __all_sync(~0u, wait(base + M::kSP + 8 * (x % M::kBuffers), (x / M::kBuffers) & 1, abort_flag));
             if (!ok) break;
             tc::tc_fence_after_sync();
             const bool whole = __all_sync(~0u, !listed || n >= 32);   // a row that has not listed the block has no weight there: base2
             uint32_t u[32], d[32], p[16], ds[16];
-            tc::tmem_ld_x32_issue(mine + (x & 1) * 128, u);
-            tc::tmem_ld_x32_issue(mine + (x & 1) * 128 + 64, d);
+            tc::tmem_ld_x32_issue(mine + x % M::kBuffers * 128, u);
+            tc::tmem_ld_x32_issue(mine + x % M::kBuffers * 128 + 64, d);
             tc::tmem_ld_x32_wait(u);
             tc::tmem_ld_x32_wait(d);
 #pragma unroll
@@ -956,7 +1008,7 @@ __global__ void __launch_bounds__(kGradKVThreads, 1) grad_kv_kernel(const Args a
     }
     if (warp == 9) {
         tc::tc_fence_after_sync();
-        tc::tmem_dealloc(tmem, 512);
+        tc::tmem_dealloc(tmem, M::kAlloc);
     }
 }
 
