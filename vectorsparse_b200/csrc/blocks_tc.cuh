@@ -155,8 +155,8 @@ struct Scan {
         end = min(s.blocks, (s.end(last, len) + kBlock - 1) / kBlock);
         fetch(0, then);
     }
-    // The next 32 blocks' words go to `to` (a row of 32 for each of four words); false where there are no more.  One lane then goes through the chunk on its own:
-    // shuffles for each of its entries, between waits of that lane, cost the warp a thousand cycles an entry.
+    // The next 32 blocks' words go to `to` (a row of 32 for each of four words); false where there are no more.  What goes through the chunk then
+    // needs no shuffles: between waits of a single lane those cost the warp a thousand cycles an entry.
     __device__ __forceinline__ bool next(uint32_t (*to)[32], uint32_t &some) {
         if (base >= end) return false;
         const int lane = threadIdx.x & 31;
@@ -561,6 +561,7 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
                 tc::tma_load_4d(base + M::kG + x * kRows * 128, &map_g, base + M::kBarQ, x * 64, t.kvh * s.group, t.i0, t.b);
             }
         }
+        const bool leader = elect_one();
         uint32_t x = 0;
         bool ok = true;
         auto load = [&](const CUtensorMap *map, uint32_t to, uint32_t bar, int j) {
@@ -571,20 +572,22 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
         uint32_t(*chunk)[32] = reinterpret_cast<uint32_t(*)[32]>(sm + M::kChunk);
         uint32_t some;
         while (scan.next(chunk, some))
-            if (lane == 0)
-                for (; some && ok; some &= some - 1, ++x) {
-                    const int y = __ffs(some) - 1, block = scan.base - 32 + y;
-                    ok = x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
-                    if (!ok) break;
+            for (; some && ok; some &= some - 1, ++x) {
+                const int y = __ffs(some) - 1, block = scan.base - 32 + y;
+                if (!(ok = x < 2 || wait_all(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) break;
+                if (leader) {
                     Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
                     *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][y], chunk[1][y], chunk[2][y], chunk[3][y]);
                     to->block = block;
                     tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
                     load(&map_k, base + M::kK + (x & 1) * M::kSlotBytes, base + M::kKFull + 8 * (x & 1), block);
-                    ok = x < 1 || wait(base + M::kVEmpty, (x - 1) & 1, abort_flag);
-                    if (ok) load(&map_v, base + M::kV, base + M::kVFull, block);
                 }
-        if (lane == 0) {
+                __syncwarp();
+                if (!(ok = x < 1 || wait_all(base + M::kVEmpty, (x - 1) & 1, abort_flag))) break;
+                if (leader) load(&map_v, base + M::kV, base + M::kVFull, block);
+                __syncwarp();
+            }
+        if (leader) {
             if (ok && (x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
                 reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
                 tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
@@ -774,7 +777,7 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
 
     if (threadIdx.x == 0) {
         for (int bar : {M::kKV, M::kSP, M::kSP + 8, M::kDone, M::kDrain}) tc::mbar_init(base + bar, 1);
-        for (int i = 0; i < 2 * 2; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
+        for (int i = 0; i < 4; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
         tc::mbar_init(base + M::kPds, 8);
         for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
         *abort_flag = 0;
@@ -785,7 +788,7 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
         tc::tmem_relinquish();
     }
     // rows of the last places, which no copy fills, are contracted over too: zeros
-    for (int x = threadIdx.x; x < (kRows - live) * 8 * 2 * 2 * (DP / 64); x += kGradKVThreads)
+    for (int x = threadIdx.x; x < (kRows - live) * 8 * 4 * (DP / 64); x += kGradKVThreads)
         *reinterpret_cast<uint4 *>(sm + M::kStage + x / ((kRows - live) * 8) * (kRows * 128) + live * 128 + x % ((kRows - live) * 8) * 16) = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
     tc::tc_fence_before_sync();
@@ -831,14 +834,14 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
             if (lane == 0)
                 for (; some && ok; some &= some - 1, ++x) {
                     const int src = __ffs(some) - 1;
-                    ok = x < 2 || wait(base + M::kEmpty + 8 * ((x & 1)), ((x - 2) >> 1) & 1, abort_flag);
+                    ok = x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
                     if (!ok) break;
                     const int i0 = (from + src) * a.tile;
                     Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
                     *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][src], chunk[1][src], chunk[2][src], chunk[3][src]);
                     to->block = i0;
                     tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                    const uint32_t bar = base + M::kFull + 8 * ((x & 1)), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
+                    const uint32_t bar = base + M::kFull + 8 * (x & 1), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
                     tc::mbar_expect_tx(bar, 2 * q_bytes);
                     for (int y = 0; y < DP / 64; ++y) {
                         tc::tma_load_4d(at + y * kRows * 128, &map_q, bar, y * 64, kvh * s.group, i0, b);
@@ -847,14 +850,14 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
                 }
         }
         if (lane == 0) {
-            if (ok && (x < 2 || wait(base + M::kEmpty + 8 * ((x & 1)), ((x - 2) >> 1) & 1, abort_flag))) {
+            if (ok && (x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
                 reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
                 tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                tc::mbar_arrive(base + M::kFull + 8 * ((x & 1)));
+                tc::mbar_arrive(base + M::kFull + 8 * (x & 1));
             }
             if (*abort_flag)   // copies in flight end before the shared memory is given back
                 for (uint32_t z = x > 2 ? x - 2 : 0; z < x; ++z)
-                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * ((z & 1)), (z >> 1) & 1); ++y) {}
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (z & 1), (z >> 1) & 1); ++y) {}
             for (uint32_t y = 0; y < tc::kMaxPolls && !tc::mbar_try_wait(base + M::kKV, 0); ++y) {}   // nobody else waits for these where no tile has the block
         }
     } else if (warp == 9) {
