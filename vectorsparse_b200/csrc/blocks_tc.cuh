@@ -49,7 +49,21 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uin
     *abort_flag = 1;
     return false;
 }
-// The same by a whole warp, which stays together.
+// Whether a phase is over, without waiting (try_wait may: it suspends the thread where the phase is not over).
+__device__ __forceinline__ bool is_over(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// wait() by a whole warp, which stays together.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) { return __all_sync(~0u, wait(bar, parity, abort_flag)); }
 // One lane of a warp that is together.  The warp that issues products goes through its loop as a whole, and this lane issues: descriptors then come out of uniform
 // registers; in a loop of one lane each of their halves is moved there first, and the products wait for that.
@@ -870,7 +884,7 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
         const uint32_t p_lo = tc::smem_desc_lo(base + M::kP, M::kPBytes), ds_lo = tc::smem_desc_lo(base + M::kP + M::kPBytes, M::kPBytes);
         const bool leader = elect_one();
         bool ok = wait_all(base + M::kKV, 0, abort_flag);
-        uint32_t x = 0;
+        uint32_t x = 0, summed = 0;   // tiles whose scores, and whose gradients, have been issued
         auto grads = [&](uint32_t y) {
             const uint32_t at = (y & 1) * (2 * M::kQBytes >> 4);
             if (!(ok = ok && wait_all(base + M::kPds, y & 1, abort_flag))) return;
@@ -889,9 +903,14 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
                 tc::mma_commit(base + M::kEmpty + 8 * (y & 1));
             }
             __syncwarp();
+            ++summed;
         };
         for (; ok; ++x) {
             const uint32_t at = (x & 1) * (2 * M::kQBytes >> 4), to = tmem + x % M::kBuffers * 128;
+            // Where the next tile has not come yet, the gradients of the last one go first: they need not wait for it, and its place is free the sooner.
+            while (ok && summed < x && !__all_sync(~0u, is_over(base + M::kFull + 8 * (x & 1), (x >> 1) & 1)))
+                if (__all_sync(~0u, is_over(base + M::kPds, summed & 1)) || *abort_flag) grads(summed);
+            if (!ok) break;
             ok = wait_all(base + M::kFull + 8 * (x & 1), (x >> 1) & 1, abort_flag);
             if (!ok || __any_sync(~0u, reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0)) break;
             tc::tc_fence_after_sync();   // S and dP go where those of kBuffers tiles ago stood: read before P and dS were said to be there
@@ -907,10 +926,9 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
                 tc::mma_commit(base + M::kSP + 8 * (x % M::kBuffers));
             }
             __syncwarp();
-            if (M::kBuffers == 1) grads(x);
-            else if (x > 0) grads(x - 1);
+            if (M::kBuffers == 1 || summed < x) grads(summed);
         }
-        if (M::kBuffers == 2 && ok && x > 0) grads(x - 1);
+        if (ok && summed < x) grads(summed);
         if (leader) {
             tc::mma_commit(base + M::kDrain);
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
