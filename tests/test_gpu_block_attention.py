@@ -335,3 +335,52 @@ def test_refusals():
         leaves = [x.clone().requires_grad_() for x in (q, k, v)]
         g, = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 0.125).sum(), leaves[0], create_graph=True)
         g.sum().backward()
+
+
+def test_a_workspace_of_exactly_the_size_and_too_small_ones():
+    """The C entry points take the sizes that they name and refuse a byte less, before anything runs."""
+    import ctypes as C
+
+    from vectorsparse_b200 import _lib
+    q, k, v, _ = tensors(1, 130, 130, 4, 2, 64, torch.float16, 6)
+    blocks = torch_ops.select_blocks(q, k, 2)
+    want = torch_ops.selected_attention(q, k, v, blocks, 0.125)
+    n = ops.selected_attention_workspace(q, k)
+    buffer = torch.full((n + 64,), 0x5a, dtype=torch.uint8, device=DEV)
+    out, lse = torch.empty_like(q), torch.empty((1, 4, 130), dtype=torch.float32, device=DEV)
+    strides = [(C.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
+    def call(nbytes):
+        return _lib.lib().vs_selected_attention(0, 1, 130, 130, 4, 2, 64, 2, 1, q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(), strides[2], None,
+                                                blocks.data_ptr(), out.data_ptr(), None, lse.data_ptr(), C.c_float(0.125), buffer.data_ptr(), nbytes,
+                                                torch.cuda.current_stream().cuda_stream)
+    assert call(n - 1) == -3
+    assert call(n) == 0
+    assert torch.equal(out, want) and (buffer[n:] == 0x5a).all()
+
+
+def test_backward_in_a_graph_beside_an_eager_one_and_two_calls_at_once():
+    """A captured step beside an eager graph of other leaves; the same operator on two streams at once."""
+    q, k, v, grad = tensors(1, 260, 260, 4, 1, 128, torch.bfloat16, 13)
+    blocks = torch_ops.select_blocks(q, k, 3)
+    eager = [x.clone().requires_grad_() for x in (q, k, v)]
+    held = torch_ops.selected_attention(*eager, blocks, 0.1)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch_ops.selected_attention(*leaves, blocks, 0.1)
+        grads = torch.autograd.grad(out, leaves, grad)
+    graph.replay()
+    want = torch.autograd.grad(held, eager, grad)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, grads))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for _ in range(5):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                x = [t.detach().requires_grad_() for t in (q, k, v)]
+                y = torch_ops.selected_attention(*x, torch_ops.select_blocks(q, k, 3), 0.1)
+                results.append((y, *torch.autograd.grad(y, x, grad)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in results for a, b in zip(r, (held, *want)))

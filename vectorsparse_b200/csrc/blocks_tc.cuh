@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
     } else {
         const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane, qx = r / s.group, i = t.i0 + qx;
         float *meet = reinterpret_cast<float *>(sm + M::kMeet);   // [2][2][128]: what the two threads of a row tell each other
-        const bool there = r < a.tile * s.group && i < s.queries;
+        const bool there = r < a.tile * s.group && i < s.queries, alive = there && i < s.rows(t.b);   // rows behind a sequence's end have zeros, whatever stands there
         const int h = t.kvh * s.group + r % s.group, end = there ? s.end(i, len) : 0;
         const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
         const float c = a.scale * kLog2e;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries];
             const int block = e.block;
             if (block < 0) break;
-            const bool listed = there && (e.rows[qx >> 5] >> (qx & 31) & 1u);
+            const bool listed = alive && (e.rows[qx >> 5] >> (qx & 31) & 1u);
             const int n = listed ? min(kBlock, end - block * kBlock) : 0;   // keys of the row
             tc::tc_fence_after_sync();
             uint32_t u[32];
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 uint32_t o[32];
                 if (x > 0) tc::tmem_ld_x32(mine + 128 + half * (DP / 2) + 32 * g, o);
 #pragma unroll
-                for (int y = 0; y < 32; ++y) f[y] = x > 0 && total != 0.f ? __uint_as_float(o[y]) * inv : 0.f;
+                for (int y = 0; y < 32; ++y) f[y] = x > 0 && alive && total != 0.f ? __uint_as_float(o[y]) * inv : 0.f;
             };
             // the two warps of a quarter take a half of the dimensions each
             uint8_t *stage = sm + M::kQ + quarter * 32 * 128 + (DP == 128 ? half * kRows * 128 : 0);
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 float f[32];
                 result(g, f);
 #pragma unroll
-                for (int y = 0; y < 32; ++y) bad |= there && !finite(f[y]);
+                for (int y = 0; y < 32; ++y) bad |= alive && !finite(f[y]);
 #pragma unroll
                 for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
             });
@@ -486,8 +486,8 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
 #pragma unroll
                     for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
                 });
-            bad |= there && total != total;
-            if (there && half == 0) a.lse[((int64_t)t.b * s.heads + h) * s.queries + i] = total == 0.f ? INFINITY : top + log2f(total);
+            bad |= alive && total != total;
+            if (there && half == 0) a.lse[((int64_t)t.b * s.heads + h) * s.queries + i] = !alive || total == 0.f ? INFINITY : top + log2f(total);
         }
     }
     tc::tc_fence_before_sync();
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
     } else {
         const int quarter = warp & 3, half = warp >> 2;   // two warps to a quarter of the rows, 32 keys each
         const int r = quarter * 32 + lane, qx = r / s.group, i = t.i0 + qx;
-        const bool there = r < a.tile * s.group && i < s.queries;
+        const bool there = r < a.tile * s.group && i < s.queries, alive = there && i < s.rows(t.b);   // rows behind a sequence's end have zeros, whatever stands there
         const int h = t.kvh * s.group + r % s.group, end = there ? s.end(i, len) : 0;
         const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
         const float c = a.scale * kLog2e;
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
             const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm)[x % kEntries];
             const int block = e.block;
             if (block < 0) break;
-            const bool listed = there && (e.rows[qx >> 5] >> (qx & 31) & 1u);
+            const bool listed = alive && (e.rows[qx >> 5] >> (qx & 31) & 1u);
             const int n = listed ? min(kBlock, end - block * kBlock) : 0;   // keys of the row
             if (x == 0) {   // the loader has waited for the kernels that wrote these
                 lift = Lift<T>::grad(a.most);
@@ -730,8 +730,8 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
                 if (x > 0) tc::tmem_ld_x32(mine + 128 + half * (DP / 2) + 32 * g, o);
 #pragma unroll
                 for (int y = 0; y < 32; ++y) {
-                    f[y] = x > 0 ? __uint_as_float(o[y]) * back : 0.f;
-                    bad |= there && !finite(f[y]);
+                    f[y] = x > 0 && alive ? __uint_as_float(o[y]) * back : 0.f;
+                    bad |= alive && !finite(f[y]);
                 }
 #pragma unroll
                 for (int y = 0; y < 4; ++y) v[y] = pack8<T>(f + 8 * y);
