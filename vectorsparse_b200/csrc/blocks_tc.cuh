@@ -223,11 +223,14 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const float *f) {
 // two CTAs share an SM and one's products run under the other's exponentials.
 // The maximum that weights are taken relative to follows the true one only when that has grown by 2^8: weights then stay below 256, exact enough in
 // either type, and O is seldom rescaled.
+// Bound by the hand-overs between its roles: with one multiplication to a product and no exponentials an earlier form took 635 us of its 810 at 16384 x 16384,
+// 32 heads on 4, d = 128, 16 blocks each (158 000 tiles of 128 x 64).  Now 650 us: 1.02 PFLOP/s on the tiles, 0.40 on the pairs that the lists name, the unions being
+// 2.5 times as long as a list.  Two blocks to a step, and a loader that stays together as a warp, were slower.
 constexpr float kSlack = 8.f;
 template <int DP> struct ForwardSmem {
     static constexpr int kSlots = DP == 128 ? 4 : 6;
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
-    static constexpr int kQ = 3072, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // ahead: entries, barriers, a chunk of the scan, 2 KB for the rows' threads
+    static constexpr int kQ = 3 * 1024, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // ahead: entries, barriers, a chunk of the scan, 2 KB for the rows' threads
     static constexpr int kEntriesAt = 0, kBars = kEntries * sizeof(Entry);
     static constexpr int kBarQ = kBars, kFull = kBarQ + 8, kEmpty = kFull + 8 * kSlots, kS = kEmpty + 8 * kSlots, kP = kS + 16, kPv = kP + 16, kDrain = kPv + 16, kAbort = kDrain + 8,
                          kHolder = kAbort + 4;
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
 // Weights and the scores' gradients are rounded to 16 bits for their products.  fp16 keeps its precision only above 2^-14, so there both are multiplied by powers of
-// two first: the weights, at most 1, by 2^14; the gradients by the one that brings the largest element of grad_out to 1 .. 2 (found by the delta kernel).
+// two first: the weights, at most 1, by 2^14; the gradients by the one that brings the largest element of grad_out to 32 .. 64 (found by the delta kernel).
 template <typename T> struct Lift {
     static constexpr float kWeight = std::is_same<T, __half>::value ? 14.f : 0.f;   // exponent
     static __device__ __forceinline__ float grad(const uint32_t *most) {
@@ -518,6 +521,7 @@ __device__ __forceinline__ float exp2i(float e) { return __uint_as_float((uint32
 // dQ: a tile of queries through the union of its lists, as forward.  Per block S = Q K^T and dP = dO V^T, dS = P (dP - delta) back into S's place as an operand,
 // dQ += dS K with the same keys, now contracted over.  Keys are double buffered, values not: their place is free once dP is there, long before the
 // next ones are needed.  256 columns of tensor memory, 113 KB of shared memory (d = 128): two CTAs an SM, one's products under the other's exponentials.
+// Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 500 us, 0.89 PFLOP/s on them.
 template <int DP> struct GradQSmem {
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
     static constexpr int kQ = 1024, kG = kQ + kQBytes, kK = kG + kQBytes, kV = kK + 2 * kSlotBytes, kBytes = kV + kSlotBytes;
@@ -756,6 +760,8 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 // Q and dO are double buffered.  d > 64: 192 KB of shared memory, one CTA an SM, S and dP double buffered in tensor memory: the products of the next tile
 // run under this one's exponentials.  d <= 64: two CTAs an SM with one buffer each, so that one begins and ends under the other's work; few tiles have listed a
 // block where a tile is 128 queries.  The softmax has eight warps, two to a quarter of the rows, 32 keys each.
+// Bound by the hand-overs through shared memory (P and dS are written and waited for before the second products): the tiles above take 938 us, 0.63 PFLOP/s on them;
+// 16 warps for the softmax 933.  A block that all later queries have listed (up to 392 tiles there, 138 on average) is one CTA's work and starts first.
 template <int DP> struct GradKVSmem {
     static constexpr int kBuffers = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;   // of S and dP; CTAs an SM
     static constexpr uint32_t kColumns = kBuffers * 128 + 128;   // of tensor memory: S and dP, the gradients
