@@ -242,7 +242,7 @@ template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint3
     if (e == cudaSuccess)
         e = launch_behind(blocks::tcore::grad_q_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kGradQThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
     if (e == cudaSuccess)
-        e = launch_behind(blocks::tcore::grad_kv_kernel<T, DP>, (unsigned)blocks_all, blocks::tcore::kGradKVThreads, SmemKV::kBytes, st, a, q, g, k, v, redo_kv, status);
+        e = launch_behind(blocks::tcore::grad_kv_kernel<T, DP>, (unsigned)blocks_all, SmemKV::kThreads, SmemKV::kBytes, st, a, q, g, k, v, redo_kv, status);
     if (e != cudaSuccess) return (int)e;
     a.redo = redo;
     e = launch_behind(blocks::rows_kernel<T, true>, again_grid(tiles), blocks::kRowThreads, 0, st, a);

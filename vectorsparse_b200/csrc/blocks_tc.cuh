@@ -49,19 +49,26 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uin
     *abort_flag = 1;
     return false;
 }
-// Whether a phase is over, without waiting (try_wait may: it suspends the thread where the phase is not over).
-__device__ __forceinline__ bool is_over(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
+// Whether phases are over, without waiting (try_wait may: it suspends the thread where the phase is not over).  Three at once, as bits: an answer takes some 300 cycles under the copies' and products' traffic, and they come together.
+__device__ __forceinline__ uint32_t are_over(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, uint32_t bar2, uint32_t parity2) {
+    uint32_t bits;
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, q, r;\n"
+        ".reg .b32 x, y;\n"
         "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 r, [%5], %6;\n"
         "selp.u32 %0, 1, 0, p;\n"
+        "selp.u32 x, 2, 0, q;\n"
+        "selp.u32 y, 4, 0, r;\n"
+        "or.b32 %0, %0, x;\n"
+        "or.b32 %0, %0, y;\n"
         "}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
+        : "=&r"(bits)
+        : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1), "r"(bar2), "r"(parity2)
         : "memory");
-    return ok != 0;
+    return bits;
 }
 // wait() by a whole warp, which stays together.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) { return __all_sync(~0u, wait(bar, parity, abort_flag)); }
@@ -764,19 +771,22 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 // 16 warps for the softmax 933.  A block that all later queries have listed (up to 392 tiles there, 138 on average) is one CTA's work and starts first.
 template <int DP> struct GradKVSmem {
     static constexpr int kBuffers = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;   // of S and dP; CTAs an SM
+    // Q and dO of tile x are copies 2 x and 2 x + 1, copy n in place n % kPlaces; d <= 64: always Q in an even one, dO behind it
+    static constexpr uint32_t kPlaces = DP == 64 ? 4 : 5;
+    static constexpr int kGroups = DP == 64 ? 1 : 2, kThreads = 64 + 256 * kGroups;   // of eight softmax warps, which take turns
     static constexpr uint32_t kColumns = kBuffers * 128 + 128;   // of tensor memory: S and dP, the gradients
     static constexpr uint32_t kAlloc = kColumns > 256 ? 512 : 256;
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2, kPBytes = kRows * kBlock * 2;
-    static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes, kBytes = kStage + 4 * kQBytes;   // P, dS; twice Q, dO
+    static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes,   // P, dS; places for Q and dO
+                         kBytes = kStage + kPlaces * kQBytes;
     static constexpr int kBars = kEntries * sizeof(Entry);
-    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 16, kSP = kEmpty + 16, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
+    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 8 * kPlaces, kSP = kEmpty + 8 * kPlaces, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
                          kAbort = kDrain + 8, kHolder = kAbort + 4;
     static constexpr int kChunk = 512;
     static_assert(kHolder + 4 <= kChunk && kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
 };
-constexpr int kGradKVThreads = 320;
 template <typename T, int DP>
-__global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
+__global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCtas) grad_kv_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
                                                                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, uint32_t *redo,
                                                                     uint32_t *status) {
     using M = GradKVSmem<DP>;
@@ -797,7 +807,7 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
 
     if (threadIdx.x == 0) {
         for (int bar : {M::kKV, M::kSP, M::kSP + 8, M::kDone, M::kDrain}) tc::mbar_init(base + bar, 1);
-        for (int i = 0; i < 4; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
+        for (uint32_t i = 0; i < 2 * M::kPlaces; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
         tc::mbar_init(base + M::kPds, 8);
         for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
         *abort_flag = 0;
@@ -808,7 +818,7 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
         tc::tmem_relinquish();
     }
     // rows of the last places, which no copy fills, are contracted over too: zeros
-    for (int x = threadIdx.x; x < (kRows - live) * 8 * 4 * (DP / 64); x += kGradKVThreads)
+    for (int x = threadIdx.x; x < (kRows - live) * 8 * (int)M::kPlaces * (DP / 64); x += M::kThreads)
         *reinterpret_cast<uint4 *>(sm + M::kStage + x / ((kRows - live) * 8) * (kRows * 128) + live * 128 + x % ((kRows - live) * 8) * 16) = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
     tc::tc_fence_before_sync();
@@ -841,8 +851,9 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
                               : 0u;
         };
         uint32_t(*chunk)[32] = reinterpret_cast<uint32_t(*)[32]>(sm + M::kChunk);
-        uint32_t x = 0;
+        uint32_t x = 0, copies = 0;
         bool ok = true;
+        auto free = [&](uint32_t n) { return n < M::kPlaces || wait(base + M::kEmpty + 8 * (n % M::kPlaces), (n / M::kPlaces - 1) & 1, abort_flag); };
         fetch(shown);
         for (int from = shown; from < tiles; from += 32) {   // as Scan::next
             __syncwarp();
@@ -854,115 +865,162 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
             if (lane == 0)
                 for (; some && ok; some &= some - 1, ++x) {
                     const int src = __ffs(some) - 1;
-                    ok = x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag);
-                    if (!ok) break;
                     const int i0 = (from + src) * a.tile;
+                    auto copy = [&](const CUtensorMap *map, uint32_t n) {
+                        const uint32_t bar = base + M::kFull + 8 * (n % M::kPlaces), at = base + M::kStage + n % M::kPlaces * M::kQBytes;
+                        tc::mbar_expect_tx(bar, q_bytes);
+                        for (int y = 0; y < DP / 64; ++y) tc::tma_load_4d(at + y * kRows * 128, map, bar, y * 64, kvh * s.group, i0, b);
+                    };
+                    if (!(ok = free(2 * x))) break;
                     Entry *to = reinterpret_cast<Entry *>(sm) + x % kEntries;
                     *reinterpret_cast<uint4 *>(to->rows) = make_uint4(chunk[0][src], chunk[1][src], chunk[2][src], chunk[3][src]);
                     to->block = i0;
                     tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                    const uint32_t bar = base + M::kFull + 8 * (x & 1), at = base + M::kStage + (x & 1) * 2 * M::kQBytes;
-                    tc::mbar_expect_tx(bar, 2 * q_bytes);
-                    for (int y = 0; y < DP / 64; ++y) {
-                        tc::tma_load_4d(at + y * kRows * 128, &map_q, bar, y * 64, kvh * s.group, i0, b);
-                        tc::tma_load_4d(at + M::kQBytes + y * kRows * 128, &map_g, bar, y * 64, kvh * s.group, i0, b);
-                    }
+                    copy(&map_q, 2 * x);
+                    copies = 2 * x + 1;
+                    if (!(ok = free(2 * x + 1))) break;
+                    copy(&map_g, 2 * x + 1);
+                    copies = 2 * x + 2;
                 }
         }
         if (lane == 0) {
-            if (ok && (x < 2 || wait(base + M::kEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
-                reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
-                tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
-                tc::mbar_arrive(base + M::kFull + 8 * (x & 1));
+            if (ok && free(2 * x) && free(2 * x + 1)) {
+                for (uint32_t y = x; y < x + M::kGroups; ++y) {   // the end, for each group, with the number of tiles
+                    Entry *to = reinterpret_cast<Entry *>(sm) + y % kEntries;
+                    to->rows[0] = x;
+                    to->block = -1;
+                    tc::mbar_arrive(base + M::kE + 8 * (y % kEntries));
+                }
+                tc::mbar_arrive(base + M::kFull + 8 * (2 * x % M::kPlaces));
+                tc::mbar_arrive(base + M::kFull + 8 * ((2 * x + 1) % M::kPlaces));
             }
             if (*abort_flag)   // copies in flight end before the shared memory is given back
-                for (uint32_t z = x > 2 ? x - 2 : 0; z < x; ++z)
-                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (z & 1), (z >> 1) & 1); ++y) {}
+                for (uint32_t n = copies > M::kPlaces ? copies - M::kPlaces : 0; n < copies; ++n)
+                    for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kFull + 8 * (n % M::kPlaces), (n / M::kPlaces) & 1); ++y) {}
             for (uint32_t y = 0; y < tc::kMaxPolls && !tc::mbar_try_wait(base + M::kKV, 0); ++y) {}   // nobody else waits for these where no tile has the block
         }
     } else if (warp == 9) {
         constexpr uint32_t kIdescS = idesc<T>(kBlock, 0, 0), kIdescG = idesc<T>(DP == 64 ? 2 * kBlock : kBlock, 1, 1);
         const uint32_t hi = tc::smem_desc_hi(1024, (uint32_t)tc::kSwizzle128B);
         const uint32_t k_lo = tc::smem_desc_lo(base + M::kK, 16), v_lo = tc::smem_desc_lo(base + M::kV, 16);
-        const uint32_t q_lo = tc::smem_desc_lo(base + M::kStage, 16), g_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, 16);
+        const uint32_t q_lo = tc::smem_desc_lo(base + M::kStage, 16);
         // contracted over the rows: 64-dimension slabs; at d <= 64 Q's slab and dO's are the two halves of one operand, P and dS of the other
-        const uint32_t qt_lo = tc::smem_desc_lo(base + M::kStage, kRows * 128), gt_lo = tc::smem_desc_lo(base + M::kStage + M::kQBytes, kRows * 128);
+        const uint32_t qt_lo = tc::smem_desc_lo(base + M::kStage, kRows * 128);
         const uint32_t p_lo = tc::smem_desc_lo(base + M::kP, M::kPBytes), ds_lo = tc::smem_desc_lo(base + M::kP + M::kPBytes, M::kPBytes);
         const bool leader = elect_one();
         bool ok = wait_all(base + M::kKV, 0, abort_flag);
-        uint32_t x = 0, summed = 0;   // tiles whose scores, and whose gradients, have been issued
-        auto grads = [&](uint32_t y) {
-            const uint32_t at = (y & 1) * (2 * M::kQBytes >> 4);
-            if (!(ok = ok && wait_all(base + M::kPds, y & 1, abort_flag))) return;
-            tc::tc_fence_after_sync();
-            if (leader) {
-#pragma unroll
-                for (int k = 0; k < kRows / 16; ++k) {
-                    if constexpr (DP == 64) {   // rows of the result: Q's dimensions, then dO's; columns: with P, then with dS
-                        tc::mma_f16_ss(tmem_acc, tc::desc64(qt_lo + at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, y > 0 || k > 0);
-                    } else {
-                        tc::mma_f16_ss(tmem_acc, tc::desc64(gt_lo + at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, y > 0 || k > 0);
-                        tc::mma_f16_ss(tmem_acc + 64, tc::desc64(qt_lo + at + 128 * k, hi), tc::desc64(ds_lo + 128 * k, hi), kIdescG, y > 0 || k > 0);
-                    }
-                }
-                tc::mma_commit(base + M::kDone);
-                tc::mma_commit(base + M::kEmpty + 8 * (y & 1));
+        uint32_t scored = 0, summed = 0, idle = 0;   // tiles whose scores, and whose gradients, have been issued
+        bool last = false;
+        struct Turn {   // place and phase of a copy: counted on, not divided, so that they and the descriptors made of them stay in uniform registers
+            uint32_t place, phase;
+            __device__ void next() {
+                place += 2;
+                if (place >= M::kPlaces) place -= M::kPlaces, phase ^= 1;
             }
-            __syncwarp();
-            ++summed;
+        } q_turn = {0, 0}, g_turn = {1, 0}, q_sum = {0, 0}, g_sum = {1, 0};
+        auto product = [&](uint32_t at, uint32_t to, uint32_t with) {   // S or dP: rows of a copy times the keys or values
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+                tc::mma_f16_ss(to, tc::desc64(at + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi), tc::desc64(with + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi),
+                               kIdescS, k > 0);
         };
-        for (; ok; ++x) {
-            const uint32_t at = (x & 1) * (2 * M::kQBytes >> 4), to = tmem + x % M::kBuffers * 128;
-            // Where the next tile has not come yet, the gradients of the last one go first: they need not wait for it, and its place is free the sooner.
-            while (ok && summed < x && !__all_sync(~0u, is_over(base + M::kFull + 8 * (x & 1), (x >> 1) & 1)))
-                if (__all_sync(~0u, is_over(base + M::kPds, summed & 1)) || *abort_flag) grads(summed);
-            if (!ok) break;
-            ok = wait_all(base + M::kFull + 8 * (x & 1), (x >> 1) & 1, abort_flag);
-            if (!ok || __any_sync(~0u, reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0)) break;
-            tc::tc_fence_after_sync();   // S and dP go where those of kBuffers tiles ago stood: read before P and dS were said to be there
-            if (leader) {
+        // Whichever can go goes: gradients first, for they free places.  S and dP go where those of kBuffers tiles ago stood, which were read before P and dS were
+        // said to be there.
+        while (ok && !(last && summed == scored)) {
+            const uint32_t over = __reduce_and_sync(~0u, are_over(base + M::kPds, summed & 1, base + M::kFull + 8 * q_turn.place, q_turn.phase,
+                                                                  base + M::kFull + 8 * g_turn.place, g_turn.phase));
+            if (summed < scored && (over & 1)) {
+                tc::tc_fence_after_sync();
+                if (leader) {
+                    const uint32_t q_at = qt_lo + q_sum.place * (M::kQBytes >> 4), g_at = qt_lo + g_sum.place * (M::kQBytes >> 4);
+                    if constexpr (DP == 64) {   // rows of the result: Q's dimensions, then dO's; columns: with P, then with dS
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k)
-                    tc::mma_f16_ss(to, tc::desc64(q_lo + at + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
-                                   tc::desc64(k_lo + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
+                        for (int k = 0; k < kRows / 16; ++k)
+                            tc::mma_f16_ss(tmem_acc, tc::desc64(q_at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, summed > 0 || k > 0);
+                    } else {
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k)
-                    tc::mma_f16_ss(to + 64, tc::desc64(g_lo + at + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
-                                   tc::desc64(v_lo + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
-                tc::mma_commit(base + M::kSP + 8 * (x % M::kBuffers));
+                        for (int k = 0; k < kRows / 16; ++k)
+                            tc::mma_f16_ss(tmem_acc + 64, tc::desc64(q_at + 128 * k, hi), tc::desc64(ds_lo + 128 * k, hi), kIdescG, summed > 0 || k > 0);
+                        tc::mma_commit(base + M::kEmpty + 8 * q_sum.place);
+#pragma unroll
+                        for (int k = 0; k < kRows / 16; ++k)
+                            tc::mma_f16_ss(tmem_acc, tc::desc64(g_at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, summed > 0 || k > 0);
+                    }
+                    tc::mma_commit(base + M::kDone);
+                    if (DP == 64) tc::mma_commit(base + M::kEmpty + 8 * q_sum.place);
+                    tc::mma_commit(base + M::kEmpty + 8 * g_sum.place);
+                }
+                __syncwarp();
+                ++summed;
+                q_sum.next();
+                g_sum.next();
+            } else if (!last && scored < summed + M::kBuffers && over >= 6) {
+                last = __any_sync(~0u, reinterpret_cast<volatile Entry *>(sm)[scored % kEntries].block < 0);
+                if (!last) {
+                    tc::tc_fence_after_sync();
+                    if (leader) {
+                        product(q_lo + q_turn.place * (M::kQBytes >> 4), tmem + scored % M::kBuffers * 128, k_lo);
+                        product(q_lo + g_turn.place * (M::kQBytes >> 4), tmem + scored % M::kBuffers * 128 + 64, v_lo);
+                        tc::mma_commit(base + M::kSP + 8 * (scored % M::kBuffers));
+                    }
+                    __syncwarp();
+                    ++scored;
+                    q_turn.next();
+                    g_turn.next();
+                }
+            } else {
+                if (++idle == kMaxPolls) *abort_flag = 1;
+                ok = !__any_sync(~0u, *abort_flag != 0);
+                continue;
             }
-            __syncwarp();
-            if (M::kBuffers == 1 || summed < x) grads(summed);
+            idle = 0;
         }
-        if (ok && summed < x) grads(summed);
         if (leader) {
             tc::mma_commit(base + M::kDrain);
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
         }
         __syncwarp();
     } else {
-        const int quarter = warp & 3, half = warp >> 2;
+        const int group = warp > 9, quarter = warp & 3, half = (group ? warp - 10 : warp) >> 2;
         const int r = quarter * 32 + lane, qx = r / s.group, g = r % s.group, h = kvh * s.group + g;
         const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + 32 * half;
         const float c = a.scale * kLog2e;
         float lift = 1.f;
-        uint32_t x = 0;
+        uint32_t x = group, total = 0;
         bool ok = true;
-        for (;; ++x) {
-            ok = __all_sync(~0u, wait(base + M::kE + 8 * (x % kEntries), (x / kEntries) & 1, abort_flag));
-            if (!ok) break;
-            const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm)[x % kEntries];
+        // what a row has in a tile; its two numbers come from L2 and are asked for before its scores are waited for
+        struct Row {
+            bool listed;
+            int n;   // keys of the row from this warp's first on
+            float lse, delta;
+        } next;
+        bool more = false;
+        auto look = [&](uint32_t y) {   // the row of tile y into `next`
+            ok = __all_sync(~0u, wait(base + M::kE + 8 * (y % kEntries), (y / kEntries) & 1, abort_flag));
+            if (!ok) return;
+            const volatile Entry &e = reinterpret_cast<volatile Entry *>(sm)[y % kEntries];
             const int i0 = e.block, i = i0 + qx;
-            if (i0 < 0) break;
-            if (x == 0) lift = Lift<T>::grad(a.most) * exp2i(-Lift<T>::kWeight);   // the loader has waited for the kernels that wrote it
-            const bool listed = r < live && i < s.queries && (e.rows[qx >> 5] >> (qx & 31) & 1u);
-            const int n = listed ? min(kBlock, s.end(i, len) - j * kBlock) - 32 * half : 0;   // keys of the row from this warp's first on
-            float base2 = INFINITY, minus_delta = 0.f;
-            if (listed) {
-                const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
-                base2 = __ldcg(a.lse + row) - Lift<T>::kWeight;
-                minus_delta = -__ldcg(a.delta + row) * lift;
+            more = i0 >= 0;
+            if (!more) {
+                total = e.rows[0];
+                return;
             }
+            next.listed = r < live && i < s.queries && (e.rows[qx >> 5] >> (qx & 31) & 1u);
+            next.n = next.listed ? min(kBlock, s.end(i, len) - j * kBlock) - 32 * half : 0;
+            next.lse = INFINITY;
+            next.delta = 0.f;
+            if (next.listed) {
+                const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+                next.lse = __ldcg(a.lse + row);
+                next.delta = __ldcg(a.delta + row);
+            }
+        };
+        look(x);
+        if (ok && more) lift = Lift<T>::grad(a.most) * exp2i(-Lift<T>::kWeight);   // the loader has waited for the kernels that wrote it
+        for (; ok && more; x += M::kGroups) {
+            const bool listed = next.listed;
+            const int n = next.n;
+            const float base2 = next.lse - Lift<T>::kWeight, minus_delta = -next.delta * lift;
             ok = __all_sync(~0u, wait(base + M::kSP + 8 * (x % M::kBuffers), (x / M::kBuffers) & 1, abort_flag));
             if (!ok) break;
             tc::tc_fence_after_sync();
@@ -997,13 +1055,14 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
             tc::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(base + M::kPds);
+            look(x + M::kGroups);
         }
-        if (ok && x > 0) ok = __all_sync(~0u, wait(base + M::kDone, (x - 1) & 1, abort_flag));
-        if (ok) {
+        if (ok && total > 0) ok = __all_sync(~0u, wait(base + M::kDone, (total - 1) & 1, abort_flag));
+        if (ok && group == 0) {
             // accumulators: a dimension to a lane, keys in columns.  d > 64: dV in columns 0 .. 63, dK in 64 ..; d <= 64: dK in lanes 0 .. 63 of columns 64 ..,
             // dV in lanes 64 .. of columns 0 ..  The two halves of the warps take one of the two each, or 32 keys each.
             tc::tc_fence_after_sync();
-            const float back_v = exp2i(-Lift<T>::kWeight), back_k = x > 0 ? a.scale / (lift * exp2i(Lift<T>::kWeight)) : 0.f;
+            const float back_v = exp2i(-Lift<T>::kWeight), back_k = total > 0 ? a.scale / (lift * exp2i(Lift<T>::kWeight)) : 0.f;
             const uint32_t lanes = tmem_acc + ((uint32_t)(quarter * 32) << 16);
             const bool is_k = DP == 64 ? quarter < 2 : half == 1;
             const int dim = (DP == 64 ? quarter % 2 : quarter) * 32 + lane;
@@ -1015,10 +1074,10 @@ __global__ void __launch_bounds__(kGradKVThreads, DP == 64 ? 2 : 1) grad_kv_kern
             for (int part = 0; part < (DP == 64 ? 1 : 2); ++part) {
                 const int first = DP == 64 ? 32 * half : 32 * part;
                 uint32_t o[32];
-                if (x > 0) tc::tmem_ld_x32(lanes + (is_k ? 64 : 0) + first, o);
+                if (total > 0) tc::tmem_ld_x32(lanes + (is_k ? 64 : 0) + first, o);
 #pragma unroll
                 for (int y = 0; y < 32; ++y) {
-                    const float f = x > 0 ? __uint_as_float(o[y]) * back : 0.f;
+                    const float f = total > 0 ? __uint_as_float(o[y]) * back : 0.f;
                     if (dim < s.d && first + y < keys) {
                         bad |= !finite(f);
                         out[(first + y) * pitch] = from_f32<T>(f);
