@@ -70,6 +70,31 @@ __device__ __forceinline__ uint32_t are_over(uint32_t bar0, uint32_t parity0, ui
         : "memory");
     return bits;
 }
+// Waits for three phases at once by a whole warp, which stays together: their answers come together, as above.  What the phases guard is read behind this alone: a load
+// next to these instructions does not wait for their answers.
+__device__ __forceinline__ bool wait_three(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, uint32_t bar2, uint32_t parity2, volatile uint32_t *abort_flag) {
+    bool ok = false;
+    for (uint32_t i = 0; i < kMaxPolls && !ok; ++i) {
+        uint32_t over;
+        asm volatile(
+            "{\n"
+            ".reg .pred p, q, r;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n"
+            "and.pred p, p, q;\n"
+            "and.pred p, p, r;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(over)
+            : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1), "r"(bar2), "r"(parity2)
+            : "memory");
+        ok = over != 0;
+        if (!ok && *abort_flag) break;
+    }
+    if (!ok) *abort_flag = 1;
+    return __all_sync(~0u, ok);
+}
 // wait() by a whole warp, which stays together.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) { return __all_sync(~0u, wait(bar, parity, abort_flag)); }
 // One lane of a warp that is together.  The warp that issues products goes through its loop as a whole, and this lane issues: descriptors then come out of uniform
@@ -231,8 +256,8 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const float *f) {
 // The maximum that weights are taken relative to follows the true one only when that has grown by 2^8: weights then stay below 256, exact enough in
 // either type, and O is seldom rescaled.
 // Bound by the hand-overs between its roles: with one multiplication to a product and no exponentials an earlier form took 635 us of its 810 at 16384 x 16384,
-// 32 heads on 4, d = 128, 16 blocks each (158 000 tiles of 128 x 64).  Now 650 us: 1.02 PFLOP/s on the tiles, 0.40 on the pairs that the lists name, the unions being
-// 2.5 times as long as a list.  Two blocks to a step, and a loader that stays together as a warp, were slower.
+// 32 heads on 4, d = 128, 16 blocks each (158 000 tiles of 128 x 64).  Now 637 us: 1.04 PFLOP/s on the tiles, 0.41 on the pairs that the lists name, the unions being
+// 2.5 times as long as a list.  The waits of a step's products taken together: 652 before.  Two blocks to a step, and a loader that stays together as a warp, were slower.
 constexpr float kSlack = 8.f;
 template <int DP> struct ForwardSmem {
     static constexpr int kSlots = DP == 128 ? 4 : 6;
@@ -287,9 +312,9 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
     bool bad = false;
     pdl_launch_dependents();
 
+    pdl_wait();   // all roles: the bounded waits below are for this kernel's own work, not for that of kernels before it
     if (warp == 8) {
         // loader: position 2 x holds the keys, 2 x + 1 the values of the x-th block
-        pdl_wait();   // the bits are the kernel's before
         const uint32_t q_bytes = (uint32_t)(a.tile * s.group * 128 * (DP / 64));
         if (lane == 0) {
             tc::mbar_expect_tx(base + M::kBarQ, q_bytes);
@@ -343,7 +368,8 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         uint32_t x = 0;
         auto values = [&](uint32_t y) {   // O += P V of the y-th block
             const uint32_t at = 2 * y + 1, slot = at % M::kSlots;
-            ok = ok && wait_all(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag) && wait_all(base + M::kP + 8 * (y & 1), (y >> 1) & 1, abort_flag);
+            const uint32_t p_bar = base + M::kP + 8 * (y & 1), p_phase = (y >> 1) & 1;
+            ok = ok && wait_three(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, p_bar, p_phase, p_bar, p_phase, abort_flag);
             if (!ok) return;
             tc::tc_fence_after_sync();
             if (leader) {
@@ -357,7 +383,9 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         };
         for (; ok; ++x) {
             const uint32_t at = 2 * x, slot = at % M::kSlots;
-            ok = wait_all(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, abort_flag);
+            // S goes where the P of two blocks ago stood: its product has ended (of a barrier without a phase yet the one before its first is over)
+            const uint32_t pv_bar = base + M::kPv + 8 * (x & 1), pv_phase = ((x - 2) >> 1) & 1;
+            ok = wait_three(base + M::kFull + 8 * slot, (at / M::kSlots) & 1, pv_bar, pv_phase, pv_bar, pv_phase, abort_flag);
             if (!ok) break;
             if (__any_sync(~0u, reinterpret_cast<volatile Entry *>(sm + M::kEntriesAt)[x % kEntries].block < 0)) {
                 if (leader) {
@@ -366,8 +394,6 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
                 }
                 break;
             }
-            // S goes where the P of two blocks ago stood: its product has ended
-            if (x >= 2 && !(ok = wait_all(base + M::kPv + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) break;
             tc::tc_fence_after_sync();
             if (leader) {
 #pragma unroll
@@ -528,7 +554,8 @@ __device__ __forceinline__ float exp2i(float e) { return __uint_as_float((uint32
 // dQ: a tile of queries through the union of its lists, as forward.  Per block S = Q K^T and dP = dO V^T, dS = P (dP - delta) back into S's place as an operand,
 // dQ += dS K with the same keys, now contracted over.  Keys are double buffered, values not: their place is free once dP is there, long before the
 // next ones are needed.  256 columns of tensor memory, 113 KB of shared memory (d = 128): two CTAs an SM, one's products under the other's exponentials.
-// Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 500 us, 0.89 PFLOP/s on them.
+// Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 476 us, 0.94 PFLOP/s on them
+// (500 with one wait after another).
 template <int DP> struct GradQSmem {
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
     static constexpr int kQ = 1024, kG = kQ + kQBytes, kK = kG + kQBytes, kV = kK + 2 * kSlotBytes, kBytes = kV + kSlotBytes;
@@ -576,8 +603,8 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder);
     bool bad = false;
 
+    pdl_wait();   // all roles: the bounded waits below are for this kernel's own work, not for that of kernels before it
     if (warp == 8) {
-        pdl_wait();
         const uint32_t q_bytes = (uint32_t)(a.tile * s.group * 128 * (DP / 64));
         if (lane == 0) {
             tc::mbar_expect_tx(base + M::kBarQ, 2 * q_bytes);
@@ -613,10 +640,11 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
                 __syncwarp();
             }
         if (leader) {
-            if (ok && (x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag))) {
+            if (ok && (x < 2 || wait(base + M::kKEmpty + 8 * (x & 1), ((x - 2) >> 1) & 1, abort_flag)) && (x < 1 || wait(base + M::kVEmpty, (x - 1) & 1, abort_flag))) {
                 reinterpret_cast<Entry *>(sm)[x % kEntries].block = -1;
                 tc::mbar_arrive(base + M::kE + 8 * (x % kEntries));
                 tc::mbar_arrive(base + M::kKFull + 8 * (x & 1));
+                tc::mbar_arrive(base + M::kVFull);
             }
             if (*abort_flag) {   // copies in flight end before the shared memory is given back
                 for (uint32_t y = 0; y < 1024 && !tc::mbar_try_wait(base + M::kBarQ, 0); ++y) {}
@@ -635,19 +663,15 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
         bool ok = wait_all(base + M::kBarQ, 0, abort_flag);
         for (uint32_t x = 0; ok; ++x) {
             const uint32_t slot = x & 1, at = slot * (M::kSlotBytes >> 4);
-            ok = wait_all(base + M::kKFull + 8 * slot, (x >> 1) & 1, abort_flag);
+            // S goes where dS stood (of a barrier without a phase yet the one before its first is over)
+            ok = wait_three(base + M::kKFull + 8 * slot, (x >> 1) & 1, base + M::kDq, (x - 1) & 1, base + M::kVFull, x & 1, abort_flag);
             if (!ok || __any_sync(~0u, reinterpret_cast<volatile Entry *>(sm)[x % kEntries].block < 0)) break;
-            if (x > 0 && !(ok = wait_all(base + M::kDq, (x - 1) & 1, abort_flag))) break;   // S goes where dS stood
             tc::tc_fence_after_sync();
-            if (leader)
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     tc::mma_f16_ss(tmem, tc::desc64(q_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
                                    tc::desc64(k_lo + at + (k / 4) * (kBlock * 128 >> 4) + (k % 4) * 2, hi), kIdescS, k > 0);
-            __syncwarp();
-            if (!(ok = wait_all(base + M::kVFull, x & 1, abort_flag))) break;
-            tc::tc_fence_after_sync();
-            if (leader) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     tc::mma_f16_ss(tmem + 64, tc::desc64(g_lo + (k / 4) * (kRows * 128 >> 4) + (k % 4) * 2, hi),
@@ -764,11 +788,13 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 // dK, dV: a block of 64 keys of one head through the tiles of queries in which any has listed it.  Per tile S = Q K^T and dP = dO V^T as above, rows in lanes;
 // P and dS go to shared memory, where they are the operands of dV^T[d x 64] += dO^T P and dK^T += Q^T dS: contracted over the rows, all heads of the group
 // summed on the way, in the order of the tiles.  d <= 64: both at once, [dO Q]^T [P dS], whose other two quarters are not used.
-// Q and dO are double buffered.  d > 64: 192 KB of shared memory, one CTA an SM, S and dP double buffered in tensor memory: the products of the next tile
-// run under this one's exponentials.  d <= 64: two CTAs an SM with one buffer each, so that one begins and ends under the other's work; few tiles have listed a
-// block where a tile is 128 queries.  The softmax has eight warps, two to a quarter of the rows, 32 keys each.
-// Bound by the hand-overs through shared memory (P and dS are written and waited for before the second products): the tiles above take 938 us, 0.63 PFLOP/s on them;
-// 16 warps for the softmax 933.  A block that all later queries have listed (up to 392 tiles there, 138 on average) is one CTA's work and starts first.
+// d > 64: 225 KB of shared memory, one CTA an SM, five places for copies of Q and dO, which come one by one; S and dP double buffered in tensor memory, so that the
+// products of the next tile run under this one's exponentials, and two groups of softmax warps that take tiles in turn.  d <= 64: two CTAs an SM with one buffer and
+// one group each, so that one begins and ends under the other's work; few tiles have listed a block where a tile is 128 queries.  A group has eight warps, two to a
+// quarter of the rows, 32 keys each.
+// Bound by shared memory and hand-overs: a tile's products read 192 KB of operands there (1540 cycles), its copies and P, dS write 96 KB (770), and it takes 3200: the
+// tiles above 837 us, 0.71 PFLOP/s on them (938 with four places, one group and one wait after another).  A block that most later queries have listed (up to 392
+// tiles there, 138 on average) is one CTA's work and starts first.
 template <int DP> struct GradKVSmem {
     static constexpr int kBuffers = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;   // of S and dP; CTAs an SM
     // Q and dO of tile x are copies 2 x and 2 x + 1, copy n in place n % kPlaces; d <= 64: always Q in an even one, dO behind it
@@ -827,8 +853,8 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder), tmem_acc = tmem + M::kBuffers * 128;
     bool bad = false;
 
+    pdl_wait();   // all roles: the bounded waits below are for this kernel's own work, not for that of kernels before it
     if (warp == 8) {
-        pdl_wait();
         if (lane == 0) {
             tc::mbar_expect_tx(base + M::kKV, 2 * M::kSlotBytes);
             for (int y = 0; y < DP / 64; ++y) {
