@@ -2,7 +2,8 @@
 
 Host side of libvsparse_b200.so: the CVSE builder (`cvse`), the operators named as in the vectorSparse
 reference (`spmm.wmmaSpmm`, `spmm.cudaSpmm`, `sddmm.wmmaSddmm`, `sddmm.cudaSddmm`), batched forms, the masked
-row softmax, fixed-mask sparse attention, and sharding helpers for several GPUs (`shard`).
+row softmax, fixed-mask sparse attention, attention over blocks of keys that the data choose (`ops.select_blocks`,
+`ops.selected_attention`) and over a paged cache in 8 bits (`ops.BlockCache`), and sharding helpers for several GPUs (`shard`).
 """
 from . import _lib, cvse  # noqa: F401
 from ._lib import VS_F16, VS_F32, VS_PATH_CUDA_CORE, VS_PATH_TENSOR, VsError  # noqa: F401

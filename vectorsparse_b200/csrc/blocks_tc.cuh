@@ -242,6 +242,10 @@ template <typename T, int DP, typename F> __device__ __forceinline__ void write_
             *reinterpret_cast<uint4 *>(out + at + c * 8) = *reinterpret_cast<const uint4 *>(stage + at_slab / 8 * slab + r * 128 + (((at_slab % 8) ^ (r & 7)) << 4));
     }
 }
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+    else return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
 // The two warps of a quarter of the rows meet (64 threads, barriers 1 .. 4).
 __device__ __forceinline__ void bar_pair(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 template <typename T> __device__ __forceinline__ uint4 pack8(const float *f) {
@@ -552,10 +556,11 @@ template <typename T> struct Lift {
 __device__ __forceinline__ float exp2i(float e) { return __uint_as_float((uint32_t)((int)e + 127) << 23); }   // a whole exponent
 
 // dQ: a tile of queries through the union of its lists, as forward.  Per block S = Q K^T and dP = dO V^T, dS = P (dP - delta) back into S's place as an operand,
-// dQ += dS K with the same keys, now contracted over.  Keys are double buffered, values not: their place is free once dP is there, long before the
+// dQ += dS K with the same keys, now contracted over.  A row's dS sum to 0, so its products with the keys cancel and a
+// rounding of dS counts more than one of the result (1.5 times its error): dS goes in as two words, itself and what its rounding left over.  Keys are double buffered, values not: their place is free once dP is there, long before the
 // next ones are needed.  256 columns of tensor memory, 113 KB of shared memory (d = 128): two CTAs an SM, one's products under the other's exponentials.
-// Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 476 us, 0.94 PFLOP/s on them
-// (500 with one wait after another).
+// Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 550 us
+// (476 without the second word).
 template <int DP> struct GradQSmem {
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
     static constexpr int kQ = 1024, kG = kQ + kQBytes, kK = kG + kQBytes, kV = kK + 2 * kSlotBytes, kBytes = kV + kSlotBytes;
@@ -686,6 +691,9 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 #pragma unroll
                 for (int k = 0; k < kBlock / 16; ++k)
                     tc::mma_f16_ts(tmem + 128, tmem + 8 * k, tc::desc64(kt_lo + at + 128 * k, hi), kIdescQ, x > 0 || k > 0);
+#pragma unroll
+                for (int k = 0; k < kBlock / 16; ++k)   // what the rounding of dS left over
+                    tc::mma_f16_ts(tmem + 128, tmem + 32 + 8 * k, tc::desc64(kt_lo + at + 128 * k, hi), kIdescQ, true);
                 tc::mma_commit(base + M::kDq);
                 tc::mma_commit(base + M::kKEmpty + 8 * slot);
             }
@@ -727,7 +735,7 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
             tc::tc_fence_after_sync();
             const bool whole = __all_sync(~0u, n <= 0 || n == kBlock);
             const float off = n > 0 ? -lse : -INFINITY;   // a row that has not listed the block has no weight there
-            uint32_t u[32], d[32], ds[16];
+            uint32_t u[32], d[32], ds[16], low[16];
             tc::tmem_ld_x32_issue(mine + 32 * half, u);
             tc::tmem_ld_x32_issue(mine + 64 + 32 * half, d);
             tc::tmem_ld_x32_wait(u);
@@ -743,10 +751,13 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
                     if (32 * half + 2 * k + 1 >= n) f.y = 0.f;
                 }
                 ds[k] = pack2<T>(f.x, f.y);
+                const float2 left = fma2(unpack2<T>(ds[k]), make_float2(-1.f, -1.f), f);
+                low[k] = pack2<T>(left.x, left.y);
             }
-            // dS goes where the first half's scores stood, which that half's other warp has read before it comes here
+            // dS goes where the scores stood, which both warps of a quarter have read before they come here
             bar_pair(1 + quarter);
             tc::tmem_st_x16(mine + 16 * half, ds);
+            tc::tmem_st_x16(mine + 32 + 16 * half, low);
             tc::tmem_st_wait();
             tc::tc_fence_before_sync();
             __syncwarp();

@@ -17,7 +17,14 @@ of fixed-mask sparse attention into torch.autograd, so that the pair can sit ins
     c = sparse_dense_product(values, b, mask)                 # [m, N] = A(values) @ b, differentiable in values and b
     # backward: d b = A^T @ d c (vs_spmm_t), d values = (d c @ b^T) sampled at the structure (vs_sddmm)
 
-On plain contiguous fp16 CUDA tensors both are recorded in torch's graph by the binding, without a Python function per pass; the two
+Attention over blocks of 64 keys chosen by the data, and the same for single tokens over a paged cache in 8 bits:
+
+    blocks = select_blocks(q, k, 16)                          # q [B, Lq, Hq, D], k, v [B, Lk, Hkv, D], fp16 or bf16
+    out = selected_attention(q, k, v, blocks, scale)          # differentiable in q, k and v
+    cache_append(cache, k, v, table, tails, lengths)          # cache: a BlockCache
+    out = cache_attention(q1, cache, table, tails, lengths, scale, cache_select(q1, cache, table, lengths, 16))
+
+On plain contiguous fp16 CUDA tensors the first two are recorded in torch's graph by the binding, without a Python function per pass; the two
 torch.autograd.Function classes take everything else (modes, tracers, transforms, subclasses) and say what the gradients are.
 """
 from __future__ import annotations
