@@ -384,3 +384,21 @@ def test_backward_in_a_graph_beside_an_eager_one_and_two_calls_at_once():
                 results.append((y, *torch.autograd.grad(y, x, grad)))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for r in results for a, b in zip(r, (held, *want)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,count", [(1, 1, 4, 5, 1, 80, 2), (2, 2, 2, 8, 4, 32, 20), (1, 3, 7, 2, 2, 128, 1), (1, 1, 1, 64, 1, 8, 1)])
+def test_a_handful_of_rows(dtype, B, Lq, Lk, Hq, Hkv, D, count):
+    """So few products are computed in fp32: every result within its own rounding and the fp32 sums, without the weights' 16-bit ones."""
+    q, k, v, grad = tensors(B, Lq, Lk, Hq, Hkv, D, dtype, 31 * Lk + D)
+    blocks = torch_ops.select_blocks(q, k, count)
+    check(dtype, q, k, v, blocks, D ** -0.5, True, None, grad)
+    leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+    out = torch_ops.selected_attention(*leaves, blocks, D ** -0.5)
+    got = (out, *torch.autograd.grad(out, leaves, grad))
+    want = plain.attention(*(x.double().cpu().numpy() for x in (q, k, v)), blocks.cpu().numpy(), D ** -0.5, True, None, grad.double().cpu().numpy())
+    for x, y in zip(got, want):
+        y = np.asarray(y)
+        # half a step of the type, and 2^-16 of the largest element for fp32 sums of some hundred products, for exp2 and for out's remainder in 16 bits
+        allowed = np.abs(y) * torch.finfo(dtype).eps / 2 + (2.0 ** -16 + torch.finfo(dtype).tiny) * max(1.0, np.abs(y).max())
+        assert (np.abs(x.detach().double().cpu().numpy() - y) <= allowed).all()

@@ -194,6 +194,12 @@ inline int64_t query_tiles(const blocks::Shape &s) {
 }
 inline unsigned again_grid(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 4 * 148); }
 
+// A handful of products: the row kernels alone, in fp32 throughout.  Nothing averages the 16-bit roundings of a tile's weights there, and it is no slower: 5 rows of 4 keys 8.4
+// us and 21.1 backward against 8.2 and 21.6 by tiles, 32 rows of 2 keys 6.0 and 10.5 against 7.2 and 16.7; 64 rows of 8 keys 22 and 23 against 6.9 and 15.3.
+inline bool few(const blocks::Shape &s) {
+    return (int64_t)s.batch * s.queries * s.heads <= 64 && (int64_t)s.batch * s.queries * s.heads * std::min<int64_t>(s.keys, (int64_t)s.count * blocks::kBlock) <= 64;
+}
+
 template <typename T, int DP> int forward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
     const blocks::Shape &s = a.s;
     using Smem = blocks::tcore::ForwardSmem<DP>;
@@ -212,9 +218,9 @@ template <typename T, int DP> int forward(blocks::Args a, uint32_t *redo, uint32
 }
 template <typename T> int attention(blocks::Args a, uint32_t *redo, cudaStream_t st) {
     const blocks::Shape &s = a.s;
-    if (s.keys == 0) {   // no key to attend to
-        a.tile = tile_queries(s.group);
-        blocks::rows_kernel<T, false><<<again_grid(query_tiles(s)), blocks::kRowThreads, 0, st>>>(a);
+    if (s.keys == 0 || few(s)) {
+        a.tile = 1;
+        blocks::rows_kernel<T, false><<<again_grid((int64_t)s.batch * s.kv_heads * s.queries), blocks::kRowThreads, 0, st>>>(a);
         return (int)cudaGetLastError();
     }
     int sms = 0;
@@ -255,6 +261,14 @@ template <typename T> int attention_backward(blocks::Args a, uint32_t *redo, cud
     uint32_t *status = nullptr;
     const int rc = current_device(&sms, &status);
     if (rc != VS_OK) return rc;
+    if (few(a.s)) {
+        a.tile = 1;
+        const int64_t rows = (int64_t)a.s.batch * a.s.queries * a.s.heads;
+        cudaError_t e = launch_behind(blocks::delta_kernel<T>, (unsigned)((rows + 15) / 16), 256, 0, st, a);
+        if (e == cudaSuccess) e = launch_behind(blocks::rows_kernel<T, true>, again_grid((int64_t)a.s.batch * a.s.kv_heads * a.s.queries), blocks::kRowThreads, 0, st, a);
+        if (e == cudaSuccess) e = launch_behind(blocks::keys_kernel<T>, again_grid((int64_t)a.s.batch * a.s.kv_heads * a.s.blocks), blocks::kRowThreads, 0, st, a);
+        return (int)e;
+    }
     return a.s.d <= 64 ? backward<T, 64>(a, redo, status, st) : backward<T, 128>(a, redo, status, st);
 }
 

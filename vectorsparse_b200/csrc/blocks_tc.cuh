@@ -559,7 +559,7 @@ __device__ __forceinline__ float exp2i(float e) { return __uint_as_float((uint32
 // dQ += dS K with the same keys, now contracted over.  A row's dS sum to 0, so its products with the keys cancel and a
 // rounding of dS counts more than one of the result (1.5 times its error): dS goes in as two words, itself and what its rounding left over.  Keys are double buffered, values not: their place is free once dP is there, long before the
 // next ones are needed.  256 columns of tensor memory, 113 KB of shared memory (d = 128): two CTAs an SM, one's products under the other's exponentials.
-// Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 550 us
+// Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 531 us
 // (476 without the second word).
 template <int DP> struct GradQSmem {
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
