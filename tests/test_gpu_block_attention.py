@@ -402,3 +402,23 @@ def test_a_handful_of_rows(dtype, B, Lq, Lk, Hq, Hkv, D, count):
         # half a step of the type, and 2^-16 of the largest element for fp32 sums of some hundred products, for exp2 and for out's remainder in 16 bits
         allowed = np.abs(y) * torch.finfo(dtype).eps / 2 + (2.0 ** -16 + torch.finfo(dtype).tiny) * max(1.0, np.abs(y).max())
         assert (np.abs(x.detach().double().cpu().numpy() - y) <= allowed).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_key_gradients_of_blocks_that_any_number_of_tiles_has_listed(dtype, D):
+    """Block j of the keys is listed by the queries of the first TILES[j] tiles: odd and even numbers, one and some hundred.  With 32 heads to a head of keys a tile
+    is four queries.  The same bits in every run."""
+    tiles = (1, 2, 3, 4, 5, 6, 7, 8, 150, 151)
+    queries, keys = 4 * max(tiles), 64 * len(tiles)
+    q, k, v, grad = tensors(1, queries, keys, 32, 1, D, dtype, D)
+    blocks = torch.full((1, 1, queries, len(tiles)), -1, dtype=torch.int32, device=DEV)
+    for j, n in enumerate(tiles):
+        blocks[0, 0, :4 * n, j] = j
+    check(dtype, q, k, v, blocks, D ** -0.5, False, None, grad)
+    def gradients():
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        return torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, D ** -0.5, False), leaves, grad)
+    first = gradients()
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(first, gradients()))

@@ -817,7 +817,7 @@ template <int DP> struct GradKVSmem {
     static constexpr int kK = 1024, kV = kK + kSlotBytes, kP = kV + kSlotBytes, kStage = kP + 2 * kPBytes,   // P, dS; places for Q and dO
                          kBytes = kStage + kPlaces * kQBytes;
     static constexpr int kBars = kEntries * sizeof(Entry);
-    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 8 * kPlaces, kSP = kEmpty + 8 * kPlaces, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 8, kDrain = kE + 8 * kEntries,
+    static constexpr int kKV = kBars, kFull = kKV + 8, kEmpty = kFull + 8 * kPlaces, kSP = kEmpty + 8 * kPlaces, kPds = kSP + 16, kDone = kPds + 8, kE = kDone + 16, kDrain = kE + 8 * kEntries,
                          kAbort = kDrain + 8, kHolder = kAbort + 4;
     static constexpr int kChunk = 512;
     static_assert(kHolder + 4 <= kChunk && kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
     }
 
     if (threadIdx.x == 0) {
-        for (int bar : {M::kKV, M::kSP, M::kSP + 8, M::kDone, M::kDrain}) tc::mbar_init(base + bar, 1);
+        for (int bar : {M::kKV, M::kSP, M::kSP + 8, M::kDone, M::kDone + 8, M::kDrain}) tc::mbar_init(base + bar, 1);
         for (uint32_t i = 0; i < 2 * M::kPlaces; ++i) tc::mbar_init(base + M::kFull + 8 * i, 1);   // and kEmpty, behind it
         tc::mbar_init(base + M::kPds, 8);
         for (int i = 0; i < kEntries; ++i) tc::mbar_init(base + M::kE + 8 * i, 1);
@@ -983,7 +983,7 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
                         for (int k = 0; k < kRows / 16; ++k)
                             tc::mma_f16_ss(tmem_acc, tc::desc64(g_at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, summed > 0 || k > 0);
                     }
-                    tc::mma_commit(base + M::kDone);
+                    tc::mma_commit(base + M::kDone + 8 * (summed & 1));
                     if (DP == 64) tc::mma_commit(base + M::kEmpty + 8 * q_sum.place);
                     tc::mma_commit(base + M::kEmpty + 8 * g_sum.place);
                 }
@@ -1012,7 +1012,7 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
             }
             idle = 0;
         }
-        if (leader) {
+        if (leader) {   // the results are read behind this; and tensor memory is given back
             tc::mma_commit(base + M::kDrain);
             for (uint32_t y = 0; y < 4096 && !tc::mbar_try_wait(base + M::kDrain, 0); ++y) {}
         }
@@ -1080,7 +1080,9 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
                 p[k] = pack2<T>(w.x, w.y);
                 ds[k] = pack2<T>(f.x, f.y);
             }
-            if (x > 0 && !(ok = __all_sync(~0u, wait(base + M::kDone, (x - 1) & 1, abort_flag)))) break;   // P and dS of the tile before have been read
+            // P and dS of the tile before have been read.  A barrier for every second tile: the phase before this one, of tile x - 3, is over, for this group has waited for it
+            // ahead of tile x - 2 (one group: likewise).
+            if (x > 0 && !(ok = __all_sync(~0u, wait(base + M::kDone + 8 * ((x - 1) & 1), ((x - 1) >> 1) & 1, abort_flag)))) break;
             uint8_t *to = sm + M::kP + r * 128;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
@@ -1094,7 +1096,9 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
             if (lane == 0) tc::mbar_arrive(base + M::kPds);
             look(x + M::kGroups);
         }
-        if (ok && total > 0) ok = __all_sync(~0u, wait(base + M::kDone, (total - 1) & 1, abort_flag));
+        // All products, of this group's tiles and of the other's.  The last tile may be the other group's, and the end is posted when the place of Q of the tile before it is
+        // free, ahead of that tile's kDone: a wait for kDone could take an earlier phase for the last one.  kDrain has one phase, behind the last product.
+        if (ok && total > 0) ok = __all_sync(~0u, wait(base + M::kDrain, 0, abort_flag));
         if (ok && group == 0) {
             // accumulators: a dimension to a lane, keys in columns.  d > 64: dV in columns 0 .. 63, dK in 64 ..; d <= 64: dK in lanes 0 .. 63 of columns 64 ..,
             // dV in lanes 64 .. of columns 0 ..  The two halves of the warps take one of the two each, or 32 keys each.
