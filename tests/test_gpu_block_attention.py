@@ -422,3 +422,18 @@ def test_key_gradients_of_blocks_that_any_number_of_tiles_has_listed(dtype, D):
     first = gradients()
     for _ in range(20):
         assert all(torch.equal(a, b) for a, b in zip(first, gradients()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(1, 0, -1, 0), (0, 1, -1), (1, 1, 0, 0, -1, -1, 0, 0)])
+def test_selection_where_the_heads_of_a_group_cancel(dtype, heads):
+    """Heads whose large parts cancel: what is left is far below the rounding of a 32-bit sum on its way."""
+    q, k, _, _ = tensors(1, 150, 64 * 40, 2 * len(heads), 2, 64, dtype, 14)
+    large = (tensors(1, 150, 1, 2, 2, 64, dtype, 15)[0].float().clamp(-4, 4) * 2.0 ** 12).to(dtype)
+    for h, sign in enumerate(heads):
+        for kv in range(2):
+            x = q[:, :, kv * len(heads) + h]
+            x.copy_(large[:, :, kv] * sign if sign else x * 2.0 ** -8)
+    for causal in (True, False):
+        got = torch_ops.select_blocks(q, k, 6, causal).cpu().numpy()
+        assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), 6, causal, None)), causal

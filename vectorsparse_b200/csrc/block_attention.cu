@@ -116,7 +116,7 @@ template <typename T, int QT> int launch_scores(const blocks::Shape &s, const bl
     blocks::score_kernel<T, QT><<<(unsigned)grid, blocks::kScoreThreads, smem, st>>>(s, q, means, lists);
     return (int)cudaGetLastError();
 }
-// The workspace of a choice: means in 64 and in 32 bits and the norms of the latter, then the scores of a slab and the norms of its queries.  Slabs of 48 MB stay in
+// The workspace of a choice: means in 64 and in 32 bits and the norms of the latter, then the scores of a slab and the error bounds of its queries.  Slabs of 48 MB stay in
 // L2 between the two kernels that share them.
 struct SelectSpace {
     int64_t means, blocks, tiles, slab;   // elements of the means, blocks of keys, tiles of queries, tiles of a slab
@@ -148,7 +148,7 @@ template <typename T> int select(const blocks::Shape &s, const blocks::Operand &
         if (rc != VS_OK) return rc;
         blocks::Slab slab;
         slab.scores = reinterpret_cast<float *>(at + up256(space.blocks * 4));
-        slab.norms = slab.scores + space.slab * blocks::kFastQueries * s.blocks;
+        slab.errors = slab.scores + space.slab * blocks::kFastQueries * s.blocks;
         for (slab.first = 0; slab.first < space.tiles; slab.first += space.slab) {
             slab.tiles = std::min(space.slab, space.tiles - slab.first);
             cudaError_t e = launch_behind(blocks::fast_score_kernel<T>, (unsigned)slab.tiles, blocks::kFastThreads, smem, st, s, q, (const float *)means32, slab);

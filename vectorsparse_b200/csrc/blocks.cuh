@@ -199,7 +199,7 @@ constexpr int fast_bytes(int d) { return (kFastQueries * fast_pitch(d) + kFastBl
 struct Slab {   // tiles of kFastQueries queries of a head of keys, from `first` on
     int64_t first, tiles;
     float *scores;   // [tiles][kFastQueries][blocks]
-    float *norms;    // [tiles][kFastQueries]: of the queries' sums
+    float *errors;   // [tiles][kFastQueries]: steps of 2^-24 that a score is off by at most, for a mean of norm 1
 };
 struct FastTile {
     int b, h, i0, most;   // most: candidates of any query of the tile
@@ -285,6 +285,7 @@ template <typename T> __global__ void __launch_bounds__(kFastThreads, 2) fast_sc
     extern __shared__ __align__(16) float fsm[];
     const int pitch = fast_pitch(s.d), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     float *sums = fsm, *piece = sums + kFastQueries * pitch;
+    __shared__ float summands[kFastQueries];   // squares of the norms of the heads' magnitudes, summed
     pdl_launch_dependents();
     const int64_t index = slab.tiles - 1 - blockIdx.x;   // the last queries have most candidates: they go first
     const FastTile t(s, slab.first + index);
@@ -296,16 +297,24 @@ template <typename T> __global__ void __launch_bounds__(kFastThreads, 2) fast_sc
     const T *qp = static_cast<const T *>(q.at) + t.b * q.batch + t.h * s.group * q.head;
     for (int x = tid; x < kFastQueries * chunks; x += kFastThreads) {
         const int i = x / chunks, c = x % chunks * 8;
-        float sum[8] = {};
+        float sum[8] = {}, size[8] = {};
         if (t.i0 + i < rows && c < s.d) {
 #pragma unroll 8
             for (int g = 0; g < s.group; ++g) {
                 float f[8];
                 load8(qp + (t.i0 + i) * q.token + g * q.head + c, f);
 #pragma unroll
-                for (int y = 0; y < 8; ++y) sum[y] += f[y];
+                for (int y = 0; y < 8; ++y) {
+                    sum[y] += f[y];
+                    size[y] += fabsf(f[y]);
+                }
             }
         }
+        float square = 0.f;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) square = fmaf(size[y], size[y], square);
+        for (int o = chunks / 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);   // 8 or 16 neighbours have a query; all lanes are here
+        if (c == 0) summands[i] = square;
 #pragma unroll
         for (int y = 0; y < 8; y += 4) *reinterpret_cast<float4 *>(sums + i * pitch + c + y) = make_float4(sum[y], sum[y + 1], sum[y + 2], sum[y + 3]);
     }
@@ -313,12 +322,14 @@ template <typename T> __global__ void __launch_bounds__(kFastThreads, 2) fast_sc
     static_assert(kFastThreads == 4 * kFastQueries, "four threads to a query's norm");
     {
         const float *p = sums + tid / 4 * pitch;
-        float square = 0.f;
+        float square = 0.f;   // of the norm of the sum
         for (int x = tid % 4; x < s.d; x += 4) square = fmaf(p[x], p[x], square);
 #pragma unroll
         for (int o = 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
         pdl_wait();   // the means are the kernel's before, and whoever reads the last slab is done
-        if (tid % 4 == 0) slab.norms[index * kFastQueries + tid / 4] = sqrtf(square) * 1.001f;
+        // one rounding for each of the d terms of a product and those of its operands, relative to the sum; one for each of the group's additions, relative to what is added,
+        // which the sum itself may be far below
+        if (tid % 4 == 0) slab.errors[index * kFastQueries + tid / 4] = ((s.d + 8) * sqrtf(square) + (s.group - 1) * sqrtf(summands[tid / 4])) * 1.001f;
     }
     // queries 4 ty .. 4 ty + 3, blocks tx + 16 x
     const int tx = lane % 16, ty = warp * 2 + lane / 16;
@@ -372,7 +383,7 @@ template <typename T> __global__ void __launch_bounds__(kFastThreads, 2) fast_sc
 
 // The list of one query from its n > want > 0 candidates' scores.  A lane holds kHeld of them in registers; more are read each time.
 template <typename T, int kHeld> __device__ __forceinline__ void rank_row(const Shape &s, const FastTile &t, const Operand &q, int i, int own, int n, int want, const float *row,
-                                                                          const float *query_norm, const double *means, const float *mean_norms, int32_t *list, Members &m) {
+                                                                          const float *error, const double *means, const float *mean_norms, int32_t *list, Members &m) {
     const int lane = threadIdx.x & 31;
     float v[kHeld], top = -FLT_MAX, low = FLT_MAX, norm = 0.f;
     bool number = true;
@@ -397,8 +408,7 @@ template <typename T, int kHeld> __device__ __forceinline__ void rank_row(const 
         low = fminf(low, f);
     }
     float hi = unsortable32(__reduce_max_sync(~0u, sortable32(top))), lo = unsortable32(__reduce_min_sync(~0u, sortable32(low))), at = 0.5f * hi + 0.5f * lo;
-    // one rounding for each of the d terms of a sum, the group's, and those of the operands; what is denormal besides
-    const float off = (float)(s.d + s.group + 8) * 0x1p-24f * __ldcg(query_norm) * __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(norm))) * 1.01f + 0x1p-120f;
+    const float off = 0x1p-24f * __ldcg(error) * __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(norm))) * 1.01f + 0x1p-120f;
     const bool usable = __all_sync(~0u, number) && off <= FLT_MAX;
     bool found = false;
     int reach_lo = n, reach_hi = 1;   // how many reach lo: more than `want`; and hi: fewer, or, at first, perhaps as many
@@ -468,10 +478,10 @@ template <typename T> __global__ void __launch_bounds__(kFastThreads) fast_rank_
         for (int x = lane; x < s.count; x += 32) list[x] = x < all ? x : want == 0 && i < rows && x == 0 ? own : -1;
         return;
     }
-    const float *row = slab.scores + row_index * s.blocks, *query_norm = slab.norms + row_index;
-    if (n <= 64) rank_row<T, 2>(s, t, q, i, own, n, want, row, query_norm, means, mean_norms, list, members_all[warp]);
-    else if (n <= 128) rank_row<T, 4>(s, t, q, i, own, n, want, row, query_norm, means, mean_norms, list, members_all[warp]);
-    else rank_row<T, 8>(s, t, q, i, own, n, want, row, query_norm, means, mean_norms, list, members_all[warp]);
+    const float *row = slab.scores + row_index * s.blocks, *error = slab.errors + row_index;
+    if (n <= 64) rank_row<T, 2>(s, t, q, i, own, n, want, row, error, means, mean_norms, list, members_all[warp]);
+    else if (n <= 128) rank_row<T, 4>(s, t, q, i, own, n, want, row, error, means, mean_norms, list, members_all[warp]);
+    else rank_row<T, 8>(s, t, q, i, own, n, want, row, error, means, mean_norms, list, members_all[warp]);
 }
 
 // 64 bits throughout, for lists and sequences that the kernel above has no room for.
