@@ -437,3 +437,24 @@ def test_selection_where_the_heads_of_a_group_cancel(dtype, heads):
     for causal in (True, False):
         got = torch_ops.select_blocks(q, k, 6, causal).cpu().numpy()
         assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), 6, causal, None)), causal
+
+
+@pytest.mark.parametrize("q_scale,k_scale", [(1.0, 1.0), (1.0, 2.0 ** -76), (2.0 ** -76, 1.0), (2.0 ** -50, 2.0 ** -66)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_selection_of_near_ties_whose_squares_underflow(q_scale, k_scale, causal):
+    """Scores that differ in the 28th bit, of operands whose squares are below 32 bits' range.  All blocks have the same keys but for the order of the two
+    elements of some pairs, which a query with equal elements in a pair does not see but for the rounding of its sum, and an element of their own under a
+    query element of 2^-20."""
+    blocks, rng = 44, np.random.default_rng(7)
+    k = np.tile(rng.standard_normal((64, 64)).astype(np.float32), (blocks, 1, 1))
+    for j in range(blocks):
+        for p in range(1, 32):
+            if rng.random() < 0.5:
+                k[j][:, [2 * p, 2 * p + 1]] = k[j][:, [2 * p + 1, 2 * p]]
+    k[:, :, 0] = rng.permutation(blocks)[:, None] / 32
+    q = np.repeat(rng.standard_normal((1, 20, 1, 32)), 2, 3).astype(np.float32)
+    q[..., 0] = 2.0 ** -20
+    k = torch.from_numpy(k.reshape(1, 64 * blocks, 1, 64)).bfloat16().mul(k_scale).to(DEV)
+    q = torch.from_numpy(q).bfloat16().mul(q_scale).to(DEV)
+    got = torch_ops.select_blocks(q, k, 6, causal).cpu().numpy()
+    assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), 6, causal, None))

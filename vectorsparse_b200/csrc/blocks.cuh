@@ -97,6 +97,9 @@ __global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const
 // ---- choosing -----------------------------------------------------------------------------------------------------
 // Score of block j for query i: (sum of the group's query heads) . (mean of the block's keys), everything in 64 bits: its order decides whole
 // numbers, and 32-bit sums in two orders disagree about blocks that are close.
+// A bound on the norm of up to kMaxD elements from the fp32 sum of their squares, in any order: a square below 2^-126 is off by 2^-150 at most, and one below 2^-150
+// counts as nothing, so the sum by d 2^-149 and its root by less than 2^-70.
+__device__ __forceinline__ float norm_bound(float squares) { return fmaf(sqrtf(squares), 1.001f, 0x1p-70f); }
 // Means: one CTA per (b, kv head, block), 8 dimensions to a thread, the tokens shared by groups of threads; in 64 bits, and in 32 with a bound on their norm.
 // Bound by the latency of its few loads: 1024 blocks of 64 tokens, d = 128, 14 us (1.2 TB/s).
 constexpr int kMeanThreads = 128;
@@ -132,7 +135,7 @@ template <typename T> __global__ void __launch_bounds__(kMeanThreads) means_kern
         atomicAdd(&squares, rounded * rounded);   // a bound, with room for the order of its sum
     }
     __syncthreads();
-    if (threadIdx.x == 0) norms[at] = sqrtf(squares) * 1.001f;
+    if (threadIdx.x == 0) norms[at] = norm_bound(squares);
 }
 
 // Scores as whole numbers of the same order, above 0; what is no number counts as the lowest score.
@@ -329,7 +332,7 @@ template <typename T> __global__ void __launch_bounds__(kFastThreads, 2) fast_sc
         pdl_wait();   // the means are the kernel's before, and whoever reads the last slab is done
         // one rounding for each of the d terms of a product and those of its operands, relative to the sum; one for each of the group's additions, relative to what is added,
         // which the sum itself may be far below
-        if (tid % 4 == 0) slab.errors[index * kFastQueries + tid / 4] = ((s.d + 8) * sqrtf(square) + (s.group - 1) * sqrtf(summands[tid / 4])) * 1.001f;
+        if (tid % 4 == 0) slab.errors[index * kFastQueries + tid / 4] = (s.d + 8) * norm_bound(square) + (s.group - 1) * norm_bound(summands[tid / 4]);
     }
     // queries 4 ty .. 4 ty + 3, blocks tx + 16 x
     const int tx = lane % 16, ty = warp * 2 + lane / 16;
@@ -408,6 +411,7 @@ template <typename T, int kHeld> __device__ __forceinline__ void rank_row(const 
         low = fminf(low, f);
     }
     float hi = unsortable32(__reduce_max_sync(~0u, sortable32(top))), lo = unsortable32(__reduce_min_sync(~0u, sortable32(low))), at = 0.5f * hi + 0.5f * lo;
+    // besides, products and sums below 2^-126 are off by 2^-150 each
     const float off = 0x1p-24f * __ldcg(error) * __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(norm))) * 1.01f + 0x1p-120f;
     const bool usable = __all_sync(~0u, number) && off <= FLT_MAX;
     bool found = false;
