@@ -4,7 +4,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstdlib>
@@ -15,6 +14,7 @@
 #include "vsparse_b200.h"
 #include "common.cuh"
 #include "host.h"
+#include "smem_limit.h"
 #include "blocks.cuh"
 #include "blocks_tc.cuh"
 #include "cache.cuh"
@@ -44,19 +44,14 @@ cudaError_t launch_behind(void (*kernel)(Exp...), unsigned grid, unsigned block,
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Act>(args)...);
 }
-// The most shared memory that a kernel may ask for, told to the runtime once per device and kernel (the kernel's address is the key).
+// The most shared memory that a kernel may ask for, told to the runtime where it grows (the kernel's address is the key).
 template <auto kKernel> int allow_smem(int bytes) {
-    static std::atomic<int> known[64];
+    static SmemLimit limit;
     int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
-    if (dev < 0 || dev >= 64) return VS_ERR_ARG;
-    if (known[dev].load(std::memory_order_acquire) >= bytes) return VS_OK;
-    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return (int)e;
-    int now = known[dev].load(std::memory_order_relaxed);
-    while (now < bytes && !known[dev].compare_exchange_weak(now, bytes, std::memory_order_release)) {}
-    return VS_OK;
+    if (dev < 0 || dev >= SmemLimit::kDevices) return VS_ERR_ARG;
+    return limit.raise(dev, bytes, [&] { return (int)cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
 }
 
 // ---- attention over chosen blocks -----------------------------------------------------------------------------------
