@@ -7,6 +7,7 @@
 //
 // A multiplied tile knows nothing of single keys: 0 * Inf in it is a NaN that the operator does not have.  So a tile whose result is not finite says so in its
 // word of `redo`, and the row kernels behind compute it again; they read only what a row attends to.
+// A tile in which a bounded wait ran out has written nothing or a part: it goes the same way, besides the bit in the status word.
 #pragma once
 #include <cuda.h>
 
@@ -533,8 +534,9 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
     tc::tc_fence_before_sync();
     const bool again = __syncthreads_or(bad);
     if (threadIdx.x == 0) {
-        redo[t.index] = again;
-        if (*abort_flag) atomicOr(status, kStatusForward);
+        const bool gave_up = *abort_flag != 0;
+        redo[t.index] = again || gave_up;
+        if (gave_up) atomicOr(status, kStatusForward);
     }
     if (warp == 9) {
         tc::tc_fence_after_sync();
@@ -787,8 +789,9 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
     tc::tc_fence_before_sync();
     const bool again = __syncthreads_or(bad);
     if (threadIdx.x == 0) {
-        redo[t.index] = again;
-        if (*abort_flag) atomicOr(status, kStatusGradQ);
+        const bool gave_up = *abort_flag != 0;
+        redo[t.index] = again || gave_up;
+        if (gave_up) atomicOr(status, kStatusGradQ);
     }
     if (warp == 9) {
         tc::tc_fence_after_sync();
@@ -1130,8 +1133,9 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
     tc::tc_fence_before_sync();
     const bool again = __syncthreads_or(bad);
     if (threadIdx.x == 0) {
-        redo[bh * s.blocks + j] = again;
-        if (*abort_flag) atomicOr(status, kStatusGradKV);
+        const bool gave_up = *abort_flag != 0;
+        redo[bh * s.blocks + j] = again || gave_up;
+        if (gave_up) atomicOr(status, kStatusGradKV);
     }
     if (warp == 9) {
         tc::tc_fence_after_sync();
