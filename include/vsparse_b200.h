@@ -294,7 +294,8 @@ int vs_device_status(int clear, uint32_t *status);
  * reads lse and, for rowsum(out o grad_out), out and out_low: from the rounded out alone the gradients of q and k would be twice as far off.  scale: finite and above 0.
  * Scores, their maximum and sum, and all sums over keys are fp32; the weights (at most 256 in magnitude ahead of the division)
  * are rounded to the type for the product with v, as are they and the scores' gradients in the backward pass (for q's gradient the latter in two
- * words); a handful of rows and keys is computed in fp32 throughout.
+ * words); a handful of rows and keys is computed in fp32 throughout.  fp16: the scores' gradients are multiplied by a power of two before they are rounded, one that fits the largest
+ * finite element of grad_out in the row (for q), or in the rows that have listed the block (for k), so that small gradients keep their bits whatever stands in other rows.
  *
  * vs_selected_attention_backward: gradients of q, k and v (all three written whole) for grad_out; the gradients of a head of keys are summed over its group,
  * in the same order in every call.  Both take a workspace of vs_selected_attention_workspace_bytes(..., backward).

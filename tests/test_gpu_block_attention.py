@@ -458,3 +458,46 @@ def test_selection_of_near_ties_whose_squares_underflow(q_scale, k_scale, causal
     q = torch.from_numpy(q).bfloat16().mul(q_scale).to(DEV)
     got = torch_ops.select_blocks(q, k, 6, causal).cpu().numpy()
     assert np.array_equal(got, plain.select(plain.f64(q), plain.f64(k), 6, causal, None))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** -4, 4.0), (4.0, 2.0 ** -4)])   # sums that show what their terms have lost: gradients of q, of k
+@pytest.mark.parametrize("value", [float("inf"), float("nan"), 1000.0])
+def test_small_gradients_beside_a_row_of_large_ones(D, q_size, k_size, value):
+    """fp16, grad_out of 1e-4: the scores' gradients lie below the type's normal range unless they are lifted, whatever stands in one row of grad_out.
+
+    Besides the tolerances above: with M the largest element of the rows that share a lift (the row for grad_q, the rows that have listed the block for grad_k), a
+    score's gradient is multiplied by 32 / M or more before it is rounded, and below the normal range a rounding is off by 2^-25, so a term by 2^-25 M / 32 times its
+    key or query."""
+    q, k, v, grad = tensors(2, 200, 200, 4, 2, D, torch.float16, 17)
+    q, k, v, grad = q * q_size, k * k_size, v * 2.0 ** -4, (grad.float() * 1e-4).half()
+    blocks = lists(2, 2, 200, 200, 3, 17)
+    b, i, h = 1, 150, 2
+    blocks[b, h // 2, i] = torch.tensor([1, 3, -1], dtype=torch.int32)
+    given = grad.clone()
+    reached = [np.zeros(x.shape, bool) for x in (q, k, v)]
+    if np.isfinite(value):
+        given[b, i, h] = grad[b, i, h] = (grad[b, i, h].float() * 1e7).half()   # N(0, 1000^2)
+    else:
+        given[b, i, h, 5] = value
+        grad[b, i, h] = 0
+        reached[0][b, i, h] = True
+        for x in reached[1:]:
+            x[b, 64:128, h // 2] = x[b, 192:, h // 2] = True
+    leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 1.0, False), leaves, given)
+    assert ops.device_status() == 0
+    args = [plain.f64(x) for x in (q, k, v)] + [blocks.cpu().numpy(), 1.0, False, None, plain.f64(grad)]
+    below = [np.zeros(x.shape) for x in args[:3]]
+    peak = np.zeros((2, 2, 4))
+    rows = [(b, h, i, plain.named(args[3], b, h, i, 200, 200, False, None), slice(2 * h, 2 * h + 2)) for b in range(2) for h in range(2) for i in range(200)]
+    for b, h, i, t, heads in rows:
+        peak[b, h, np.unique(t // 64)] = np.maximum(peak[b, h, np.unique(t // 64)], np.abs(args[7][b, i, heads]).max())
+    for b, h, i, t, heads in rows:
+        if len(t):
+            below[0][b, i, heads] = 2.0 ** -30 * np.abs(args[7][b, i, heads]).max(-1)[:, None] * np.abs(args[1][b, t, h]).sum(0)
+            below[1][b, t, h] += 2.0 ** -30 * peak[b, h, t // 64][:, None] * np.abs(args[0][b, i, heads]).sum(0)
+    u = torch.finfo(torch.float16).eps / 2
+    for name, a, want, m, floor, not_here in zip(("grad_q", "grad_k", "grad_v"), got, plain.attention(*args)[1:], magnitudes(*args)[1:], below, reached):
+        error = np.where(not_here, 0, np.abs(plain.f64(a) - want))
+        assert (error <= (3 * u + 2.0 ** -18) * m + u * np.abs(want) + floor + 2.0 ** -24).all(), (name, float(error.max()))

@@ -94,6 +94,7 @@ void contiguous(blocks::Operand &o, const void *at, int64_t tokens, int64_t head
 inline int64_t up256(int64_t bytes) { return (bytes + 255) & ~255ll; }
 inline int64_t bits_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * s.words * s.blocks * 4); }
 
+inline int64_t rows_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.heads * s.queries * 4); }
 inline int64_t redo_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * ((int64_t)s.queries + s.blocks) * 4); }   // a word per tile and block
 
 // Queries of a tile: the largest power of two whose rows (queries x heads of the group) fit 128.
@@ -240,6 +241,8 @@ template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint3
     const int64_t rows = (int64_t)s.batch * s.queries * s.heads, tiles = query_tiles(s), blocks_all = (int64_t)s.batch * s.kv_heads * s.blocks;
     uint32_t *redo_kv = redo + tiles;
     cudaError_t e = launch_behind(blocks::delta_kernel<T>, (unsigned)((rows + 15) / 16), 256, 0, st, a);
+    if (std::is_same<T, __half>::value && e == cudaSuccess)
+        e = launch_behind(blocks::peaks_kernel, (unsigned)((int64_t)s.batch * s.kv_heads * s.words), blocks::kBitsThreads, 0, st, a);
     if (e == cudaSuccess)
         e = launch_behind(blocks::tcore::grad_q_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kGradQThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
     if (e == cudaSuccess)
@@ -296,7 +299,7 @@ VS_EXPORT int vs_select_blocks(int dtype, int batch, int queries, int keys, int 
 VS_EXPORT int64_t vs_selected_attention_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int d, int backward) {
     blocks::Shape s;
     if (check_shape(VS_F16, batch, queries, keys, heads, kv_heads, d, 1, 0, nullptr, s) != VS_OK) return 0;
-    return bits_bytes(s) + redo_bytes(s) + (backward ? up256((int64_t)batch * heads * queries * 4) + 256 : 0);   // the words of its rows, one of the call
+    return bits_bytes(s) + redo_bytes(s) + (backward ? 2 * rows_bytes(s) + up256((int64_t)batch * kv_heads * s.blocks * 4) : 0);   // two words of a row, one of a block
 }
 
 VS_EXPORT int vs_selected_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const void *q,
@@ -352,9 +355,11 @@ VS_EXPORT int vs_selected_attention_backward(int dtype, int batch, int queries, 
     char *at = static_cast<char *>(workspace);
     uint32_t *bits = reinterpret_cast<uint32_t *>(at), *redo = reinterpret_cast<uint32_t *>(at + bits_bytes(a.s));
     a.bits = bits; a.lse = const_cast<float *>(lse); a.scale = scale; a.result = grad_q; a.grad_k = grad_k; a.grad_v = grad_v;
-    a.delta = reinterpret_cast<float *>(at + bits_bytes(a.s) + redo_bytes(a.s));
-    a.most = reinterpret_cast<uint32_t *>(at + bits_bytes(a.s) + redo_bytes(a.s) + up256((int64_t)batch * heads * queries * 4));
-    if ((rc = make_bits(a.s, lists, bits, a.most, st)) != VS_OK) return rc;
+    at += bits_bytes(a.s) + redo_bytes(a.s);
+    a.delta = reinterpret_cast<float *>(at);
+    a.most = reinterpret_cast<uint32_t *>(at + rows_bytes(a.s));
+    a.peak = reinterpret_cast<uint32_t *>(at + 2 * rows_bytes(a.s));
+    if ((rc = make_bits(a.s, lists, bits, a.peak, st)) != VS_OK) return rc;
     return dtype == VS_F16 ? attention_backward<__half>(a, redo, st) : attention_backward<__nv_bfloat16>(a, redo, st);
 }
 

@@ -74,8 +74,9 @@ __global__ void __launch_bounds__(kBitsThreads) bits_kernel(const Shape s, const
     __shared__ uint32_t row[kBitsChunk];
     pdl_launch_dependents();
     const int64_t at = blockIdx.x;
-    if (zero && at == 0 && threadIdx.x == 0) *zero = 0;
     const int w = (int)(at % s.words);
+    if (zero && w == 0)   // a word for each block of a head of keys
+        for (int j = threadIdx.x; j < s.blocks; j += kBitsThreads) zero[at / s.words * s.blocks + j] = 0;
     const int b = (int)(at / s.words / s.kv_heads);
     const int len = s.length(b), rows = s.rows(b);
     const int32_t *list = lists + (at / s.words * s.queries + w * 32) * s.count;
@@ -581,7 +582,8 @@ struct Args {
     const uint32_t *bits;
     float *lse;           // [batch, heads, queries] base 2; +inf: the row attends to nothing
     float *delta;         // the same shape: rowsum(out o grad_out)
-    uint32_t *most;       // largest magnitude in grad_out, as the bits of a float
+    uint32_t *most;       // as lse, fp16 alone: largest finite magnitude of a row of grad_out, as the bits of a float
+    uint32_t *peak;       // [batch, kv_heads, blocks], fp16 alone: the largest of those of the rows that have listed a block
     const void *out_low;  // what rounding left of out, as out; or null
     void *result;         // out or grad_q, contiguous
     void *result_low;     // out_low or null
@@ -755,7 +757,7 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads) keys_kernel
     }
 }
 
-// rowsum(out o grad_out) of each row and the largest magnitude in grad_out; nothing of rows behind a sequence's end.  Eight dimensions to a lane, 16 lanes
+// rowsum(out o grad_out) of each row and, fp16, the largest magnitude of its grad_out that is a finite number; 0 of rows behind a sequence's end.  Eight dimensions to a lane, 16 lanes
 // to a row.  Bound by the reading of its three operands: 262 144 rows, d = 128: 50 us (4.0 TB/s).
 template <typename T> __global__ void __launch_bounds__(256) delta_kernel(const Args a) {
     const Shape &s = a.s;
@@ -778,21 +780,43 @@ template <typename T> __global__ void __launch_bounds__(256) delta_kernel(const 
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             sum = fmaf(o[x], g[x], sum);
-            most = fmaxf(most, fabsf(g[x]));
+            if (std::is_same<T, __half>::value && fabsf(g[x]) <= FLT_MAX) most = fmaxf(most, fabsf(g[x]));
         }
     }
-    const uint32_t all_most = __reduce_max_sync(~0u, __float_as_uint(most));
-    __shared__ uint32_t warps_most[8];
-    if (threadIdx.x % 32 == 0) warps_most[threadIdx.x / 32] = all_most;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        uint32_t top = 0;
-        for (int x = 0; x < 8; ++x) top = max(top, warps_most[x]);
-        if (top > *reinterpret_cast<volatile uint32_t *>(a.most)) atomicMax(a.most, top);   // a maximum: the order does not count
-    }
 #pragma unroll
-    for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (at < all && c == 0) a.delta[((int64_t)b * s.heads + h) * s.queries + i] = sum;
+    for (int o = 8; o; o >>= 1) {
+        sum += __shfl_xor_sync(~0u, sum, o);
+        if (std::is_same<T, __half>::value) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+    }
+    if (at < all && c == 0) {
+        const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+        a.delta[row] = sum;
+        if (std::is_same<T, __half>::value) a.most[row] = __float_as_uint(most);
+    }
+}
+
+// The largest of `most` among the rows that have listed a block: a CTA takes a word of 32 queries, all heads of the group.  Bound by its launch: a
+// training step of 4 x 2048 queries and 16 heads takes 337 us with it and 331 with one maximum for the whole call.
+__global__ void __launch_bounds__(kBitsThreads) peaks_kernel(const Args a) {
+    __shared__ uint32_t query[32];
+    const Shape &s = a.s;
+    const int64_t at = blockIdx.x, bh = at / s.words;
+    const int w = (int)(at % s.words), kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads), lane = threadIdx.x & 31, i = w * 32 + lane;
+    if (threadIdx.x < 32) query[lane] = 0;
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
+    uint32_t most = 0;
+    if (i < s.queries)
+        for (int g = threadIdx.x >> 5; g < s.group; g += kBitsThreads / 32) most = max(most, __ldcg(a.most + ((int64_t)b * s.heads + kvh * s.group + g) * s.queries + i));
+    atomicMax(query + lane, most);   // maxima: the order does not count
+    __syncthreads();
+    for (int j = threadIdx.x; j < s.blocks; j += kBitsThreads) {
+        uint32_t rows = __ldcg(a.bits + at * s.blocks + j), top = 0;
+        if (!rows) continue;
+        for (; rows; rows &= rows - 1) top = max(top, query[__ffs(rows) - 1]);
+        atomicMax(a.peak + bh * s.blocks + j, top);
+    }
 }
 
 }  // namespace blocks

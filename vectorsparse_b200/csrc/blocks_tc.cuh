@@ -546,11 +546,12 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
 // Weights and the scores' gradients are rounded to 16 bits for their products.  fp16 keeps its precision only above 2^-14, so there both are multiplied by powers of
-// two first: the weights, at most 1, by 2^14; the gradients by the one that brings the largest element of grad_out to 32 .. 64 (found by the delta kernel).
+// two first: the weights, at most 1, by 2^14; the gradients by the one that brings the largest finite element of grad_out to 32 .. 64: for dQ the largest of the row, for dK, whose
+// sums join rows, that of the rows that have listed the block.  So no row's gradients depend on how large another's are where the two do not meet in a sum.
 template <typename T> struct Lift {
     static constexpr float kWeight = std::is_same<T, __half>::value ? 14.f : 0.f;   // exponent
     static __device__ __forceinline__ float grad(const uint32_t *most) {
-        if (!std::is_same<T, __half>::value) return 1.f;
+        if constexpr (!std::is_same<T, __half>::value) return 1.f;
         const uint32_t e = __ldcg(most) >> 23;
         return e < 6 || e >= 253 ? 1.f : __uint_as_float((259u - e) << 23);   // 2^(5 - (e - 127))
     }
@@ -724,13 +725,11 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
             if (block < 0) break;
             const bool listed = alive && (e.rows[qx >> 5] >> (qx & 31) & 1u);
             const int n = listed ? min(kBlock, end - block * kBlock) : 0;   // keys of the row
-            if (x == 0) {   // the loader has waited for the kernels that wrote these
-                lift = Lift<T>::grad(a.most);
-                if (there) {
-                    const int64_t row = ((int64_t)t.b * s.heads + h) * s.queries + i;
-                    lse = __ldcg(a.lse + row);
-                    minus_delta = -__ldcg(a.delta + row) * lift;
-                }
+            if (x == 0 && there) {
+                const int64_t row = ((int64_t)t.b * s.heads + h) * s.queries + i;
+                lift = Lift<T>::grad(a.most + row);
+                lse = __ldcg(a.lse + row);
+                minus_delta = -__ldcg(a.delta + row) * lift;
             }
             ok = __all_sync(~0u, wait(base + M::kSP, x & 1, abort_flag));
             if (!ok) break;
@@ -1056,7 +1055,7 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
             }
         };
         look(x);
-        if (ok && more) lift = Lift<T>::grad(a.most) * exp2i(-Lift<T>::kWeight);   // the loader has waited for the kernels that wrote it
+        if (ok && more) lift = Lift<T>::grad(a.peak + bh * s.blocks + j) * exp2i(-Lift<T>::kWeight);
         for (; ok && more; x += M::kGroups) {
             const bool listed = next.listed;
             const int n = next.n;
