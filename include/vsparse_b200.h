@@ -277,7 +277,7 @@ int vs_device_status(int clear, uint32_t *status);
  * strides given as three HOST int64 in elements (batch, token, head), multiples of 8 and, where the dimension is larger than one, not 0.
  * Results are contiguous in the same order.  Device pointers of tensors 16-byte aligned.
  * heads is a multiple of kv_heads: heads / kv_heads (at most 128) query heads share a head of keys, and its list of blocks.
- * d: a multiple of 8 up to 128.  keys: up to 1 048 576.
+ * d: a multiple of 8 up to 128.  keys: up to 1 048 576; queries: up to 2^31 - 65 536; count, here and below: up to 67 108 863.
  * Query i stands at position p = i + keys - queries.  causal != 0 (then queries <= keys): it attends to keys t <= p.
  * lengths (or NULL): int32 [batch], how many tokens of a padded batch are there (queries == keys); queries behind the end attend to
  * nothing, keys behind it are not attended to, and what stands there is not looked at.

@@ -119,3 +119,16 @@ def test_the_plain_choice():
     got = plain.select(q, k, 2, True, None)                 # queries at positions 70 .. 199
     assert got[0, 0, 0].tolist() == [0, 1] and got[0, 0, 58].tolist() == [1, 2] and got[0, 0, 129].tolist() == [1, 3]
     assert plain.top(np.array([1.0, np.nan, 1.0, np.inf]), None, 3) == [0, 2, 3] and plain.top(np.array([]), 0, 2) == [0, -1]
+
+
+def test_sizes_whose_indices_leave_32_bits_are_refused():
+    """Queries are counted in words of 32 and tiles of 128 that reach past the last one, the entries of 32 lists by one number, and the places behind a list's end in steps of 32."""
+    L, most, many = _lib.lib(), 0x7fff0000, (2 ** 31 - 1) // 32
+    assert attention(queries=most + 1, keys=64, causal=0) == -3
+    assert attention(queries=2 ** 31 - 1, keys=64, causal=0) == -3
+    assert L.vs_selected_attention_workspace_bytes(1, most, 64, 1, 1, 8, 1) > L.vs_selected_attention_workspace_bytes(1, most - 64, 64, 1, 1, 8, 1) > 0
+    assert L.vs_selected_attention_workspace_bytes(1, most + 1, 64, 1, 1, 8, 1) == 0
+    assert attention(count=many + 1) == -3
+    assert L.vs_select_blocks(F16, 1, 8, 8, 1, 1, 64, many + 1, 1, P, STRIDES, P, STRIDES, None, P, P, 1 << 40, None) == -3
+    assert L.vs_cache_select(BF16, 1, 2, 1, 64, P, P, 1, P, STRIDES, P, 1, P, many + 1, P, None) == -3
+    assert L.vs_cache_attention(F16, 1, 1, 2, 1, 64, P, P, P, P, P, P, 1, P, STRIDES, P, 1000, P, P, P, many + 1, P, C.c_float(1.0), P, 1 << 40, None) == -3

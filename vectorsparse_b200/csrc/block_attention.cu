@@ -62,7 +62,7 @@ int check_shape(int dtype, int batch, int queries, int keys, int heads, int kv_h
     if (batch < 0 || queries < 0 || keys < 0) return VS_ERR_SHAPE;
     if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads / kv_heads > 128) return VS_ERR_SHAPE;
     if (d < 8 || d > blocks::kMaxD || d % 8 != 0) return VS_ERR_SHAPE;
-    if (count < 1 || keys > blocks::kMaxBlocks * blocks::kBlock) return VS_ERR_SHAPE;
+    if (count < 1 || count > blocks::kMaxCount || queries > blocks::kMaxQueries || keys > blocks::kMaxBlocks * blocks::kBlock) return VS_ERR_SHAPE;
     if (causal != 0 && causal != 1) return VS_ERR_ARG;
     if (causal && queries > keys) return VS_ERR_SHAPE;
     if (lengths && queries != keys) return VS_ERR_SHAPE;
@@ -447,7 +447,7 @@ VS_EXPORT int vs_cache_select(int dtype, int pages, int heads, int kv_heads, int
                               int32_t *lists, void *stream) {
     int rc = check_cache(dtype, pages, 0, kv_heads, d, sequences, max_blocks);
     if (rc != VS_OK) return rc;
-    if (heads < kv_heads || heads % kv_heads != 0 || count < 1 || max_blocks > blocks::kMaxBlocks) return VS_ERR_SHAPE;
+    if (heads < kv_heads || heads % kv_heads != 0 || count < 1 || count > blocks::kMaxCount || max_blocks > blocks::kMaxBlocks) return VS_ERR_SHAPE;
     if (sequences == 0) return VS_OK;
     if (!q || !q_strides || !lengths || !lists || (max_blocks > 0 && !table) || (pages > 0 && (!k_scales || !k_sums))) return VS_ERR_NULL;
     if (!aligned16(q) || !aligned16(k_sums)) return VS_ERR_ALIGN;
@@ -487,7 +487,7 @@ VS_EXPORT int vs_cache_attention(int dtype, int pages, int tails, int heads, int
                                  const int32_t *lists, int count, void *out, float scale, void *workspace, int64_t workspace_bytes, void *stream) {
     int rc = check_cache(dtype, pages, tails, kv_heads, d, sequences, max_blocks);
     if (rc != VS_OK) return rc;
-    if (heads < kv_heads || heads % kv_heads != 0 || (lists && count < 1)) return VS_ERR_SHAPE;
+    if (heads < kv_heads || heads % kv_heads != 0 || (lists && (count < 1 || count > blocks::kMaxCount))) return VS_ERR_SHAPE;
     if (!scale_ok(scale)) return VS_ERR_ARG;
     if (sequences == 0) return VS_OK;
     if (!q || !q_strides || !lengths || !out || !tail_indices || (max_blocks > 0 && !table) || (pages > 0 && (!k_codes || !v_codes || !k_scales || !v_scales)) ||

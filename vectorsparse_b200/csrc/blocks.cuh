@@ -23,6 +23,8 @@ namespace blocks {
 constexpr int kBlock = 64;
 constexpr int kMaxD = 128;
 constexpr int kMaxBlocks = 16384;   // per sequence: scores of one query fit in shared memory
+constexpr int kMaxQueries = 0x7fff0000;      // tiles and chunks of tiles that reach past the last query are counted in 32 bits
+constexpr int kMaxCount = 0x7fffffff / 32;   // entries of a list: those of a word's 32 lists too
 
 struct Shape {
     int batch, queries, keys, heads, kv_heads, d, count;
