@@ -350,3 +350,27 @@ def test_selection_of_equal_scores_and_missing_pages(blocks):
             order = [j for j in best[r] if j != blocks - 1] + [j for j in range(blocks - 1) if j not in best[r] and j != gone]
             want = sorted(order[:count - 1] + [blocks - 1])
             assert got[r, 0, :len(want)].tolist() == want and (got[r, 0, len(want):] == -1).all(), (count, r)
+
+
+def test_per_sequence_tensors_of_another_shape_are_refused():
+    """lengths, tails and counts have one dimension: of as many elements in two, the binding's quick path is no more permissive than the operators."""
+    m = Model(2, 3, 1, 64, torch.float16)
+    x = torch.randn(2, 70, 1, 64, device=DEV, dtype=torch.float16)
+    q, lengths, (table, tails) = x[:, :2].reshape(2, 2, 64), m.lengths(), m.dev
+    m.append(x, x)
+    for call in (lambda **k: torch_ops.cache_append(m.cache, x, x, table, k.get("tails", tails), k.get("lengths", lengths), k.get("counts")),
+                 lambda **k: torch_ops.cache_attention(q, m.cache, table, k.get("tails", tails), k.get("lengths", lengths), 0.125)):
+        for name in ("tails", "lengths"):
+            with pytest.raises(ValueError):
+                call(**{name: lengths[:, None]})
+    with pytest.raises(ValueError):
+        torch_ops.cache_append(m.cache, x, x, table, tails, lengths, lengths[None])
+    with pytest.raises(ValueError):
+        torch_ops.cache_select(q, m.cache, table, lengths[:, None], 1)
+    m.check()
+    q4, blocks = x[:, :, :, None].reshape(2, 70, 1, 64), torch.zeros((2, 1, 70, 1), dtype=torch.int32, device=DEV)
+    n = torch.tensor([70, 3], dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError):
+        torch_ops.select_blocks(q4, q4, 1, lengths=n[:, None])
+    with pytest.raises(ValueError):
+        torch_ops.selected_attention(q4, q4, q4, blocks, 0.125, lengths=n[None])

@@ -136,12 +136,12 @@ struct Args {
         ok = false;
         return -1;
     }
-    // a contiguous int32 tensor of exactly this many elements, or null for None
+    // a contiguous int32 tensor of one dimension and exactly this many elements, or null for None
     const int32_t *exactly(int i, int64_t numel) {
         if (none(i)) return nullptr;
         const at::Tensor *t = tensor(i);
         type(t, at::kInt);
-        if (ok && t->numel() != numel) ok = false;
+        if (ok && (t->dim() != 1 || t->numel() != numel)) ok = false;
         return ok ? static_cast<const int32_t *>(t->const_data_ptr()) : nullptr;
     }
     void need(const at::Tensor *t, int64_t numel) {
