@@ -462,7 +462,7 @@ VS_EXPORT int vs_cache_select(int dtype, int pages, int heads, int kv_heads, int
     a.s = {sequences, table, max_blocks, nullptr, lengths};
     a.q = q; a.batch = q_strides[0]; a.head = q_strides[1];
     a.group = heads / kv_heads; a.wanted = count; a.lists = lists;
-    const int smem = (int)((int64_t)max_blocks * 8 + (max_blocks + 31) / 32 * 4), threads = max_blocks > 256 ? 1024 : 256;
+    const int smem = (int)((int64_t)max_blocks * 8 + (max_blocks + 31) / 32 * 4), threads = max_blocks > 256 ? cache::kSelectThreads : 256;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == VS_F16) {
         if ((rc = allow_smem<cache::select_kernel<__half>>(smem)) != VS_OK) return rc;

@@ -208,6 +208,7 @@ template <typename T> __global__ void __launch_bounds__(kAppendThreads, 12) appe
 // Score of a complete block: (sum of the group's query heads) . (sum of the block's codes) * scale, in 64 bits.  The newest complete block is always
 // taken.  A CTA per (sequence, kv head); 16 lanes take a block's sums, 8 dimensions each, four blocks in flight.  Bound by 64-bit products and the sums over
 // lanes, then by the ranking: 64 sequences of up to 256 blocks, 8 heads, d = 128: 22 us (26 MB, 1.2 TB/s).
+constexpr int kSelectThreads = 1024;   // at most
 struct SelectArgs {
     Pages c;
     Sequences s;
@@ -216,7 +217,7 @@ struct SelectArgs {
     int group, wanted;
     int32_t *lists;      // [count][kv heads][wanted]
 };
-template <typename T> __global__ void select_kernel(const SelectArgs a) {
+template <typename T> __global__ void __launch_bounds__(kSelectThreads) select_kernel(const SelectArgs a) {
     extern __shared__ double sm[];
     const int d = a.c.d, h = blockIdx.x % a.c.kv_heads, r = blockIdx.x / a.c.kv_heads;
     const int full = min(max(a.s.lengths[r], 0) / kBlock, a.s.max_blocks);
