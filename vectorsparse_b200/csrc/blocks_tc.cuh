@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder);
     const uint32_t tmem_o = tmem + 128;
     bool bad = false;
-    pdl_launch_dependents();
+    pdl_launch_dependents();   // behind the allocation, as in the kernels below
 
     pdl_wait();   // all roles: the bounded waits below are for this kernel's own work, not for that of kernels before it
     if (warp == 8) {
@@ -585,7 +585,6 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
     const Shape &s = a.s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Tile t = tile_of(s, a.tile, blockIdx.x);
-    pdl_launch_dependents();
     if (base & 1023u) {   // there is no room for a margin: a tile whose memory does not start where the swizzle needs it is left to the kernel behind
         pdl_wait();
         if (threadIdx.x == 0) redo[t.index] = 1;
@@ -610,6 +609,8 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
     tc::tc_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder);
     bool bad = false;
+    // Behind the allocation: the next kernel's CTAs take tensor memory before they wait for this one, and an allocation here must not wait for theirs.
+    pdl_launch_dependents();
 
     pdl_wait();   // all roles: the bounded waits below are for this kernel's own work, not for that of kernels before it
     if (warp == 8) {
@@ -837,7 +838,6 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
     const int64_t bh = blockIdx.x % ((int64_t)s.batch * s.kv_heads);   // the first blocks have most queries behind them: they go first, of all heads
     const int j = (int)(blockIdx.x / ((int64_t)s.batch * s.kv_heads)), kvh = (int)(bh % s.kv_heads), b = (int)(bh / s.kv_heads);
     const int len = s.length(b), live = a.tile * s.group;
-    pdl_launch_dependents();
     if (base & 1023u) {   // as in the kernel above
         pdl_wait();
         if (threadIdx.x == 0) redo[bh * s.blocks + j] = 1;
@@ -865,6 +865,7 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
     tc::tc_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + M::kHolder), tmem_acc = tmem + M::kBuffers * 128;
     bool bad = false;
+    pdl_launch_dependents();
 
     pdl_wait();   // all roles: the bounded waits below are for this kernel's own work, not for that of kernels before it
     if (warp == 8) {
