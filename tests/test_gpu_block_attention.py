@@ -501,3 +501,35 @@ def test_small_gradients_beside_a_row_of_large_ones(D, q_size, k_size, value):
     for name, a, want, m, floor, not_here in zip(("grad_q", "grad_k", "grad_v"), got, plain.attention(*args)[1:], magnitudes(*args)[1:], below, reached):
         error = np.where(not_here, 0, np.abs(plain.f64(a) - want))
         assert (error <= (3 * u + 2.0 ** -18) * m + u * np.abs(want) + floor + 2.0 ** -24).all(), (name, float(error.max()))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("queries", [255, 256, 257, 512, 513, 1025, 3100, 60000])
+def test_key_gradients_of_blocks_that_very_many_tiles_have_listed(D, queries):
+    """Sums of one sign over as many tiles as there are queries: 128 heads, so a tile is one.
+
+    A sum in tensor memory is cut off, by less than 2^-21 of itself, in each of 8 steps to a tile, 256 tiles at a stretch: 2^-10 besides the roundings of the
+    terms, and 2^-18 for the stretches' own sum in fp32."""
+    g = torch.Generator(DEV).manual_seed(queries + D)
+    q, grad = (torch.randn((1, queries, 128, D), generator=g, device=DEV) for _ in range(2))
+    k, v = ((0.25 * torch.randn((1, 100, 1, D), generator=g, device=DEV)).half() for _ in range(2))
+    q, grad = q.half(), grad.abs().mul_(0.25).half()
+    blocks = torch.tensor([0, 1], dtype=torch.int32, device=DEV).expand(1, 1, queries, 2).contiguous()
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    _, got_k, got_v = torch.autograd.grad(torch_ops.selected_attention(*leaves, blocks, 0.125, False), leaves, grad)
+    assert ops.device_status() == 0
+    want_k, want_v, size_k = (torch.zeros((100, D), dtype=torch.float64, device=DEV) for _ in range(3))
+    k64, v64 = k[0, :, 0].double(), v[0, :, 0].double()
+    for x, d in zip(q[0].view(-1, D).split(1 << 18), grad[0].view(-1, D).split(1 << 18)):
+        x, d = x.double(), d.double()
+        p = (x @ k64.T * 0.125).softmax(-1)
+        dp = d @ v64.T
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * 0.125
+        sizes = d @ v64.T.abs()
+        sizes = p * (sizes + (p * sizes).sum(-1, keepdim=True)) * 0.125
+        want_v += p.T @ d
+        want_k += ds.T @ x
+        size_k += sizes.T @ x.abs()
+    u, steps = torch.finfo(torch.float16).eps / 2, 2.0 ** -10 + 2.0 ** -18
+    assert ((got_v[0, :, 0].double() - want_v).abs() <= (2 * u + steps) * want_v).all()
+    assert ((got_k[0, :, 0].double() - want_k).abs() <= (3 * u + steps) * size_k + u * want_k.abs() + 2.0 ** -24).all()

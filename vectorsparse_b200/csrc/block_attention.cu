@@ -95,14 +95,18 @@ inline int64_t up256(int64_t bytes) { return (bytes + 255) & ~255ll; }
 inline int64_t bits_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * s.words * s.blocks * 4); }
 
 inline int64_t rows_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.heads * s.queries * 4); }
-inline int64_t redo_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * ((int64_t)s.queries + s.blocks) * 4); }   // a word per tile and block
-
 // Queries of a tile: the largest power of two whose rows (queries x heads of the group) fit 128.
 inline int tile_queries(int group) {
     int t = 128;
     while (t * group > 128) t /= 2;
     return t;
 }
+// Where a block can have more tiles than are summed at a stretch: what is put aside.
+inline int64_t aside_bytes(const blocks::Shape &s) {
+    const int tile = tile_queries(s.group);
+    return s.queries / tile < (int)blocks::tcore::kRun ? 0 : (int64_t)s.batch * s.kv_heads * s.blocks * 4 * (s.d <= 64 ? blocks::tcore::GradKVSmem<64>::kAside : blocks::tcore::GradKVSmem<128>::kAside);
+}
+inline int64_t redo_bytes(const blocks::Shape &s) { return up256((int64_t)s.batch * s.kv_heads * ((int64_t)s.queries + s.blocks) * 4); }   // a word per tile and block
 
 template <typename T, int QT> int launch_scores(const blocks::Shape &s, const blocks::Operand &q, const double *means, int32_t *lists, cudaStream_t st) {
     const int smem = (int)blocks::score_bytes<QT>(s.blocks, s.d);
@@ -299,7 +303,7 @@ VS_EXPORT int vs_select_blocks(int dtype, int batch, int queries, int keys, int 
 VS_EXPORT int64_t vs_selected_attention_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int d, int backward) {
     blocks::Shape s;
     if (check_shape(VS_F16, batch, queries, keys, heads, kv_heads, d, 1, 0, nullptr, s) != VS_OK) return 0;
-    return bits_bytes(s) + redo_bytes(s) + (backward ? 2 * rows_bytes(s) + up256((int64_t)batch * kv_heads * s.blocks * 4) : 0);   // two words of a row, one of a block
+    return bits_bytes(s) + redo_bytes(s) + (backward ? 2 * rows_bytes(s) + up256((int64_t)batch * kv_heads * s.blocks * 4) + aside_bytes(s) : 0);   // two words of a row, one of a block
 }
 
 VS_EXPORT int vs_selected_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int d, int count, int causal, const void *q,
@@ -359,6 +363,7 @@ VS_EXPORT int vs_selected_attention_backward(int dtype, int batch, int queries, 
     a.delta = reinterpret_cast<float *>(at);
     a.most = reinterpret_cast<uint32_t *>(at + rows_bytes(a.s));
     a.peak = reinterpret_cast<uint32_t *>(at + 2 * rows_bytes(a.s));
+    a.aside = reinterpret_cast<float *>(at + 2 * rows_bytes(a.s) + up256((int64_t)batch * kv_heads * a.s.blocks * 4));
     if ((rc = make_bits(a.s, lists, bits, a.peak, st)) != VS_OK) return rc;
     return dtype == VS_F16 ? attention_backward<__half>(a, redo, st) : attention_backward<__nv_bfloat16>(a, redo, st);
 }

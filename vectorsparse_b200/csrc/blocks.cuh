@@ -590,6 +590,7 @@ struct Args {
     void *result;         // out or grad_q, contiguous
     void *result_low;     // out_low or null
     void *grad_k, *grad_v;
+    float *aside;         // sums that grad_kv_kernel has put aside, where a block can have more tiles than it sums at a stretch
     const uint32_t *redo;
     int tile;
     float scale;

@@ -809,6 +809,11 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 // Bound by shared memory and hand-overs: a tile's products read 192 KB of operands there (1540 cycles), its copies and P, dS write 96 KB (770), and it takes 3200: the
 // tiles above 837 us, 0.71 PFLOP/s on them (938 with four places, one group and one wait after another).  A block that most later queries have listed (up to 392
 // tiles there, 138 on average) is one CTA's work and starts first.
+//
+// Sums in tensor memory are cut off, not rounded: one whose terms have one sign loses some 1.6 x 2^-23 of itself in every step (8 to a tile), 7.9e-4 of dV by 1024 tiles and
+// 4.6 % by 60 000.  So after kRun tiles the first group puts them aside, where they are added in fp32, and they begin anew: 2.0e-4 however many there are, less than half of
+// fp16's own rounding.  The tiles above take 17 us more with it; runs of 128 lose 1.0e-4 and take 57.
+constexpr uint32_t kRun = 256;
 template <int DP> struct GradKVSmem {
     static constexpr int kBuffers = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;   // of S and dP; CTAs an SM
     // Q and dO of tile x are copies 2 x and 2 x + 1, copy n in place n % kPlaces; d <= 64: always Q in an even one, dO behind it
@@ -824,6 +829,8 @@ template <int DP> struct GradKVSmem {
                          kAbort = kDrain + 8, kHolder = kAbort + 4;
     static constexpr int kChunk = 512;
     static_assert(kHolder + 4 <= kChunk && kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
+    static_assert(kRun % kGroups == 0, "the first group's tile begins a run");
+    static constexpr int kAside = 2 * kBlock * DP;   // sums of a block
 };
 template <typename T, int DP>
 __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCtas) grad_kv_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
@@ -976,15 +983,15 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
                     if constexpr (DP == 64) {   // rows of the result: Q's dimensions, then dO's; columns: with P, then with dS
 #pragma unroll
                         for (int k = 0; k < kRows / 16; ++k)
-                            tc::mma_f16_ss(tmem_acc, tc::desc64(q_at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, summed > 0 || k > 0);
+                            tc::mma_f16_ss(tmem_acc, tc::desc64(q_at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, summed % kRun > 0 || k > 0);
                     } else {
 #pragma unroll
                         for (int k = 0; k < kRows / 16; ++k)
-                            tc::mma_f16_ss(tmem_acc + 64, tc::desc64(q_at + 128 * k, hi), tc::desc64(ds_lo + 128 * k, hi), kIdescG, summed > 0 || k > 0);
+                            tc::mma_f16_ss(tmem_acc + 64, tc::desc64(q_at + 128 * k, hi), tc::desc64(ds_lo + 128 * k, hi), kIdescG, summed % kRun > 0 || k > 0);
                         tc::mma_commit(base + M::kEmpty + 8 * q_sum.place);
 #pragma unroll
                         for (int k = 0; k < kRows / 16; ++k)
-                            tc::mma_f16_ss(tmem_acc, tc::desc64(g_at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, summed > 0 || k > 0);
+                            tc::mma_f16_ss(tmem_acc, tc::desc64(g_at + 128 * k, hi), tc::desc64(p_lo + 128 * k, hi), kIdescG, summed % kRun > 0 || k > 0);
                     }
                     tc::mma_commit(base + M::kDone + 8 * (summed & 1));
                     if (DP == 64) tc::mma_commit(base + M::kEmpty + 8 * q_sum.place);
@@ -1055,9 +1062,29 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
                 next.delta = __ldcg(a.delta + row);
             }
         };
+        // accumulators: a dimension to a lane, keys in columns.  d > 64: dV in columns 0 .. 63, dK in 64 ..; d <= 64: dK in lanes 0 .. 63 of columns 64 ..,
+        // dV in lanes 64 .. of columns 0 ..  The two halves of the first group's warps take one of the two each, or 32 keys each.
+        const bool is_k = DP == 64 ? quarter < 2 : half == 1;
+        constexpr int kParts = DP == 64 ? 1 : 2;
+        const uint32_t sums_at = tmem_acc + ((uint32_t)(quarter * 32) << 16) + (is_k ? 64 : 0) + (DP == 64 ? 32 * half : 0);
+        float *aside = a.aside + (bh * s.blocks + j) * M::kAside + threadIdx.x;
         look(x);
         if (ok && more) lift = Lift<T>::grad(a.peak + bh * s.blocks + j) * exp2i(-Lift<T>::kWeight);
         for (; ok && more; x += M::kGroups) {
+            if (x > 0 && x % kRun == 0) {   // the first group: its P and dS, without which the next product does not start, are not there yet
+                if (!(ok = __all_sync(~0u, wait(base + M::kDone + 8 * ((x - 1) & 1), ((x - 1) >> 1) & 1, abort_flag)))) break;
+                tc::tc_fence_after_sync();
+#pragma unroll 1
+                for (int part = 0; part < kParts; ++part) {
+                    uint32_t o[32];
+                    tc::tmem_ld_x32(sums_at + 32 * part, o);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) {
+                        float *to = aside + (part * 32 + y) * 256;
+                        *to = x > kRun ? *to + __uint_as_float(o[y]) : __uint_as_float(o[y]);
+                    }
+                }
+            }
             const bool listed = next.listed;
             const int n = next.n;
             const float base2 = next.lse - Lift<T>::kWeight, minus_delta = -next.delta * lift;
@@ -1103,25 +1130,22 @@ __global__ void __launch_bounds__(GradKVSmem<DP>::kThreads, GradKVSmem<DP>::kCta
         // free, ahead of that tile's kDone: a wait for kDone could take an earlier phase for the last one.  kDrain has one phase, behind the last product.
         if (ok && total > 0) ok = __all_sync(~0u, wait(base + M::kDrain, 0, abort_flag));
         if (ok && group == 0) {
-            // accumulators: a dimension to a lane, keys in columns.  d > 64: dV in columns 0 .. 63, dK in 64 ..; d <= 64: dK in lanes 0 .. 63 of columns 64 ..,
-            // dV in lanes 64 .. of columns 0 ..  The two halves of the warps take one of the two each, or 32 keys each.
             tc::tc_fence_after_sync();
             const float back_v = exp2i(-Lift<T>::kWeight), back_k = total > 0 ? a.scale / (lift * exp2i(Lift<T>::kWeight)) : 0.f;
-            const uint32_t lanes = tmem_acc + ((uint32_t)(quarter * 32) << 16);
-            const bool is_k = DP == 64 ? quarter < 2 : half == 1;
             const int dim = (DP == 64 ? quarter % 2 : quarter) * 32 + lane;
             const float back = is_k ? back_k : back_v;
             T *out = static_cast<T *>(is_k ? a.grad_k : a.grad_v) + (((int64_t)b * s.keys + j * kBlock) * s.kv_heads + kvh) * s.d + dim;
             const int64_t pitch = (int64_t)s.kv_heads * s.d;
             const int keys = min(kBlock, s.keys - j * kBlock);
 #pragma unroll
-            for (int part = 0; part < (DP == 64 ? 1 : 2); ++part) {
+            for (int part = 0; part < kParts; ++part) {
                 const int first = DP == 64 ? 32 * half : 32 * part;
                 uint32_t o[32];
-                if (total > 0) tc::tmem_ld_x32(lanes + (is_k ? 64 : 0) + first, o);
+                if (total > 0) tc::tmem_ld_x32(sums_at + 32 * part, o);
 #pragma unroll
                 for (int y = 0; y < 32; ++y) {
-                    const float f = total > 0 ? __uint_as_float(o[y]) * back : 0.f;
+                    const float sum = total > kRun ? __uint_as_float(o[y]) + aside[(part * 32 + y) * 256] : __uint_as_float(o[y]);
+                    const float f = total > 0 ? sum * back : 0.f;
                     if (dim < s.d && first + y < keys) {
                         bad |= !finite(f);
                         out[(first + y) * pitch] = from_f32<T>(f);
