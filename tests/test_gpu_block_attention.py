@@ -533,3 +533,35 @@ def test_key_gradients_of_blocks_that_very_many_tiles_have_listed(D, queries):
     u, steps = torch.finfo(torch.float16).eps / 2, 2.0 ** -10 + 2.0 ** -18
     assert ((got_v[0, :, 0].double() - want_v).abs() <= (2 * u + steps) * want_v).all()
     assert ((got_k[0, :, 0].double() - want_k).abs() <= (3 * u + steps) * size_k + u * want_k.abs() + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("count", [255, 256, 257, 513, 1025, 4100])
+def test_long_lists(D, count):
+    """Sums of one sign over many blocks.  A sum in tensor memory is cut off, by less than 2^-21 of itself, in each of 4 steps to a block, 256 blocks at a stretch: 2^-11 besides
+    the roundings of the weights and of the result, and 2^-18 for fp32."""
+    g = torch.Generator(DEV).manual_seed(count + D)
+    q, k, v = (torch.randn(s, generator=g, device=DEV) for s in ((1, 70, 2, D), (1, 64 * count, 1, D), (1, 64 * count, 1, D)))
+    q, k, v = q.mul_(0.25).half(), k.half(), v.abs_().half()
+    blocks = torch.arange(count, dtype=torch.int32, device=DEV).expand(1, 1, 70, count).contiguous()
+    got = torch_ops.selected_attention(q, k, v, blocks, D ** -0.5, False)[0].double()
+    assert ops.device_status() == 0
+    want = torch.einsum("hqk,kd->qhd", (torch.einsum("qhd,kd->hqk", q[0].double(), k[0, :, 0].double()) * D ** -0.5).softmax(-1), v[0, :, 0].double())
+    u = torch.finfo(torch.float16).eps / 2
+    assert ((got - want).abs() <= (2 * u + 2.0 ** -11 + 2.0 ** -18) * want).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [40, 128])
+def test_long_lists_of_unlike_rows(dtype, D):
+    """Rows that begin after other rows' sums have been put aside, end before, miss blocks in between or have none; scores that grow along the sequence."""
+    q, k, v, grad = tensors(1, 44, 64 * 700 + 9, 4, 2, D, dtype, 23)
+    k = (k.float() * torch.linspace(0.1, 3, k.shape[1], device=DEV)[None, :, None, None]).to(dtype)
+    rng = np.random.default_rng(23)
+    blocks = np.full((1, 2, 44, 320), -1, np.int32)
+    for h in range(2):
+        for i in range(44):
+            lo, hi = [(0, 701), (300, 701), (0, 200), (650, 660), (700, 701), (256, 257), (0, 0)][i % 7]
+            some = rng.permutation(np.arange(lo, hi))[:320 if i % 3 else 300]
+            blocks[0, h, i, :len(some)] = some
+    check(dtype, q, k, v, torch.from_numpy(blocks).to(DEV), D ** -0.5, False, None, grad)

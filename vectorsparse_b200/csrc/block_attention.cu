@@ -200,18 +200,18 @@ inline bool few(const blocks::Shape &s) {
     return (int64_t)s.batch * s.queries * s.heads <= 64 && (int64_t)s.batch * s.queries * s.heads * std::min<int64_t>(s.keys, (int64_t)s.count * blocks::kBlock) <= 64;
 }
 
-template <typename T, int DP> int forward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
+template <typename T, int DP, bool kLong> int forward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
     const blocks::Shape &s = a.s;
-    using Smem = blocks::tcore::ForwardSmem<DP>;
+    using Smem = blocks::tcore::ForwardSmem<DP, kLong>;
     CUtensorMap q, k, v;
     a.tile = tile_queries(s.group);
     int rc = make_map<T>(&q, a.q, s.batch, s.queries, s.heads, s.d, s.group, a.tile);
     if (rc == VS_OK) rc = make_map<T>(&k, a.k, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
     if (rc == VS_OK) rc = make_map<T>(&v, a.v, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
-    if (rc == VS_OK) rc = allow_smem<blocks::tcore::forward_kernel<T, DP>>(Smem::kBytes + 1024);
+    if (rc == VS_OK) rc = allow_smem<blocks::tcore::forward_kernel<T, DP, kLong>>(Smem::kBytes + 1024);
     if (rc != VS_OK) return rc;
     const int64_t tiles = query_tiles(s);
-    cudaError_t e = launch_behind(blocks::tcore::forward_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kForwardThreads, Smem::kBytes + 1024, st, a, q, k, v, redo, status);
+    cudaError_t e = launch_behind(blocks::tcore::forward_kernel<T, DP, kLong>, (unsigned)tiles, blocks::tcore::kForwardThreads, Smem::kBytes + 1024, st, a, q, k, v, redo, status);
     if (e != cudaSuccess) return (int)e;
     a.redo = redo;
     return (int)launch_behind(blocks::rows_kernel<T, false>, again_grid(tiles), blocks::kRowThreads, 0, st, a);
@@ -227,7 +227,8 @@ template <typename T> int attention(blocks::Args a, uint32_t *redo, cudaStream_t
     uint32_t *status = nullptr;
     const int rc = current_device(&sms, &status);
     if (rc != VS_OK) return rc;
-    return s.d <= 64 ? forward<T, 64>(a, redo, status, st) : forward<T, 128>(a, redo, status, st);
+    if (std::min(s.count, s.blocks) > (int)blocks::tcore::kRun) return s.d <= 64 ? forward<T, 64, true>(a, redo, status, st) : forward<T, 128, true>(a, redo, status, st);
+    return s.d <= 64 ? forward<T, 64, false>(a, redo, status, st) : forward<T, 128, false>(a, redo, status, st);
 }
 template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
     const blocks::Shape &s = a.s;

@@ -156,6 +156,10 @@ struct __align__(16) Entry {
 };
 constexpr int kEntries = 8;   // in a ring: more than there are blocks between the loader and the softmax
 
+// Sums in tensor memory are cut off, not rounded: one whose terms have one sign loses some 1.6 x 2^-23 of itself in every step of 16 terms.  After so many products of a tile or block
+// (4 steps each in forward, 8 for dK and dV) a sum is put aside, added in fp32, and begun anew; what it has lost by then, 1.1e-4 and 2.0e-4, is less than half of fp16's own rounding.
+constexpr uint32_t kRun = 256;
+
 struct Tile {   // where a CTA's tile lies
     int b, kvh, i0;
     int64_t bh, index;   // index: among all tiles, in the order of the queries
@@ -264,23 +268,28 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const float *f) {
 // 32 heads on 4, d = 128, 16 blocks each (158 000 tiles of 128 x 64).  Now 637 us: 1.04 PFLOP/s on the tiles, 0.41 on the pairs that the lists name, the unions being
 // 2.5 times as long as a list.  The waits of a step's products taken together: 652 before.  Two blocks to a step, and a loader that stays together as a warp, were slower.
 constexpr float kSlack = 8.f;
-template <int DP> struct ForwardSmem {
+// kLong: lists of more than kRun blocks.  O is put aside in tensor memory every kRun blocks of the union: without it results were 4.3e-4 too small by 1024 blocks and 6.9e-3 by 16384, and
+// the gradients of q, which read them, off by 0.17 and 11 %.  d > 64: that takes the columns of both CTAs, so one to an SM.  2048 queries, 8 heads on
+// 2, 1024 blocks each: d = 128 1040 us (1037 without), d = 64 856 (826).
+template <int DP, bool kLong> struct ForwardSmem {
     static constexpr int kSlots = DP == 128 ? 4 : 6;
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
-    static constexpr int kQ = 3 * 1024, kRing = kQ + kQBytes, kBytes = kRing + kSlots * kSlotBytes;   // ahead: entries, barriers, a chunk of the scan, 2 KB for the rows' threads
+    static constexpr int kQ = 3 * 1024, kRing = kQ + kQBytes, kUsed = kRing + kSlots * kSlotBytes;   // ahead: entries, barriers, a chunk of the scan, 2 KB for the rows' threads
+    static constexpr uint32_t kColumns = kLong && DP == 128 ? 512 : 256;   // of tensor memory: S twice, O, and what is put aside
+    static constexpr int kBytes = kColumns > 256 ? 120 * 1024 : kUsed;     // no second CTA that would wait for the first one's columns
     static constexpr int kEntriesAt = 0, kBars = kEntries * sizeof(Entry);
     static constexpr int kBarQ = kBars, kFull = kBarQ + 8, kEmpty = kFull + 8 * kSlots, kS = kEmpty + 8 * kSlots, kP = kS + 16, kPv = kP + 16, kDrain = kPv + 16, kAbort = kDrain + 8,
                          kHolder = kAbort + 4;
     static constexpr int kChunk = 512, kMeet = 1024;
     static_assert(kHolder + 4 <= kChunk && kMeet + 4 * kRows * 4 <= kQ, "head");
-    static_assert(2 * (kBytes + 2048) <= 228 * 1024, "two CTAs an SM");
+    static_assert(2 * (kUsed + 2048) <= 228 * 1024 && kUsed <= kBytes && (kColumns > 256) == (2 * (kBytes + 2048) > 228 * 1024), "two CTAs an SM, or one");
 };
 constexpr int kForwardThreads = 320;
 
-template <typename T, int DP>
+template <typename T, int DP, bool kLong>
 __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v, uint32_t *redo, uint32_t *status) {
-    using M = ForwardSmem<DP>;
+    using M = ForwardSmem<DP, kLong>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = tc::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *sm = smem_raw + (base - raw);
@@ -306,7 +315,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         tc::fence_mbar_init();
     }
     if (warp == 9) {
-        tc::tmem_alloc(base + M::kHolder, 256);
+        tc::tmem_alloc(base + M::kHolder, M::kColumns);
         tc::tmem_relinquish();
     }
     tc::tc_fence_before_sync();
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             if (leader) {
 #pragma unroll
                 for (int k = 0; k < kBlock / 16; ++k)
-                    tc::mma_f16_ts(tmem_o, tmem + (y & 1) * 64 + 8 * k, tc::desc64(v_lo + slot * (M::kSlotBytes >> 4) + 128 * k, hi), kIdescO, y > 0 || k > 0);
+                    tc::mma_f16_ts(tmem_o, tmem + (y & 1) * 64 + 8 * k, tc::desc64(v_lo + slot * (M::kSlotBytes >> 4) + 128 * k, hi), kIdescO, (kLong ? y % kRun : y) > 0 || k > 0);
                 tc::mma_commit(base + M::kPv + 8 * (y & 1));
                 tc::mma_commit(base + M::kEmpty + 8 * slot);
             }
@@ -427,6 +436,8 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
         const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
         const float c = a.scale * kLog2e;
         float top = -INFINITY, total = 0.f;   // what the weights are relative to, and the sum of this thread's
+        float aside_top = -INFINITY;          // what those of the sums put aside were relative to
+        auto aside_scale = [&] { return aside_top == -INFINITY ? 0.f : ex2(aside_top - top); };
         uint32_t x = 0;
         bool ok = true;
         for (;; ++x) {
@@ -438,6 +449,25 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             const bool listed = alive && (e.rows[qx >> 5] >> (qx & 31) & 1u);
             const int n = listed ? min(kBlock, end - block * kBlock) : 0;   // keys of the row
             tc::tc_fence_after_sync();
+            if (kLong && x > 0 && x % kRun == 0) {   // this block's product, which begins anew, waits for this warp's weights
+                ok = __all_sync(~0u, wait(base + M::kPv + 8 * ((x - 1) & 1), ((x - 1) >> 1) & 1, abort_flag));
+                if (!ok) break;
+                tc::tc_fence_after_sync();
+                const float shrink = aside_scale();
+#pragma unroll 1
+                for (int k = half * (DP / 2); k < (half + 1) * (DP / 2); k += 32) {
+                    uint32_t o[32], before[32];
+                    tc::tmem_ld_x32(mine + 128 + k, o);
+                    if (x > kRun) {
+                        tc::tmem_ld_x32(mine + 128 + DP + k, before);
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(fmaf(__uint_as_float(before[y]), shrink, __uint_as_float(o[y])));
+                    }
+                    tc::tmem_st_x32(mine + 128 + DP + k, o);
+                }
+                tc::tmem_st_wait();
+                aside_top = top;
+            }
             uint32_t u[32];
             tc::tmem_ld_x32(mine + (x & 1) * 64 + 32 * half, u);
             if (__any_sync(~0u, n > 0 && n < kBlock)) {   // a block that ends inside: the queries' own, mostly
@@ -504,6 +534,13 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
             auto result = [&](int g, float (&f)[32]) {
                 uint32_t o[32];
                 if (x > 0) tc::tmem_ld_x32(mine + 128 + half * (DP / 2) + 32 * g, o);
+                if (kLong && x > kRun) {
+                    const float shrink = aside_scale();
+                    uint32_t before[32];
+                    tc::tmem_ld_x32(mine + 128 + DP + half * (DP / 2) + 32 * g, before);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(fmaf(__uint_as_float(before[y]), shrink, __uint_as_float(o[y])));
+                }
 #pragma unroll
                 for (int y = 0; y < 32; ++y) f[y] = x > 0 && alive && total != 0.f ? __uint_as_float(o[y]) * inv : 0.f;
             };
@@ -540,7 +577,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) forward_kernel(const Args 
     }
     if (warp == 9) {
         tc::tc_fence_after_sync();
-        tc::tmem_dealloc(tmem, 256);
+        tc::tmem_dealloc(tmem, M::kColumns);
     }
 }
 
@@ -810,10 +847,8 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
 // tiles above 837 us, 0.71 PFLOP/s on them (938 with four places, one group and one wait after another).  A block that most later queries have listed (up to 392
 // tiles there, 138 on average) is one CTA's work and starts first.
 //
-// Sums in tensor memory are cut off, not rounded: one whose terms have one sign loses some 1.6 x 2^-23 of itself in every step (8 to a tile), 7.9e-4 of dV by 1024 tiles and
-// 4.6 % by 60 000.  So after kRun tiles the first group puts them aside, where they are added in fp32, and they begin anew: 2.0e-4 however many there are, less than half of
-// fp16's own rounding.  The tiles above take 17 us more with it; runs of 128 lose 1.0e-4 and take 57.
-constexpr uint32_t kRun = 256;
+// After kRun tiles the first group puts the sums aside, in the workspace, where they are added in fp32: without it dV was 7.9e-4 too small by 1024 tiles and 4.6 % by 60 000, with it
+// 2.0e-4 however many there are.  The tiles above take 17 us more; runs of 128 lose 1.0e-4 and take 57.
 template <int DP> struct GradKVSmem {
     static constexpr int kBuffers = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;   // of S and dP; CTAs an SM
     // Q and dO of tile x are copies 2 x and 2 x + 1, copy n in place n % kPlaces; d <= 64: always Q in an even one, dO behind it
