@@ -565,3 +565,40 @@ def test_long_lists_of_unlike_rows(dtype, D):
             some = rng.permutation(np.arange(lo, hi))[:320 if i % 3 else 300]
             blocks[0, h, i, :len(some)] = some
     check(dtype, q, k, v, torch.from_numpy(blocks).to(DEV), D ** -0.5, False, None, grad)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("count", [256, 257, 513, 1025, 16000])
+def test_query_gradients_of_long_lists(D, count):
+    """Values that are the keys: a gradient of q is grad_out times the keys' covariance, a sum whose terms agree in sign.  With M the largest sum on the way: cut off by
+    less than 2^-21 M in each of 8 steps to a block, 256 blocks at a stretch: 2^-10 M.  A result of forward is off by up to 2^-11 of its terms' magnitudes (as above), and
+    rowsum(out o grad_out) with it: scale times that times the sum of weight times key.  fp32 besides: 2^-18 of all magnitudes.  The scores' gradients go in as two words of fp16.
+
+    The gradient's part along the exact one is a sum over all elements, in which fp32 noise and the result's rounding have no sign: there 2^-18 of the sum is left of the former,
+    and u, all of its rounding if it had one, of the latter."""
+    g = torch.Generator(DEV).manual_seed(count + D)
+    q, k, grad = (torch.randn(s, generator=g, device=DEV) for s in ((1, 70, 2, D), (1, 64 * count, 1, D), (1, 70, 2, D)))
+    q, k, grad = q.mul_(0.25).half(), k.half(), grad.half()
+    blocks = torch.arange(count, dtype=torch.int32, device=DEV).expand(1, 1, 70, count).contiguous()
+    x, scale = q.clone().requires_grad_(), D ** -0.5
+    got, = torch.autograd.grad(torch_ops.selected_attention(x, k, k, blocks, scale, False), x, grad)
+    assert ops.device_status() == 0
+    u, k64 = torch.finfo(torch.float16).eps / 2, k[0, :, 0].double()
+    along = allowed = square = 0.0
+    for i in range(0, 70, 3):
+        p = (q[0, i].double() @ k64.T * scale).softmax(-1)
+        d = grad[0, i].double()
+        dp = d @ k64.T
+        delta = (p * dp).sum(-1, keepdim=True)
+        ds = (p * (dp - delta) * scale).view(2, count, 64)
+        parts = torch.einsum("hnt,ntd->hnd", ds, k64.view(count, 64, D))
+        want, most = parts.sum(1), parts.cumsum(1).abs().amax(1)
+        sizes = p * (d.abs() @ k64.abs().T + (p * (d.abs() @ k64.abs().T)).sum(-1, keepdim=True)) * scale
+        wrong_delta = (d.abs() * (p @ k64.abs())).sum(-1, keepdim=True) * 2.0 ** -11
+        bound = 2.0 ** -10 * most + scale * wrong_delta * (p @ k64).abs() + 2.0 ** -18 * (sizes @ k64.abs()) + u * want.abs() + 2.0 ** -24
+        off = got[0, i].double() - want
+        assert (off.abs() <= bound).all(), i
+        along += (off * want).sum().item()
+        square += (want ** 2).sum().item()
+        allowed += (want.abs() * (2.0 ** -10 * most + scale * wrong_delta * (p @ k64).abs() + (u + 2.0 ** -18) * want.abs())).sum().item()
+    assert abs(along) <= allowed, (along / square, allowed / square)

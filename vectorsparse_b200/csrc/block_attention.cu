@@ -200,6 +200,9 @@ inline bool few(const blocks::Shape &s) {
     return (int64_t)s.batch * s.queries * s.heads <= 64 && (int64_t)s.batch * s.queries * s.heads * std::min<int64_t>(s.keys, (int64_t)s.count * blocks::kBlock) <= 64;
 }
 
+// Lists that can hold more blocks than are summed at a stretch.
+inline bool long_lists(const blocks::Shape &s) { return std::min(s.count, s.blocks) > (int)blocks::tcore::kRun; }
+
 template <typename T, int DP, bool kLong> int forward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
     const blocks::Shape &s = a.s;
     using Smem = blocks::tcore::ForwardSmem<DP, kLong>;
@@ -227,12 +230,12 @@ template <typename T> int attention(blocks::Args a, uint32_t *redo, cudaStream_t
     uint32_t *status = nullptr;
     const int rc = current_device(&sms, &status);
     if (rc != VS_OK) return rc;
-    if (std::min(s.count, s.blocks) > (int)blocks::tcore::kRun) return s.d <= 64 ? forward<T, 64, true>(a, redo, status, st) : forward<T, 128, true>(a, redo, status, st);
+    if (long_lists(s)) return s.d <= 64 ? forward<T, 64, true>(a, redo, status, st) : forward<T, 128, true>(a, redo, status, st);
     return s.d <= 64 ? forward<T, 64, false>(a, redo, status, st) : forward<T, 128, false>(a, redo, status, st);
 }
-template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
+template <typename T, int DP, bool kLong> int backward(blocks::Args a, uint32_t *redo, uint32_t *status, cudaStream_t st) {
     const blocks::Shape &s = a.s;
-    using SmemQ = blocks::tcore::GradQSmem<DP>;
+    using SmemQ = blocks::tcore::GradQSmem<DP, kLong>;
     using SmemKV = blocks::tcore::GradKVSmem<DP>;
     CUtensorMap q, g, k, v;
     a.tile = tile_queries(s.group);
@@ -240,7 +243,7 @@ template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint3
     if (rc == VS_OK) rc = make_map<T>(&g, a.grad_out, s.batch, s.queries, s.heads, s.d, s.group, a.tile);
     if (rc == VS_OK) rc = make_map<T>(&k, a.k, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
     if (rc == VS_OK) rc = make_map<T>(&v, a.v, s.batch, s.keys, s.kv_heads, s.d, 1, blocks::kBlock);
-    if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_q_kernel<T, DP>>(SmemQ::kBytes);
+    if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_q_kernel<T, DP, kLong>>(SmemQ::kBytes);
     if (rc == VS_OK) rc = allow_smem<blocks::tcore::grad_kv_kernel<T, DP>>(SmemKV::kBytes);
     if (rc != VS_OK) return rc;
     const int64_t rows = (int64_t)s.batch * s.queries * s.heads, tiles = query_tiles(s), blocks_all = (int64_t)s.batch * s.kv_heads * s.blocks;
@@ -249,7 +252,7 @@ template <typename T, int DP> int backward(blocks::Args a, uint32_t *redo, uint3
     if (std::is_same<T, __half>::value && e == cudaSuccess)
         e = launch_behind(blocks::peaks_kernel, (unsigned)((int64_t)s.batch * s.kv_heads * s.words), blocks::kBitsThreads, 0, st, a);
     if (e == cudaSuccess)
-        e = launch_behind(blocks::tcore::grad_q_kernel<T, DP>, (unsigned)tiles, blocks::tcore::kGradQThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
+        e = launch_behind(blocks::tcore::grad_q_kernel<T, DP, kLong>, (unsigned)tiles, blocks::tcore::kGradQThreads, SmemQ::kBytes, st, a, q, g, k, v, redo, status);
     if (e == cudaSuccess)
         e = launch_behind(blocks::tcore::grad_kv_kernel<T, DP>, (unsigned)blocks_all, SmemKV::kThreads, SmemKV::kBytes, st, a, q, g, k, v, redo_kv, status);
     if (e != cudaSuccess) return (int)e;
@@ -272,7 +275,8 @@ template <typename T> int attention_backward(blocks::Args a, uint32_t *redo, cud
         if (e == cudaSuccess) e = launch_behind(blocks::keys_kernel<T>, again_grid((int64_t)a.s.batch * a.s.kv_heads * a.s.blocks), blocks::kRowThreads, 0, st, a);
         return (int)e;
     }
-    return a.s.d <= 64 ? backward<T, 64>(a, redo, status, st) : backward<T, 128>(a, redo, status, st);
+    if (long_lists(a.s)) return a.s.d <= 64 ? backward<T, 64, true>(a, redo, status, st) : backward<T, 128, true>(a, redo, status, st);
+    return a.s.d <= 64 ? backward<T, 64, false>(a, redo, status, st) : backward<T, 128, false>(a, redo, status, st);
 }
 
 inline bool scale_ok(float scale) { return scale > 0.f && std::isfinite(scale); }

@@ -601,22 +601,26 @@ __device__ __forceinline__ float exp2i(float e) { return __uint_as_float((uint32
 // next ones are needed.  256 columns of tensor memory, 113 KB of shared memory (d = 128): two CTAs an SM, one's products under the other's exponentials.
 // Bound by its chain of products and softmax, single buffered: 8192 x 8192, 32 heads on 4, d = 128, 16 blocks each, 70 900 tiles of 128 x 64: 531 us
 // (476 without the second word).
-template <int DP> struct GradQSmem {
+// kLong: as in forward, dQ put aside every kRun blocks: without it sums of one sign were 9.8e-4 too small by 8000 blocks and 1.8e-3 by 16000, with it 4e-5.  The backward pass of the
+// queries named there: d = 128 3310 us (3235 without), d = 64 2530 (2500).
+template <int DP, bool kLong> struct GradQSmem {
     static constexpr int kSlotBytes = kBlock * DP * 2, kQBytes = kRows * DP * 2;
-    static constexpr int kQ = 1024, kG = kQ + kQBytes, kK = kG + kQBytes, kV = kK + 2 * kSlotBytes, kBytes = kV + kSlotBytes;
+    static constexpr int kQ = 1024, kG = kQ + kQBytes, kK = kG + kQBytes, kV = kK + 2 * kSlotBytes, kUsed = kV + kSlotBytes;
+    static constexpr uint32_t kColumns = kLong && DP == 128 ? 512 : 256;   // of tensor memory: S, dP, dQ, and what is put aside
+    static constexpr int kBytes = kColumns > 256 ? 120 * 1024 : kUsed;
     static constexpr int kBars = kEntries * sizeof(Entry);
     static constexpr int kBarQ = kBars, kKFull = kBarQ + 8, kKEmpty = kKFull + 16, kVFull = kKEmpty + 16, kVEmpty = kVFull + 8, kSP = kVEmpty + 8, kDs = kSP + 8, kDq = kDs + 8,
                          kE = kDq + 8, kDrain = kE + 8 * kEntries, kAbort = kDrain + 8, kHolder = kAbort + 4;
     static constexpr int kChunk = 512;
     static_assert(kHolder + 4 <= kChunk, "head");
-    static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs an SM");
+    static_assert(2 * (kUsed + 1024) <= 228 * 1024 && kUsed <= kBytes && (kColumns > 256) == (2 * (kBytes + 1024) > 228 * 1024), "two CTAs an SM, or one");
 };
 constexpr int kGradQThreads = 320;
-template <typename T, int DP>
+template <typename T, int DP, bool kLong>
 __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
                                                                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, uint32_t *redo,
                                                                     uint32_t *status) {
-    using M = GradQSmem<DP>;
+    using M = GradQSmem<DP, kLong>;
     extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t base = tc::smem_u32(sm);
     const Shape &s = a.s;
@@ -638,7 +642,7 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
         tc::fence_mbar_init();
     }
     if (warp == 9) {
-        tc::tmem_alloc(base + M::kHolder, 256);
+        tc::tmem_alloc(base + M::kHolder, M::kColumns);
         tc::tmem_relinquish();
     }
     tc::tc_fence_before_sync();
@@ -731,7 +735,7 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
             if (leader) {
 #pragma unroll
                 for (int k = 0; k < kBlock / 16; ++k)
-                    tc::mma_f16_ts(tmem + 128, tmem + 8 * k, tc::desc64(kt_lo + at + 128 * k, hi), kIdescQ, x > 0 || k > 0);
+                    tc::mma_f16_ts(tmem + 128, tmem + 8 * k, tc::desc64(kt_lo + at + 128 * k, hi), kIdescQ, (kLong ? x % kRun : x) > 0 || k > 0);
 #pragma unroll
                 for (int k = 0; k < kBlock / 16; ++k)   // what the rounding of dS left over
                     tc::mma_f16_ts(tmem + 128, tmem + 32 + 8 * k, tc::desc64(kt_lo + at + 128 * k, hi), kIdescQ, true);
@@ -772,6 +776,20 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
             ok = __all_sync(~0u, wait(base + M::kSP, x & 1, abort_flag));
             if (!ok) break;
             tc::tc_fence_after_sync();
+            if (kLong && x > 0 && x % kRun == 0) {   // the scores have been issued behind the end of the products before
+#pragma unroll 1
+                for (int k = half * (DP / 2); k < (half + 1) * (DP / 2); k += 32) {
+                    uint32_t o[32], before[32];
+                    tc::tmem_ld_x32(mine + 128 + k, o);
+                    if (x > kRun) {
+                        tc::tmem_ld_x32(mine + 128 + DP + k, before);
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) + __uint_as_float(before[y]));
+                    }
+                    tc::tmem_st_x32(mine + 128 + DP + k, o);
+                }
+                tc::tmem_st_wait();
+            }
             const bool whole = __all_sync(~0u, n <= 0 || n == kBlock);
             const float off = n > 0 ? -lse : -INFINITY;   // a row that has not listed the block has no weight there
             uint32_t u[32], d[32], ds[16], low[16];
@@ -813,6 +831,12 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
                 uint32_t o[32];
                 float f[32];
                 if (x > 0) tc::tmem_ld_x32(mine + 128 + half * (DP / 2) + 32 * g, o);
+                if (kLong && x > kRun) {
+                    uint32_t before[32];
+                    tc::tmem_ld_x32(mine + 128 + DP + half * (DP / 2) + 32 * g, before);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) + __uint_as_float(before[y]));
+                }
 #pragma unroll
                 for (int y = 0; y < 32; ++y) {
                     f[y] = x > 0 && alive ? __uint_as_float(o[y]) * back : 0.f;
@@ -832,7 +856,7 @@ __global__ void __launch_bounds__(kGradQThreads, 2) grad_q_kernel(const Args a, 
     }
     if (warp == 9) {
         tc::tc_fence_after_sync();
-        tc::tmem_dealloc(tmem, 256);
+        tc::tmem_dealloc(tmem, M::kColumns);
     }
 }
 
