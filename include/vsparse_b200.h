@@ -296,6 +296,9 @@ int vs_device_status(int clear, uint32_t *status);
  * are rounded to the type for the product with v, as are they and the scores' gradients in the backward pass (for q's gradient the latter in two
  * words); a handful of rows and keys is computed in fp32 throughout.  fp16: the scores' gradients are multiplied by a power of two before they are rounded, one that fits the largest
  * finite element of grad_out in the row (for q), or in the rows that have listed the block (for k), so that small gradients keep their bits whatever stands in other rows.
+ * What is not finite (padding that holds NaN, one Inf in v) costs time where tiles meet it, some 50 times a tile's; zeros behind a sequence's end do not.
+ * The workspace holds a bit for each query and block of keys of each head of keys, and for the gradients of long sequences 512 x d bytes (d rounded
+ * up to 64 or 128) for each block.
  *
  * vs_selected_attention_backward: gradients of q, k and v (all three written whole) for grad_out; the gradients of a head of keys are summed over its group,
  * in the same order in every call.  Both take a workspace of vs_selected_attention_workspace_bytes(..., backward).

@@ -194,7 +194,7 @@ inline int64_t query_tiles(const blocks::Shape &s) {
 }
 inline unsigned again_grid(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 4 * 148); }
 
-// A handful of products: the row kernels alone, in fp32 throughout.  Nothing averages the 16-bit roundings of a tile's weights there, and it is no slower: 5 rows of 4 keys 8.4
+// A handful of products, a prompt's first tokens: the row kernels alone, in fp32 throughout.  Nothing averages the 16-bit roundings of a tile's weights there, and it is no slower: 5 rows of 4 keys 8.4
 // us and 21.1 backward against 8.2 and 21.6 by tiles, 32 rows of 2 keys 6.0 and 10.5 against 7.2 and 16.7; 64 rows of 8 keys 22 and 23 against 6.9 and 15.3.
 inline bool few(const blocks::Shape &s) {
     return (int64_t)s.batch * s.queries * s.heads <= 64 && (int64_t)s.batch * s.queries * s.heads * std::min<int64_t>(s.keys, (int64_t)s.count * blocks::kBlock) <= 64;

@@ -196,8 +196,8 @@ __device__ __forceinline__ void write_list(const uint32_t *taken, int words, int
 // choice is that of 64 bits.  Where they do not, the scores from 2 E below the last one on are computed again in 64.
 // Two kernels, over slabs of queries whose scores stay in L2: a product of the queries' sums with the means, and a ranking by a warp per query, which needs many warps
 // to cover what it waits for and would not have them beside the product's tiles (in one kernel, with 16 warps an SM: 212 us at 16384 x 16384, 4 heads of keys,
-// d = 128; fp64 throughout, as below: 525).  Now the product takes 73, bound by fp32 arithmetic and its shared memory, and the ranking 112, bound by instructions;
-// with the means and the launches 243.
+// d = 128; fp64 throughout, as below: 525).  Now the product takes 76, bound by fp32 arithmetic and its shared memory, and the ranking 115, bound by instructions;
+// with the means and the launches 245.  Queries with more than kMembers candidates that are all alike fall out of it: 4096 queries, 2 heads on one, 1024 blocks of zeros 120 ms against 0.53.
 constexpr int kFastThreads = 256, kFastQueries = 64, kFastBlocks = 128, kFastPiece = 64, kFastPitch = kFastPiece + 4, kMembers = 256, kFastCount = 128;
 constexpr int kFastMost = 1024;   // blocks of a sequence
 __host__ __device__ constexpr int fast_pitch(int d) { return (d + 63) / 64 * 64 + 4; }

@@ -207,7 +207,8 @@ template <typename T> __global__ void __launch_bounds__(kAppendThreads, 12) appe
 // ---- choosing blocks for single tokens --------------------------------------------------------------------------------
 // Score of a complete block: (sum of the group's query heads) . (sum of the block's codes) * scale, in 64 bits.  The newest complete block is always
 // taken.  A CTA per (sequence, kv head); 16 lanes take a block's sums, 8 dimensions each, four blocks in flight.  Bound by 64-bit products and the sums over
-// lanes, then by the ranking: 64 sequences of up to 256 blocks, 8 heads, d = 128: 22 us (26 MB, 1.2 TB/s).
+// lanes, then by the ranking: 64 sequences of up to 256 blocks, 8 heads, d = 128: 20 us (26 MB, 1.3 TB/s;
+// 23 where nothing of them is in L2).
 constexpr int kSelectThreads = 1024;   // at most
 struct SelectArgs {
     Pages c;
